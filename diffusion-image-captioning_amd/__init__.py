@@ -9,6 +9,9 @@ Public surface = the reference's hot-path callables (ref CLIP-DDPM.py, SURVEY.md
     DistilBertModel          denoiser wrapper (alias of engine.Denoiser)
     AdamW                    fused optimizer with torch.optim.AdamW's interface
     diffuse_t, generate_diffuse_pair, loss, train_func, validate, sample
+and, for denoisers over longer token rows than the reference's (block.py):
+    window_attention, window_attention_grad     attention in a sliding window with first keys that stay visible
+    gated_norm, gated_norm_grad, NormParams     the norms around a block with its gate and the residual scale
 Importing the package works without a GPU (host logic, synthetic data); constructing a model or calling an op
 without the built HIP library / a visible MI355X raises RuntimeError -- there is no CPU fallback.
 """
@@ -34,6 +37,9 @@ def __getattr__(name):
     if name == "GraphedTrainStep":
         from .graph import GraphedTrainStep
         return GraphedTrainStep
+    if name in ("window_attention", "window_attention_grad", "gated_norm", "gated_norm_grad", "NormParams"):
+        from . import block
+        return getattr(block, name)
     if name in ("bleu", "harness"):
         import importlib
         return importlib.import_module(f"{__name__}.{name}")

@@ -13,7 +13,11 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB_PATH = os.path.join(HERE, "libdic_hip.so")
 _AB_LIB = os.environ.get("DIC_HIP_LIB")      # measurement aid: load another build of the same library for within-run A/B timing
-SOURCES = ["gemm.hip", "attn.hip", "norm.hip", "misc.hip"]
+SOURCES = ["gemm.hip", "attn.hip", "norm.hip", "misc.hip", "wattn.hip", "gnorm.hip"]
+# Packed fp32 instructions off: some of their forms have given wrong results now and then.  gemm.hip holds them in its generated assembly text, which the
+# assembler would refuse under this feature setting.
+NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+NO_PACKED_F32_SOURCES = ("wattn.hip", "gnorm.hip")
 
 DIC_F32, DIC_BF16 = 0, 1
 ABI_VERSION = 19          # include/dic_hip.h DIC_HIP_VERSION the struct mirrors / argtypes below were written for; lib() refuses any other library
@@ -28,6 +32,7 @@ EXPORTS = [
     "dic_te_dx0", "dic_embed_scatter", "dic_temb_grad", "dic_step_prep", "dic_randint", "dic_zero", "dic_wgrad_group", "dic_wgrad_group_ws_bytes",
     "dic_gemm_set_variant", "dic_fuse_ln_fwd_x", "dic_cfg_prep", "dic_step_ctx_set", "dic_step_advance",
     "dic_lin_prep", "dic_lin_prep_ws_bytes", "dic_ln_fwd_cen", "dic_ln_bwd_cen", "dic_set_option", "dic_rank1_add",
+    "dic_win_attn_fwd", "dic_win_attn_bwd", "dic_win_attn_ws_bytes", "dic_gated_norm_fwd", "dic_gated_norm_bwd", "dic_gated_norm_ws_bytes",
 ]
 
 
@@ -57,6 +62,23 @@ class WgradItem(C.Structure):
                 ("M", C.c_int), ("N", C.c_int)]
 
 
+class WinAttnParams(C.Structure):
+    """Mirror of DicWinAttnParams (include/dic_hip.h); a DicStrides member is three int64 in a row."""
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "out", "lse", "dout", "dq", "dk", "dv")] + [
+        (f"{n}_stride_{d}", C.c_int64) for n in ("q", "k", "v", "out", "dout", "dq", "dk", "dv") for d in "nth"] + [
+        ("key_mask", C.c_void_p), ("kv_len", C.c_void_p), ("q_pos", C.c_void_p),
+        ("N", C.c_int), ("Tq", C.c_int), ("Tk", C.c_int), ("H", C.c_int), ("Hkv", C.c_int), ("dh", C.c_int),
+        ("left", C.c_int), ("right", C.c_int), ("sinks", C.c_int), ("scale", C.c_float), ("ws", C.c_void_p), ("ws_bytes", C.c_size_t)]
+
+
+class GatedNormParams(C.Structure):
+    """Mirror of DicGatedNormParams (include/dic_hip.h); a DicNorm member is weight, bias, kind, eps."""
+    _fields_ = [(n, C.c_void_p) for n in ("x", "y", "x_new", "a", "gate", "saved", "dx_new", "da", "dx", "dy", "dgate", "dpost_w", "dpost_b", "dpre_w", "dpre_b",
+                                          "post_weight", "post_bias")] + [
+        ("post_kind", C.c_int), ("post_eps", C.c_float), ("pre_weight", C.c_void_p), ("pre_bias", C.c_void_p), ("pre_kind", C.c_int), ("pre_eps", C.c_float),
+        ("rows", C.c_int64), ("rows_per_gate", C.c_int64), ("D", C.c_int), ("residual_scale", C.c_float), ("ws", C.c_void_p), ("ws_bytes", C.c_size_t)]
+
+
 LAST_BUILD = None        # "compiled" | "reused": what the last build() call did (printed by __graft_entry__.build)
 
 
@@ -81,6 +103,8 @@ def build(verbose: bool = False, force: bool = False) -> str:
             # q_sample must round a*x, eps*b and their sum separately to be bit-exact with the reference (ref :360-362);
             # everything in misc.hip is HBM-bound, so no FMA contraction in this file costs nothing
             cmd.insert(3, "-ffp-contract=off")
+        if os.path.basename(s) in NO_PACKED_F32_SOURCES:
+            cmd[3:3] = NO_PACKED_F32
         procs.append((cmd, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)))
     for cmd, p in procs:
         out, _ = p.communicate()
@@ -174,6 +198,14 @@ def lib():
         L.dic_adamw_hl.argtypes = [P, P, P, P, P, P, I64, F, F, F, F, F, F, F, F, P]
         L.dic_cast_bf16_hl.argtypes = [P, P, P, I64, P]
         L.dic_probe_tr16.argtypes = [P, P, P]
+        for fn in ("dic_win_attn_fwd", "dic_win_attn_bwd"):
+            getattr(L, fn).argtypes = [I, C.POINTER(WinAttnParams), P]
+        for fn in ("dic_gated_norm_fwd", "dic_gated_norm_bwd"):
+            getattr(L, fn).argtypes = [I, C.POINTER(GatedNormParams), P]
+        L.dic_win_attn_ws_bytes.argtypes = [I, I, C.POINTER(WinAttnParams)]
+        L.dic_win_attn_ws_bytes.restype = C.c_size_t
+        L.dic_gated_norm_ws_bytes.argtypes = [I, C.POINTER(GatedNormParams)]
+        L.dic_gated_norm_ws_bytes.restype = C.c_size_t
         L.dic_gemm_set_variant.argtypes = [I]
         L.dic_set_option.argtypes = [C.c_char_p, I]
         L.dic_gemm_set_w4a.argtypes = [I]

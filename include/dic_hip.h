@@ -289,6 +289,72 @@ int dic_attn_fwd(int dtype, const void* qkv, const uint8_t* key_mask, void* ctx,
 int dic_attn_bwd(int dtype, const void* qkv, const uint8_t* key_mask, const void* dctx, void* dqkv,
                  int N, int Tk, int H, int dh, float p_drop, uint64_t seed, void* stream);
 
+/* ---------------------------------------------------------------- attention over long token rows: a sliding window and first keys that stay visible
+ * (hf:136-147 beyond dic_attn's 64 tokens; the reference has no such mask).  q [N][Tq][H][dh], k and v [N][Tk][Hkv][dh], out like q, each with its own
+ * strides in elements (the dh elements of a row are contiguous; pointers and strides are multiples of 16 bytes); H = G Hkv, query head h reads key
+ * head h / G; dh 64 or 128.  Query row i of sequence n stands at position t = i + (q_pos ? q_pos[n] : 0).  It sees key j when
+ *     j < kv_len[n] (Tk without kv_len)   and   key_mask[n][j] != 0 (with key_mask [N][Tk])   and   j <= t + right (right >= 0)   and
+ *     (j >= t - left (left >= 0)  or  j < sinks);                      left / right < 0: no bound on that side.
+ * fwd: out = softmax(scale q k^T over the visible keys) v, lse [N][H][Tq] (optional) = the logarithm of the softmax's denominator.  A row that sees
+ *     nothing gets out = 0 and lse = -inf.  Keys behind kv_len or masked by key_mask are never read into a result, whatever their rows hold.
+ *     Sums, maxima and lse are fp32; with DIC_BF16 the probabilities are rounded to bf16 in front of the product with v.
+ * bwd: dq, dk, dv from dout and the forward's out and lse; every row is written (zeros where nothing is seen).  Deterministic, no atomics.
+ * kv_len is read as clamped to [0, Tk], q_pos to +-2^29.  ws: dic_win_attn_ws_bytes(dtype, backward, p) bytes, 16-byte aligned, private to the call
+ * until it has run; N, Tq or Tk may be 0.                                                                                                    */
+typedef struct DicStrides { int64_t n, t, h; } DicStrides;            /* elements between sequences, tokens, heads */
+typedef struct DicWinAttnParams {
+    const void *q, *k, *v;
+    void* out;                  /* written by fwd, read by bwd */
+    float* lse;                 /* fwd: written (or NULL); bwd: read */
+    const void* dout;           /* bwd only, as are dq, dk, dv */
+    void *dq, *dk, *dv;
+    DicStrides q_stride, k_stride, v_stride, out_stride, dout_stride, dq_stride, dk_stride, dv_stride;
+    const uint8_t* key_mask;    /* [N][Tk] or NULL */
+    const int32_t* kv_len;      /* [N] or NULL */
+    const int32_t* q_pos;       /* [N] or NULL */
+    int N, Tq, Tk, H, Hkv, dh;
+    int left, right, sinks;
+    float scale;                /* > 0 */
+    void* ws; size_t ws_bytes;
+} DicWinAttnParams;
+size_t dic_win_attn_ws_bytes(int dtype, int backward, const DicWinAttnParams* p);
+int dic_win_attn_fwd(int dtype, const DicWinAttnParams* p, void* stream);
+int dic_win_attn_bwd(int dtype, const DicWinAttnParams* p, void* stream);
+
+/* ---------------------------------------------------------------- the norms around a block, its gate and the residual scale, in one pass
+ *     n = post(y),   x_new = residual_scale x + gate n,   a = pre(x_new)
+ * y [rows][D] is a block's output, x the residual stream in front of the block, x_new the stream behind it and a the next block's input (hf:236, 253 keep
+ * one norm BEHIND each sum; this is the form with norms on both sides and a gate, as a stream that is conditioned on the timestep needs).  post / pre:
+ * DIC_NORM_LAYER (x - mean) rstd w + b, DIC_NORM_RMS x rstd w + b, DIC_NORM_NONE; weight and bias [D] fp32, each may be NULL (1 and 0).  gate [rows /
+ * rows_per_gate][D] fp32, one row for every rows_per_gate consecutive rows, or NULL (1).  y NULL: a = pre(residual_scale x), the first norm of a stack
+ * (no gate, post NONE, x_new optional).  pre NONE: no a.  D <= 8192, rows contiguous, any alignment of whole elements.
+ * saved [4][rows] fp32: mean and rstd of post, mean and rstd of pre (zeros where that norm is NONE; a mean is 0 under RMS); fwd writes, bwd reads.
+ * dtype: DIC_F32, DIC_BF16, or DIC_BF16 | DIC_RES_F32 (x, x_new, dx_new, dx fp32, the rest bf16).  All arithmetic is fp32; a and its statistics come
+ * from the unrounded x_new.
+ * bwd, from dx_new (NULL: zero) and da (with pre):  d = dx_new + pre'(da),  dx = residual_scale d,  dy = post'(gate d),  and, each optional, dgate (like
+ * gate), dpost_w, dpost_b, dpre_w, dpre_b [D] fp32.  Deterministic.  ws: dic_gated_norm_ws_bytes(dtype, p) bytes, 16-byte aligned.             */
+#define DIC_NORM_NONE 0
+#define DIC_NORM_LAYER 1
+#define DIC_NORM_RMS 2
+typedef struct DicNorm { const float *weight, *bias; int kind; float eps; } DicNorm;
+typedef struct DicGatedNormParams {
+    const void *x, *y;
+    void *x_new, *a;            /* bwd reads x_new (needed when pre is not NONE) */
+    const float* gate;
+    float* saved;
+    const void *dx_new, *da;
+    void *dx, *dy;
+    float *dgate, *dpost_w, *dpost_b, *dpre_w, *dpre_b;
+    DicNorm post, pre;
+    int64_t rows, rows_per_gate;
+    int D;
+    float residual_scale;
+    void* ws; size_t ws_bytes;
+} DicGatedNormParams;
+size_t dic_gated_norm_ws_bytes(int dtype, const DicGatedNormParams* p);
+int dic_gated_norm_fwd(int dtype, const DicGatedNormParams* p, void* stream);
+int dic_gated_norm_bwd(int dtype, const DicGatedNormParams* p, void* stream);
+
 /* ---------------------------------------------------------------- TRAIN_EMBEDDING ablation (ref:98-102, 238-243, 459-468)
  * dic_te_dx0: gradient wrt the learned embedding rows x_0 [B][L][C] gathered for this batch: through q_sample into the S noised
  *   copies and the x_1 copy (dxin [S*B+B][Tk][C], rows t<L), and as the target of both embedding losses (g, same shape).

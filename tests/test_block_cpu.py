@@ -1,0 +1,106 @@
+"""C entries of the windowed attention and the gated norms without a GPU: struct layouts, workspace sizes, and what they refuse before any launch."""
+import ctypes as C
+import importlib
+import os
+import re
+
+import pytest
+
+dic = importlib.import_module("diffusion-image-captioning_amd")
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+CTYPES = {"int": C.c_int, "float": C.c_float, "size_t": C.c_size_t, "int64_t": C.c_int64}
+
+
+def header_fields(name):
+    src = re.sub(r"/\*.*?\*/", "", open(os.path.join(ROOT, "include", "dic_hip.h")).read(), flags=re.S)
+    body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), src, re.S).group(1)
+    fields = []
+    for decl in filter(None, (d.strip() for d in body.split(";"))):
+        kind, names = re.match(r"(?:const\s+)?(\w+)\s*(.*)", decl, re.S).groups()
+        for n in names.split(","):
+            n = n.strip()
+            fields.append((n.lstrip("* "), "ptr" if n.startswith("*") else kind))
+    return fields
+
+
+@pytest.mark.parametrize("struct,mirror", [("DicWinAttnParams", "WinAttnParams"), ("DicGatedNormParams", "GatedNormParams")])
+def test_struct_mirrors_follow_the_header(struct, mirror):
+    want = []
+    for name, kind in header_fields(struct):
+        if kind == "DicStrides":
+            want += [(f"{name}_{d}", C.c_int64) for d, _ in header_fields("DicStrides")]
+        elif kind == "DicNorm":
+            want += [(f"{name}_{d}", C.c_void_p if k == "ptr" else CTYPES[k]) for d, k in header_fields("DicNorm")]
+        else:
+            want.append((name, C.c_void_p if kind == "ptr" else CTYPES[kind]))
+    assert getattr(dic._lib, mirror)._fields_ == want
+
+
+def attn(**kw):
+    p = dic._lib.WinAttnParams()
+    base = dict(N=2, Tq=8, Tk=8, H=4, Hkv=2, dh=64, left=-1, right=-1, scale=0.125, ws=4096, ws_bytes=1 << 20)
+    base.update({n: 4096 for n in ("q", "k", "v", "out", "lse", "dout", "dq", "dk", "dv")})
+    for n in ("q", "out", "dout", "dq"):
+        base.update({f"{n}_stride_n": 8 * 256, f"{n}_stride_t": 256, f"{n}_stride_h": 64})
+    for n in ("k", "v", "dk", "dv"):
+        base.update({f"{n}_stride_n": 8 * 128, f"{n}_stride_t": 128, f"{n}_stride_h": 64})
+    for k, v in {**base, **kw}.items():
+        setattr(p, k, v)
+    return p
+
+
+BAD_ATTENTION = [
+    dict(dh=65), dict(dh=32), dict(H=3), dict(Hkv=0), dict(H=0), dict(N=-1), dict(Tq=-1), dict(Tk=-5), dict(Tq=1 << 30), dict(sinks=-1), dict(scale=0.0), dict(scale=float("nan")),
+    dict(scale=float("inf")), dict(q=None), dict(k=None), dict(v=None), dict(out=None), dict(q=4098), dict(v=4104), dict(k_stride_t=130), dict(q_stride_h=-64),
+    dict(v_stride_t=1 << 24), dict(out_stride_t=0), dict(N=1 << 20, H=4096, Hkv=2),
+]
+
+
+@pytest.mark.parametrize("kw", BAD_ATTENTION, ids=str)
+def test_attention_refuses(kw):
+    L, p = dic.lib(), attn(**kw)
+    backward = {k: ({"out": "dq", "out_stride_t": "dq_stride_t"}.get(k, k)) for k in kw}
+    assert L.dic_win_attn_fwd(1, C.byref(p), None) == 1001 and L.dic_last_error().startswith(b"dic_win_attn")
+    assert L.dic_win_attn_bwd(1, C.byref(attn(**{backward[k]: v for k, v in kw.items()})), None) == 1001
+
+
+def test_attention_refuses_other_types_and_missing_workspaces():
+    L = dic.lib()
+    for dtype in (-1, 2, 0x201):
+        assert L.dic_win_attn_fwd(dtype, C.byref(attn()), None) == 1001
+    assert L.dic_win_attn_fwd(1, None, None) == 1001
+    size = L.dic_win_attn_ws_bytes(1, 1, C.byref(attn()))
+    assert size >= 2 * 2 * 4 * 8 * 4
+    for kw in (dict(ws=None), dict(ws_bytes=size - 1), dict(ws=4100), dict(lse=None), dict(dout=None), dict(dk=None), dict(dk_stride_t=0)):
+        assert L.dic_win_attn_bwd(1, C.byref(attn(**kw)), None) == 1001, kw
+    assert L.dic_win_attn_ws_bytes(1, 1, C.byref(attn(dh=65))) == 0
+
+
+def norms(**kw):
+    p = dic._lib.GatedNormParams()
+    base = dict(rows=8, rows_per_gate=4, D=96, residual_scale=1.0, post_kind=1, pre_kind=2, post_eps=1e-6, pre_eps=1e-6, ws=4096, ws_bytes=1 << 20)
+    base.update({n: 4096 for n in ("x", "y", "x_new", "a", "gate", "saved", "dx_new", "da", "dx", "dy", "dgate", "dpost_w", "dpre_b")})
+    for k, v in {**base, **kw}.items():
+        setattr(p, k, v)
+    return p
+
+
+@pytest.mark.parametrize("kw", [dict(D=0), dict(D=8193), dict(rows=-1), dict(rows=7), dict(rows_per_gate=0), dict(post_kind=3), dict(pre_kind=-1), dict(post_eps=-1.0), dict(pre_eps=float("nan")),
+                                dict(post_kind=0, post_weight=4096), dict(residual_scale=float("inf")), dict(y=None)], ids=str)
+def test_norms_refuse(kw):
+    L = dic.lib()
+    assert L.dic_gated_norm_fwd(0, C.byref(norms(**kw)), None) == 1001 and L.dic_last_error().startswith(b"dic_gated_norm")
+    assert L.dic_gated_norm_bwd(0, C.byref(norms(**kw)), None) == 1001
+
+
+def test_norms_refuse_missing_pointers():
+    L = dic.lib()
+    for kw in (dict(x=None), dict(x_new=None), dict(a=None)):
+        assert L.dic_gated_norm_fwd(0, C.byref(norms(**kw)), None) == 1001, kw
+    size = L.dic_gated_norm_ws_bytes(0, C.byref(norms()))
+    assert size > 0
+    for kw in (dict(da=None), dict(x_new=None), dict(dx=None), dict(dy=None), dict(saved=None), dict(ws=None), dict(ws_bytes=size - 1), dict(gate=None), dict(pre_kind=0), dict(post_kind=0)):
+        assert L.dic_gated_norm_bwd(0, C.byref(norms(**kw)), None) == 1001, kw
+    for dtype in (-1, 2, 0x200):
+        assert L.dic_gated_norm_fwd(dtype, C.byref(norms()), None) == 1001
+    assert L.dic_gated_norm_fwd(0, None, None) == 1001
