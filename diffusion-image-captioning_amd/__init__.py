@@ -39,7 +39,8 @@ def __getattr__(name):
         return GraphedTrainStep
     if name in ("window_attention", "window_attention_grad", "gated_norm", "gated_norm_grad", "NormParams"):
         from . import block
-        return getattr(block, name)
+        globals()[name] = found = getattr(block, name)       # (from now on without this function)
+        return found
     if name in ("bleu", "harness"):
         import importlib
         return importlib.import_module(f"{__name__}.{name}")

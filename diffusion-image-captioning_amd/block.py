@@ -3,10 +3,11 @@ before and after a block with its gate and the residual scale (csrc/wattn.hip, c
 
 As everywhere in this package there is no autograd: each forward call has a call that computes its gradients, and a tensor that asks for a gradient is refused.
 Calls run on the current stream of the tensors' device, allocate what they return and their workspaces from torch's allocator, never synchronise, and can
-be captured into a graph.  Errors of the arguments raise ValueError or TypeError before anything is launched."""
+be captured into a graph.  Arguments that do not fit raise ValueError or TypeError before anything is launched."""
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from typing import NamedTuple, Optional
 
 import torch
@@ -15,17 +16,36 @@ from . import _lib
 
 _DTYPES = {torch.float32: _lib.DIC_F32, torch.bfloat16: _lib.DIC_BF16}
 _RES_F32 = 0x200
-_KINDS = {"none": 0, "layer": 1, "rms": 2}
-_INT = 2 ** 31 - 1
+_KINDS = {"layer": 1, "rms": 2}
+_FAR = 2 ** 31 - 1
+# The parameter structs as bytes: packing one takes a fifth of the time of filling its ctypes mirror, and a call on one caption is all host time.
+_WIN = struct.Struct("9P24q3P9if2P")
+_NORM = struct.Struct("17Pif2Pif2qif2P")
+_fns = {}
 
 
-def _ptr(t):
-    return None if t is None else t.data_ptr()
+def _fn(name):
+    """A C entry that takes its params as bytes."""
+    f = _fns.get(name)
+    if f is None:
+        f = _lib.lib()[name]
+        f.argtypes = [C.c_int, C.c_int, C.c_char_p] if name == "dic_win_attn_ws_bytes" else [C.c_int, C.c_char_p] if name.endswith("ws_bytes") else [C.c_int, C.c_char_p, C.c_void_p]
+        f.restype = C.c_size_t if name.endswith("ws_bytes") else C.c_int
+        _fns[name] = f
+    return f
 
 
-def _need(cond, what):
-    if not cond:
-        raise ValueError(what)
+def _launch(name, code, params, device):
+    """One C call on the current stream of `device`."""
+    stream = torch._C._cuda_getCurrentRawStream(device.index)        # (torch.cuda.current_stream(device) without building the object)
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            rc = _fn(name)(code, params, stream)
+    else:
+        rc = _fn(name)(code, params, stream)
+    if rc == 1001:
+        raise ValueError(_lib.lib().dic_last_error().decode(errors="replace"))
+    _lib.check(rc, name)
 
 
 def _on(t, like, name, dtypes, shape=None):
@@ -33,75 +53,73 @@ def _on(t, like, name, dtypes, shape=None):
         raise TypeError(f"{name} must be a tensor")
     if t.dtype not in dtypes:
         raise TypeError(f"{name}: {t.dtype} where {' or '.join(map(str, dtypes))} is needed")
-    _need(t.device == like.device, f"{name} is on {t.device}, not on {like.device}")
-    _need(shape is None or tuple(t.shape) == tuple(shape), f"{name} has shape {tuple(t.shape)}, not {shape and tuple(shape)}")
+    if not (t.device == like.device):
+        raise ValueError(f"{name} is on {t.device}, not on {like.device}")
+    if shape is not None and t.shape != shape:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, not {tuple(shape)}")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} asks for a gradient: this package has no autograd, call the operator's _grad function on detached tensors")
-    return t
 
 
-def _launch(fn, code, params, device, what):
-    """One C call on the current stream of `device`."""
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            return _lib.check(fn(code, C.byref(params), torch.cuda.current_stream().cuda_stream), what)
-    _lib.check(fn(code, C.byref(params), torch.cuda.current_stream().cuda_stream), what)
+def _ptr(t):
+    return 0 if t is None else t.data_ptr()
+
+
+def _first(t, name):
+    """What the other tensors are held against."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor")
+    if not t.is_cuda:
+        _lib.require_gpu()
+        raise ValueError(f"{name} must be on the GPU")
+    if t.dtype not in _DTYPES:
+        raise TypeError(f"{name}: {t.dtype} where torch.float32 or torch.bfloat16 is needed")
 
 
 # ------------------------------------------------------------------------------------------------ attention
 def _bound(x, name):
     if x is None:
         return -1
-    x = int(x)
-    _need(x >= 0, f"{name} must be None (no bound) or at least 0")
-    return min(x, _INT)
+    if not (x >= 0):
+        raise ValueError(f"{name} must be None (no bound) or at least 0")
+    return min(int(x), _FAR)
 
 
-def _attention(q, k, v, left, right, sinks, key_mask, kv_len, q_pos, scale, *rest):
-    """The checked arguments as a parameter struct (outputs and what the backward pass adds are filled in by the caller)."""
-    _lib.require_gpu()
-    if not isinstance(q, torch.Tensor) or q.dim() != 4:
-        raise ValueError("q must be a tensor [N, Tq, H, dh]")
-    _need(q.is_cuda, "q must be on the GPU")
-    types = (q.dtype,)
-    if q.dtype not in _DTYPES:
-        raise TypeError(f"q: {q.dtype} where float32 or bfloat16 is needed")
+def _check_rows(t, like, name, shape):
+    _on(t, like, name, (like.dtype,), shape)
+    if not (t.stride(3) == 1):
+        raise ValueError(f"the rows of {name} must be contiguous")
+
+
+def _attention(q, k, v, left, right, sinks, key_mask, kv_len, q_pos, scale):
+    """The checked arguments: (tail of the packed struct in front of the workspace, dtype code).  Strides and alignment are the C entry's to check."""
+    _first(q, "q")
+    if not (q.dim() == 4):
+        raise ValueError(f"q has shape {tuple(q.shape)}, not [N, Tq, H, dh]")
+    _check_rows(q, q, "q", q.shape)
     N, Tq, H, dh = q.shape
-    _on(q, q, "q", types)
-    _on(k, q, "k", types)
-    _need(k.dim() == 4 and k.shape[0] == N and k.shape[3] == dh, f"k has shape {tuple(k.shape)}, not [{N}, Tk, Hkv, {dh}]")
+    _on(k, q, "k", (q.dtype,))
+    if not (k.dim() == 4 and k.shape[0] == N and k.shape[3] == dh):
+        raise ValueError(f"k has shape {tuple(k.shape)}, not [{N}, Tk, Hkv, {dh}]")
+    _check_rows(k, q, "k", k.shape)
+    _check_rows(v, q, "v", k.shape)
     Tk, Hkv = k.shape[1], k.shape[2]
-    _on(v, q, "v", types, k.shape)
-    _need(dh in (64, 128), "the head dimension must be 64 or 128")
-    _need(Hkv > 0 and H % Hkv == 0 and H > 0, f"{H} query heads are no multiple of {Hkv} key heads")
     if key_mask is not None:
         _on(key_mask, q, "key_mask", (torch.bool, torch.uint8), (N, Tk))
-        _need(key_mask.is_contiguous(), "key_mask must be contiguous")
+        if not (key_mask.is_contiguous()):
+            raise ValueError("key_mask must be contiguous")
     for t, name in ((kv_len, "kv_len"), (q_pos, "q_pos")):
         if t is not None:
             _on(t, q, name, (torch.int32,), (N,))
-            _need(t.is_contiguous(), f"{name} must be contiguous")
-    p = _lib.WinAttnParams(q.data_ptr(), k.data_ptr(), v.data_ptr())
-    _strides(p, q=q, k=k, v=v)
-    p.key_mask, p.kv_len, p.q_pos = _ptr(key_mask), _ptr(kv_len), _ptr(q_pos)
-    p.N, p.Tq, p.Tk, p.H, p.Hkv, p.dh = N, Tq, Tk, H, Hkv, dh
-    p.left, p.right, p.sinks = _bound(left, "left"), _bound(right, "right"), _bound(sinks, "sinks") if sinks is not None else 0
-    p.scale = dh ** -0.5 if scale is None else float(scale)
-    _need(0.0 < p.scale < float("inf"), "scale must be positive and finite")
-    return p, _DTYPES[q.dtype]
+            if not (t.is_contiguous()):
+                raise ValueError(f"{name} must be contiguous")
+    scale = dh ** -0.5 if scale is None else float(scale)
+    if not (0.0 < scale < 3e38):
+        raise ValueError("scale must be positive and finite")
+    return (_ptr(key_mask), _ptr(kv_len), _ptr(q_pos), N, Tq, Tk, H, Hkv, dh, _bound(left, "left"), _bound(right, "right"), _bound(sinks or 0, "sinks"), scale), _DTYPES[q.dtype]
 
 
-def _strides(p, **tensors):
-    for name, t in tensors.items():
-        n, tk, h, d = t.stride()
-        _need(d == 1 or t.shape[3] == 1, f"the rows of {name} must be contiguous")
-        per = 16 // t.element_size()
-        _need(t.numel() == 0 or not (t.data_ptr() % 16 or n % per and t.shape[0] > 1 or tk % per and t.shape[1] > 1 or h % per and t.shape[2] > 1),
-              f"the rows of {name} must start at multiples of 16 bytes")
-        # (the stride of a dimension of size 0 or 1 is arbitrary and unused)
-        setattr(p, name + "_stride_n", n if t.shape[0] > 1 else 0)
-        setattr(p, name + "_stride_t", tk if t.shape[1] > 1 else 0)
-        setattr(p, name + "_stride_h", h if t.shape[2] > 1 else 0)
+_NO_STRIDE = (0, 0, 0)
 
 
 def window_attention(q, k, v, *, left=None, right=None, sinks=0, key_mask=None, kv_len=None, q_pos=None, scale=None, out=None):
@@ -113,50 +131,44 @@ def window_attention(q, k, v, *, left=None, right=None, sinks=0, key_mask=None, 
     no bound.  A row that sees nothing gives zeros and lse = -inf.  `out`: write there instead of into a new tensor.
 
     One new token behind a cache: Tq = 1, kv_len = the cache's lengths with the new key in place, q_pos = kv_len - 1, right = 0."""
-    p, code = _attention(q, k, v, left, right, sinks, key_mask, kv_len, q_pos, scale)
+    tail, code = _attention(q, k, v, left, right, sinks, key_mask, kv_len, q_pos, scale)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
-        _on(out, q, "out", (q.dtype,), q.shape)
-    lse = torch.empty((p.N, p.H, p.Tq), dtype=torch.float32, device=q.device)
-    _strides(p, out=out)
-    p.out, p.lse = out.data_ptr(), lse.data_ptr()
-    L = _lib.lib()
-    ws = _workspace(p, L.dic_win_attn_ws_bytes(code, 0, C.byref(p)), q.device)  # noqa: F841  (keeps the memory until the launch is queued)
-    _launch(L.dic_win_attn_fwd, code, p, q.device, "window_attention")
+        _check_rows(out, q, "out", q.shape)
+    lse = q.new_empty((tail[3], tail[6], tail[4]), dtype=torch.float32)
+    fields = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), 0, 0, 0, 0, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3],
+              *_NO_STRIDE, *_NO_STRIDE, *_NO_STRIDE, *_NO_STRIDE, *tail)
+    size = _fn("dic_win_attn_ws_bytes")(code, 0, _WIN.pack(*fields, 0, 0))
+    ws = q.new_empty(size, dtype=torch.uint8) if size else None
+    _launch("dic_win_attn_fwd", code, _WIN.pack(*fields, _ptr(ws), size), q.device)
     return out, lse
 
 
 def window_attention_grad(dout, q, k, v, out, lse, *, left=None, right=None, sinks=0, key_mask=None, kv_len=None, q_pos=None, scale=None, grads=None):
     """(dq, dk, dv) of window_attention for the gradient `dout` of its output; the other arguments as they went into and came out of that call.
     `grads`: three tensors to write them into (views of a packed gradient, say).  dk and dv are summed over the query heads of each key head."""
-    p, code = _attention(q, k, v, left, right, sinks, key_mask, kv_len, q_pos, scale)
+    tail, code = _attention(q, k, v, left, right, sinks, key_mask, kv_len, q_pos, scale)
     _on(dout, q, "dout", (q.dtype,), q.shape)
-    _on(out, q, "out", (q.dtype,), q.shape)
-    _on(lse, q, "lse", (torch.float32,), (p.N, p.H, p.Tq))
-    _need(lse.is_contiguous(), "lse must be contiguous")
-    if dout.stride(3) != 1 or any(s % (16 // dout.element_size()) for s in dout.stride()[:3]) or dout.data_ptr() % 16:
-        dout = dout.contiguous()                 # an expanded or transposed gradient
+    _check_rows(out, q, "out", q.shape)
+    _on(lse, q, "lse", (torch.float32,), (tail[3], tail[6], tail[4]))
+    if not (lse.is_contiguous()):
+        raise ValueError("lse must be contiguous")
+    per = 16 // q.element_size()
+    if not dout.is_contiguous() and (dout.stride(3) != 1 or any(s % per for s in dout.stride()[:3])) or dout.data_ptr() % 16:
+        dout = dout.clone(memory_format=torch.contiguous_format)                 # an expanded or transposed gradient
     if grads is None:
-        grads = [torch.empty(t.shape, dtype=q.dtype, device=q.device) for t in (q, k, v)]
+        dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
     else:
-        for t, like, name in zip(grads, (q, k, v), ("dq", "dk", "dv")):
-            _on(t, q, name, (q.dtype,), like.shape)
-    dq, dk, dv = grads
-    _strides(p, out=out, dout=dout, dq=dq, dk=dk, dv=dv)
-    p.out, p.lse, p.dout, p.dq, p.dk, p.dv = out.data_ptr(), lse.data_ptr(), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
-    L = _lib.lib()
-    ws = _workspace(p, L.dic_win_attn_ws_bytes(code, 1, C.byref(p)), q.device)  # noqa: F841
-    _launch(L.dic_win_attn_bwd, code, p, q.device, "window_attention_grad")
+        dq, dk, dv = grads
+        for t, like, name in ((dq, q, "dq"), (dk, k, "dk"), (dv, k, "dv")):
+            _check_rows(t, q, name, like.shape)
+    fields = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+              *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3], *dout.stride()[:3], *dq.stride()[:3], *dk.stride()[:3], *dv.stride()[:3], *tail)
+    size = _fn("dic_win_attn_ws_bytes")(code, 1, _WIN.pack(*fields, 0, 0))
+    ws = q.new_empty(size, dtype=torch.uint8) if size else None
+    _launch("dic_win_attn_bwd", code, _WIN.pack(*fields, _ptr(ws), size), q.device)
     return dq, dk, dv
-
-
-def _workspace(p, size, device):
-    if not size:
-        return None
-    ws = torch.empty(size, dtype=torch.uint8, device=device)
-    p.ws, p.ws_bytes = ws.data_ptr(), size
-    return ws
 
 
 # ------------------------------------------------------------------------------------------------ norms
@@ -168,41 +180,45 @@ class NormParams(NamedTuple):
     eps: float = 1e-12
 
 
-def _norms(x, like, post, pre, gate, residual_scale):
-    """(params, rows): the checked part that forward and backward share; `like` gives rows and device."""
-    D = like.shape[-1] if like.dim() else 0
-    _need(like.dim() >= 2 and 1 <= D <= 8192, "rows of 1 to 8192 elements in at least two dimensions are needed")
-    rows = like.numel() // D
-    p = _lib.GatedNormParams()
-    p.rows, p.rows_per_gate, p.D, p.residual_scale = rows, max(rows, 1), D, float(residual_scale)
-    for norm, side in ((post, "post"), (pre, "pre")):
-        if norm is None:
-            continue
-        _need(norm.kind in ("layer", "rms"), f"{side}: a norm is \"layer\" or \"rms\"")
-        for t, name in ((norm.weight, "weight"), (norm.bias, "bias")):
-            if t is not None:
-                _on(t, like, f"{side} {name}", (torch.float32,), (D,))
-                _need(t.is_contiguous(), f"{side} {name} must be contiguous")
-                setattr(p, f"{side}_{name}", t.data_ptr())
-        setattr(p, side + "_kind", _KINDS[norm.kind])
-        setattr(p, side + "_eps", float(norm.eps))
-    if gate is not None:
-        _on(gate, like, "gate", (torch.float32,))
-        _need(gate.is_contiguous() and gate.dim() in (1, 2) and gate.shape[-1] == D, f"gate must be contiguous, [{D}] or [sequences, {D}]")
-        n = 1 if gate.dim() == 1 else gate.shape[0]
-        _need(rows == 0 or (n > 0 and rows % n == 0), f"{rows} rows do not divide over {n} gates")
-        p.gate, p.rows_per_gate = gate.data_ptr(), max(rows // max(n, 1), 1)
-    return p
+def _norm(norm, like, D, side):
+    """The packed fields of one norm."""
+    if norm is None:
+        return 0, 0, 0, 0.0
+    if not (norm.kind in _KINDS):
+        raise ValueError(f'{side}: a norm is "layer" or "rms"')
+    for t, name in ((norm.weight, "weight"), (norm.bias, "bias")):
+        if t is not None:
+            _on(t, like, f"{side} {name}", (torch.float32,), (D,))
+            if not (t.is_contiguous()):
+                raise ValueError(f"{side} {name} must be contiguous")
+    return _ptr(norm.weight), _ptr(norm.bias), _KINDS[norm.kind], float(norm.eps)
 
 
-def _rows(t, like, name, dtypes, shape):
-    _on(t, like, name, dtypes, shape)
-    _need(t.is_contiguous(), f"{name} must be contiguous")
-    return t
+def _shapes(x, gate):
+    """(rows, D, rows that share a gate row) of x [..., D]."""
+    if not (x.dim() >= 2 and 1 <= x.shape[-1] <= 8192):
+        raise ValueError("rows of 1 to 8192 elements in at least two dimensions are needed")
+    D = x.shape[-1]
+    rows = x.numel() // D
+    if gate is None:
+        return rows, D, 1
+    _on(gate, x, "gate", (torch.float32,))
+    if not (gate.is_contiguous() and gate.dim() in (1, 2) and gate.shape[-1] == D):
+        raise ValueError(f"gate must be contiguous, [{D}] or [sequences, {D}]")
+    n = 1 if gate.dim() == 1 else gate.shape[0]
+    if not (rows == 0 or (n > 0 and rows % n == 0)):
+        raise ValueError(f"{rows} rows do not divide over {n} gates")
+    return rows, D, max(rows // max(n, 1), 1)
+
+
+def _packed(t, like, name, dtype):
+    _on(t, like, name, (dtype,), like.shape)
+    if not (t.is_contiguous()):
+        raise ValueError(f"{name} must be contiguous")
 
 
 def _norm_code(stream, inner):
-    if stream not in _DTYPES or inner not in _DTYPES or (stream, inner) == (torch.bfloat16, torch.float32):
+    if inner not in _DTYPES or (stream, inner) == (torch.bfloat16, torch.float32):
         raise TypeError(f"a {stream} residual stream with {inner} blocks: float32 with float32 or bfloat16, or bfloat16 with bfloat16")
     return _DTYPES[inner] | (_RES_F32 if stream != inner else 0)
 
@@ -212,63 +228,69 @@ def gated_norm(x, y=None, *, post=None, gate=None, residual_scale=1.0, pre=None,
 
     y [..., D] is a block's output, x the residual stream in front of the block (x may be float32 beside a bfloat16 y).  post, pre: NormParams or None (no
     norm; without pre, a is None).  gate: float32 [D], [N, D] (one row for each of N equal runs of rows: the sequences of [N, T, D]), or None.  `saved`
-    [4, rows] holds the rows' statistics for gated_norm_grad.  Without y it is a stack's first norm: a = pre(residual_scale x), of type `dtype` (x's)."""
-    _lib.require_gpu()
-    _need(isinstance(x, torch.Tensor) and x.is_cuda, "x must be a tensor on the GPU")
+    [4, rows] holds the rows' statistics for gated_norm_grad.  Without y it is a stack's first norm: a = pre(residual_scale x), of type `dtype` (x's); at
+    scale 1 x_new is then x itself."""
+    _first(x, "x")
     inner = y.dtype if isinstance(y, torch.Tensor) else (dtype or x.dtype)
-    _need(y is None or dtype in (None, inner), "dtype is the type of a without y")
     code = _norm_code(x.dtype, inner)
-    _rows(x, x, "x", (x.dtype,), x.shape)
+    _packed(x, x, "x", x.dtype)
     if y is not None:
-        _rows(y, x, "y", (inner,), x.shape)
+        _packed(y, x, "y", inner)
+        if not (dtype in (None, inner)):
+            raise ValueError("dtype is the type of a without y")
     else:
-        _need(post is None and gate is None and pre is not None, "without y there is a pre norm and nothing else")
-    p = _norms(x, x, post, pre, gate, residual_scale)
-    x_new = x if y is None and residual_scale == 1.0 else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    a = torch.empty(x.shape, dtype=inner, device=x.device) if pre is not None else None
-    saved = torch.empty((4, p.rows), dtype=torch.float32, device=x.device)
-    p.x, p.y, p.a, p.saved = x.data_ptr(), _ptr(y), _ptr(a), saved.data_ptr()
-    p.x_new = None if x_new is x else x_new.data_ptr()
-    _launch(_lib.lib().dic_gated_norm_fwd, code, p, x.device, "gated_norm")
+        if not (post is None and gate is None and pre is not None):
+            raise ValueError("without y there is a pre norm and nothing else")
+    rows, D, per_gate = _shapes(x, gate)
+    sides = *_norm(post, x, D, "post"), *_norm(pre, x, D, "pre")
+    x_new = x if y is None and residual_scale == 1.0 else torch.empty_like(x)
+    a = None if pre is None else torch.empty_like(x if y is None else y, dtype=inner)
+    saved = x.new_empty((4, rows), dtype=torch.float32)
+    _launch("dic_gated_norm_fwd", code, _NORM.pack(x.data_ptr(), _ptr(y), 0 if x_new is x else x_new.data_ptr(), _ptr(a), _ptr(gate), saved.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, 0,
+                                                   *sides, rows, per_gate, D, residual_scale, 0, 0), x.device)
     return x_new, a, saved
 
 
 def gated_norm_grad(dx_new, da, x_new, y, saved, *, post=None, gate=None, residual_scale=1.0, pre=None):
     """Gradients of gated_norm as a dict: "dx", "dy", "gate", "post_weight", "post_bias", "pre_weight", "pre_bias", as far as there are such inputs.
     dx_new (None: zero) and da (None without pre) are the gradients of its outputs; x_new, y and saved as they went into and came out of that call."""
-    _lib.require_gpu()
-    _need(isinstance(x_new, torch.Tensor) and x_new.is_cuda, "x_new must be a tensor on the GPU")
+    _first(x_new, "x_new")
     given = y if y is not None else da
     inner = given.dtype if isinstance(given, torch.Tensor) else x_new.dtype
     code = _norm_code(x_new.dtype, inner)
-    _rows(x_new, x_new, "x_new", (x_new.dtype,), x_new.shape)
-    _need((da is None) == (pre is None), "da is the gradient of pre's output: both or neither")
+    _packed(x_new, x_new, "x_new", x_new.dtype)
+    if not ((da is None) == (pre is None)):
+        raise ValueError("da is the gradient of pre's output: both or neither")
+    if not (dx_new is not None or da is not None):
+        raise ValueError("neither output has a gradient")
     if dx_new is not None:
-        _rows(dx_new, x_new, "dx_new", (x_new.dtype,), x_new.shape)
+        _packed(dx_new, x_new, "dx_new", x_new.dtype)
     if da is not None:
-        _rows(da, x_new, "da", (inner,), x_new.shape)
+        _packed(da, x_new, "da", inner)
     if y is not None:
-        _rows(y, x_new, "y", (inner,), x_new.shape)
+        _packed(y, x_new, "y", inner)
     else:
-        _need(post is None and gate is None and pre is not None, "without y there is a pre norm and nothing else")
-    _need(dx_new is not None or da is not None, "neither output has a gradient")
-    p = _norms(x_new, x_new, post, pre, gate, residual_scale)
-    _rows(saved, x_new, "saved", (torch.float32,), (4, p.rows))
-    new = lambda t: torch.empty(t.shape, dtype=t.dtype, device=t.device)  # noqa: E731
-    got = {"dx": new(x_new)}
+        if not (post is None and gate is None and pre is not None):
+            raise ValueError("without y there is a pre norm and nothing else")
+    rows, D, per_gate = _shapes(x_new, gate)
+    sides = *_norm(post, x_new, D, "post"), *_norm(pre, x_new, D, "pre")
+    _on(saved, x_new, "saved", (torch.float32,), (4, rows))
+    if not (saved.is_contiguous()):
+        raise ValueError("saved must be contiguous")
+    got = {"dx": torch.empty_like(x_new)}
     if y is not None:
-        got["dy"] = new(y)
+        got["dy"] = torch.empty_like(y)
     if gate is not None:
-        got["gate"] = new(gate) if p.rows else torch.zeros_like(gate)
-    for norm, side in ((post, "post"), (pre, "pre")):
-        for name in ("weight", "bias"):
-            t = getattr(norm, name) if norm is not None else None
-            if t is not None:
-                got[f"{side}_{name}"] = new(t)
-    p.x_new, p.y, p.saved, p.dx_new, p.da = x_new.data_ptr(), _ptr(y), saved.data_ptr(), _ptr(dx_new), _ptr(da)
-    p.dx, p.dy, p.dgate = _ptr(got["dx"]), _ptr(got.get("dy")), _ptr(got.get("gate"))
-    p.dpost_w, p.dpost_b, p.dpre_w, p.dpre_b = (_ptr(got.get(k)) for k in ("post_weight", "post_bias", "pre_weight", "pre_bias"))
-    L = _lib.lib()
-    ws = _workspace(p, L.dic_gated_norm_ws_bytes(code, C.byref(p)), x_new.device)  # noqa: F841
-    _launch(L.dic_gated_norm_bwd, code, p, x_new.device, "gated_norm_grad")
+        got["gate"] = torch.empty_like(gate) if rows else torch.zeros_like(gate)
+    for norm, weight, bias in ((post, "post_weight", "post_bias"), (pre, "pre_weight", "pre_bias")):
+        if norm is not None:
+            if norm.weight is not None:
+                got[weight] = torch.empty_like(norm.weight)
+            if norm.bias is not None:
+                got[bias] = torch.empty_like(norm.bias)
+    fields = (0, _ptr(y), x_new.data_ptr(), 0, _ptr(gate), saved.data_ptr(), _ptr(dx_new), _ptr(da), got["dx"].data_ptr(), _ptr(got.get("dy")), _ptr(got.get("gate")),
+              _ptr(got.get("post_weight")), _ptr(got.get("post_bias")), _ptr(got.get("pre_weight")), _ptr(got.get("pre_bias")), *sides, rows, per_gate, D, residual_scale)
+    size = _fn("dic_gated_norm_ws_bytes")(code, _NORM.pack(*fields, 0, 0))
+    ws = x_new.new_empty(size, dtype=torch.uint8) if size else None
+    _launch("dic_gated_norm_bwd", code, _NORM.pack(*fields, _ptr(ws), size), x_new.device)
     return got

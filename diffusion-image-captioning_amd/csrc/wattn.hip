@@ -7,7 +7,9 @@
 // from LDS in the same token order, which ds_read_b64_tr_b16 (bf16) or plain 4-byte reads (fp32) give.
 // Tiles come in by LDS-DMA, double-buffered; rows of keys that nobody may see (key_mask, kv_len) are zero-filled by the descriptor's bounds check, so
 // that an infinity or NaN in them cannot reach 0 * v.
+#include <atomic>
 #include <cmath>
+#include <type_traits>
 #include "common.h"
 #include "../../include/dic_hip.h"
 
@@ -26,18 +28,45 @@ struct WinArgs {
     const uint8_t* key_mask;
     const int* kv_len;
     const int* q_pos;
+    float* sinks_ws;                            // backward workspace [N Hkv][chunks][sink_rows][dk, dv]
+    float* parts;                               // few-rows workspace: [N Hkv][splits][rows][DH], then {m, l} of each
     int N, Tq, Tk, H, Hkv, G, left, right, sinks;
+    int near_sinks;                             // backward: sinks that the window pass takes along
+    int sink_keys, sink_rows, chunks;           // or those that have a pass of their own, that rounded up to 32, and pieces of that pass
     float scale, c;                             // c = scale * log2(e)
 };
 
 __device__ __forceinline__ int tok(int r, int hi) { return (r & 3) + 8 * (r >> 2) + 4 * hi; }     // row of register r of a 32x32 accumulator
 __device__ __forceinline__ f32x16 zero16() { f32x16 z; for (int i = 0; i < 16; ++i) z[i] = 0.f; return z; }
 
-// An LDS tile holds token rows of DH elements as 16-byte chunks, chunk c of row r at slot c ^ swz(r).  The order makes both readings free of bank
-// conflicts: 16 consecutive rows at one chunk index (row operands, ds_read_b128), and 64 bytes of each of 4 consecutive rows (transposing reads).
+// An LDS tile holds token rows of DH elements, cut into segments of 64 bytes (4 chunks of 16).  One DMA instruction fills a piece of 1 KiB, in which the same
+// segment of 4 rows (512-byte rows: 2) lies side by side; pieces are PS bytes apart.  Both readings are then free of bank conflicts -- 64 bytes of each of 4
+// rows are 256 consecutive bytes (transposing reads), and the padding between pieces turns 16 consecutive rows at one chunk over all banks (row operands,
+// ds_read_b128; 128-byte rows, two quads to a piece, also swap neighbouring chunks in every odd quad) -- and every address is a lane's base plus a constant.
 template <typename T, int DH> struct Lay {
     static constexpr int ROWB = DH * (int)sizeof(T), CH = ROWB / 16, NF = ROWB / 32, ND = DH / 32, PIECE_ROWS = 1024 / ROWB;
-    __device__ static __forceinline__ int swz(int row) { return CH == 8 ? (((row >> 1) & 1) << 2) | ((row >> 2) & 3) : ((row & 3) << 2) | ((row >> 2) & 3); }
+    static constexpr int PS = CH == 8 ? 1056 : 1040, SEG = CH == 32 ? 128 : 256;            // bytes between pieces; between a row's segments
+    static constexpr int bytes(int rows) { return rows / PIECE_ROWS * PS; }
+    // what a lane of the DMA instruction carries: row and chunk inside the piece
+    __device__ static __forceinline__ int dma_row(int lane) { return CH == 8 ? (lane >> 5) * 4 + ((lane >> 2) & 3) : CH == 16 ? (lane >> 2) & 3 : (lane >> 2) & 1; }
+    __device__ static __forceinline__ int dma_chunk(int lane) {
+        return CH == 8 ? ((lane >> 4) & 1) * 4 + ((lane & 3) ^ (lane >> 5)) : CH == 16 ? (lane >> 4) * 4 + (lane & 3) : (lane >> 3) * 4 + (lane & 3);
+    }
+    // row operand of a 32-row block: lane's row lane & 31, chunk 2 s + (lane >> 5) at base + step(s)
+    __device__ static __forceinline__ int row_base(int lane) {
+        const int r = lane & 31, hi = lane >> 5, q = (r >> 2) & 1;
+        return CH == 8 ? (r >> 3) * PS + q * 512 + (r & 3) * 64 + ((hi ^ q) << 4) : CH == 16 ? (r >> 2) * PS + (r & 3) * 64 + (hi << 4) : (r >> 1) * PS + (r & 1) * 64 + (hi << 4);
+    }
+    static constexpr int step(int s) { return (s >> 1) * SEG + (s & 1) * 32; }
+    // bf16, transposing reads: 4 elements of rows 4 hi + (t >> 2), t = lane & 15, of a 16-row block; + up for the rows 8 further on
+    __device__ static __forceinline__ int tr_base(int lane) {
+        const int hi = lane >> 5, c = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1), r = (lane & 15) >> 2, sub = (lane & 1) * 8;
+        return CH == 8 ? hi * 512 + r * 64 + ((c ^ hi) << 4) + sub : hi * PS + r * 64 + (c << 4) + sub;
+    }
+    static constexpr int up = 8 / PIECE_ROWS * PS;
+    // fp32, by element: lane's element lane & 31 of row tok(r, hi), at base + at(r)
+    __device__ static __forceinline__ int el_base(int lane) { return (lane >> 5) * (4 / PIECE_ROWS) * PS + ((lane >> 4) & 1) * SEG + (lane & 15) * 4; }
+    static constexpr int at(int r) { return (8 / PIECE_ROWS) * (r >> 2) * PS + (PIECE_ROWS == 4 ? (r & 3) * 64 : ((r & 3) >> 1) * PS + (r & 1) * 64); }
 };
 
 // Row operand of a 32-token block: lane holds row (lane & 31), bytes 32 s + 16 (lane >> 5).
@@ -46,14 +75,13 @@ template <> struct Mma<bf16_t> {
     typedef bf16x8 Frag;
     __device__ static __forceinline__ f32x16 mac(Frag a, Frag b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
     // acc[d][col] += sum over 32 tokens of tile[token][32 db + d] * p[token][col], p in accumulator order
-    template <int DH> __device__ static __forceinline__ f32x16 mac_t(const char* tile, int row0, int db, const f32x16& p, f32x16 acc, int lane) {
+    template <int DH> __device__ static __forceinline__ f32x16 mac_t(const char* tile, int db, const f32x16& p, f32x16 acc, int lane) {
         using L = Lay<bf16_t, DH>;
-        const int hi = lane >> 5, half = (lane >> 4) & 1, t = lane & 15;
+        const char* base = tile + L::tr_base(lane) + db * L::SEG;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-            const int r0 = row0 + 16 * s + 4 * hi + (t >> 2), c = db * 4 + half * 2 + ((t & 3) >> 1), sub = (t & 1) * 8;
-            s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR(s16x4))(tile + r0 * L::ROWB + ((c ^ L::swz(r0)) << 4) + sub));
-            s16x4 up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR(s16x4))(tile + (r0 + 8) * L::ROWB + ((c ^ L::swz(r0 + 8)) << 4) + sub));
+            s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR(s16x4))(base + 2 * s * L::up));
+            s16x4 up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR(s16x4))(base + (2 * s + 1) * L::up));
             s16x8 a = __builtin_shufflevector(lo, up, 0, 1, 2, 3, 4, 5, 6, 7);
             i32x4 b;
 #pragma unroll
@@ -77,15 +105,11 @@ template <> struct Mma<float> {
         for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
         return c;
     }
-    template <int DH> __device__ static __forceinline__ f32x16 mac_t(const char* tile, int row0, int db, const f32x16& p, f32x16 acc, int lane) {
+    template <int DH> __device__ static __forceinline__ f32x16 mac_t(const char* tile, int db, const f32x16& p, f32x16 acc, int lane) {
         using L = Lay<float, DH>;
-        const int hi = lane >> 5, d = lane & 31;
+        const char* base = tile + L::el_base(lane) + 2 * db * L::SEG;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const int row = row0 + tok(r, hi);
-            const float a = *(const float*)(tile + row * L::ROWB + (((db * 8 + (d >> 2)) ^ L::swz(row)) << 4) + (d & 3) * 4);
-            acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[r], acc, 0, 0, 0);
-        }
+        for (int r = 0; r < 16; ++r) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(*(const float*)(base + L::at(r)), p[r], acc, 0, 0, 0);
         return acc;
     }
     __device__ static __forceinline__ float dot(Frag a, Frag b) { return (a[0] * b[0] + a[1] * b[1]) + (a[2] * b[2] + a[3] * b[3]); }
@@ -112,24 +136,26 @@ __device__ __forceinline__ void dma4(unsigned voff, const i32x4& rsrc, unsigned 
 // this wave's DMA has landed and, behind the barrier, everybody's has; everybody is done with the buffer that is refilled next
 __device__ __forceinline__ void dma_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// ROWS token rows from `base` (row stride st bytes) into a tile; bit r of `valid`: row r is read, else zero.  NW waves share the pieces.
-template <typename T, int DH, int ROWS, int NW>
-__device__ __forceinline__ void load_tile(const char* base, unsigned st, unsigned long long valid, unsigned lds, int wave, int lane) {
+// ROWS token rows from `base` (row stride st bytes) into a tile; bit r of `valid`: row r is read, else zero.  Waves first, first + step, ... share the pieces.
+template <typename T, int DH, int ROWS>
+__device__ __forceinline__ void load_tile(const char* base, unsigned st, unsigned long long valid, unsigned lds, int first, int step, int lane) {
     using L = Lay<T, DH>;
     const i32x4 rs = tile_rsrc(base);
     constexpr int P = ROWS / L::PIECE_ROWS;
-    static_assert(ROWS % L::PIECE_ROWS == 0 && P % NW == 0, "pieces divide over the waves");
+    static_assert(ROWS % L::PIECE_ROWS == 0, "whole pieces");
+    auto one = [&](int piece, bool all) {
+        const int row = piece * L::PIECE_ROWS + L::dma_row(lane);
+        const unsigned off = (unsigned)row * st + (unsigned)L::dma_chunk(lane) * 16u;
+        dma16(all || ((valid >> row) & 1ull) ? off : 0xfffffff0u, rs, lds + (unsigned)(piece * L::PS));
+    };
+    if (P >= 4 && step == 4 && valid == (ROWS == 64 ? ~0ull : (1ull << ROWS % 64) - 1)) {
 #pragma unroll
-    for (int j = 0; j < P / NW; ++j) {
-        const int piece = j * NW + wave, row = piece * L::PIECE_ROWS + lane / L::CH, c = (lane % L::CH) ^ L::swz(row);
-        const unsigned off = ((valid >> row) & 1ull) ? (unsigned)row * st + (unsigned)c * 16u : 0xfffffff0u;
-        dma16(off, rs, lds + (unsigned)piece * 1024u);
-    }
+        for (int j = 0; j < P / 4; ++j) one(4 * j + first, true);
+    } else for (int piece = first; piece < P; piece += step) one(piece, false);
 }
 template <typename T, int DH>
-__device__ __forceinline__ typename Mma<T>::Frag row_frag(const char* tile, int row, int s, int hi) {
-    using L = Lay<T, DH>;
-    return *(const typename Mma<T>::Frag*)(tile + row * L::ROWB + (((2 * s + hi) ^ L::swz(row)) << 4));
+__device__ __forceinline__ typename Mma<T>::Frag row_frag(const char* tile, int s, int lane) {
+    return *(const typename Mma<T>::Frag*)(tile + Lay<T, DH>::row_base(lane) + Lay<T, DH>::step(s));
 }
 
 __device__ __forceinline__ unsigned long long below(int x) { return x <= 0 ? 0ull : x >= 64 ? ~0ull : (1ull << x) - 1ull; }
@@ -177,27 +203,29 @@ __device__ __forceinline__ int xcd_item() {
 // key_mask bits of a tile: lane reads its key's byte (called one tile ahead), the ballot is the tile's mask
 __device__ __forceinline__ int mask_byte(const WinArgs& a, int n, int j) { return a.key_mask && j >= 0 && j < a.Tk ? a.key_mask[(size_t)n * a.Tk + j] : 1; }
 
-constexpr int BM = 128, NWAVE = 4;              // queries (or keys) per workgroup: 32 per wave
-constexpr int BQ = 32;                          // queries per tile of the dk / dv kernel
+template <typename T> constexpr int MOST_WAVES = sizeof(T) == 2 ? 8 : 4;      // of a workgroup: fp32 operands need more than half of a SIMD's registers
+// waves that a SIMD is to hold at once: what the registers of bf16 rows of 64 allow, 2 for rows of 128, 1 for fp32
+template <typename T, int DH, int MOST> constexpr int RESIDENT = sizeof(T) == 4 ? 1 : DH == 64 ? MOST : 2;
+constexpr int BQ = 32;                          // queries (or keys) per wave, and rows of a statistics tile
 __host__ __device__ __forceinline__ long long stats_floats(long long N, long long H, long long Tq) { return N * H * ((Tq + BQ - 1) / BQ) * 2 * BQ; }
 __device__ __forceinline__ long long stats_at(const WinArgs& a, int n, int h, int i0) { return stats_floats(1, (long long)n * a.H + h, a.Tq) + 2 * i0; }
 
 // ------------------------------------------------------------------------------------------------ forward
 template <typename T, int DH, int BN>
-__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void win_fwd_kernel(const WinArgs a) {
+__global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 4>)) void win_fwd_kernel(const WinArgs a) {
     using L = Lay<T, DH>;
     using M = Mma<T>;
-    constexpr int NB = BN / 32, TILE = BN * L::ROWB;
+    constexpr int NB = BN / 32, TILE = L::bytes(BN);
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hi = lane >> 5;
-    const int nqt = (a.Tq + BM - 1) / BM;
+    const int nw = blockDim.x >> 6, bm = nw * BQ, nqt = (a.Tq + bm - 1) / bm;
     int item = xcd_item();
     const int g = item % a.G; item /= a.G;
     const int qt = nqt - 1 - item % nqt; item /= nqt;         // long rows first
     const int hk = item % a.Hkv, n = item / a.Hkv, h = hk * a.G + g;
     const Seq sq = sequence(a, n);
-    const int i0 = qt * BM + wave * 32, i = i0 + (lane & 31), ic = min(i, a.Tq - 1);
-    const Walk wk = walk_of(a, sq.pos + qt * BM, sq.pos + min(qt * BM + BM, a.Tq) - 1, sq.kvl, BN);
+    const int i0 = qt * bm + wave * BQ, i = i0 + (lane & 31), ic = min(i, a.Tq - 1);
+    const Walk wk = walk_of(a, sq.pos + qt * bm, sq.pos + min(qt * bm + bm, a.Tq) - 1, sq.kvl, BN);
     const Span sp = span_of(a, sq.pos + ic, sq.kvl);
     const bool wave_rows = i0 < a.Tq;
     // what every row of this wave sees: [in_lo, in_hi)
@@ -214,8 +242,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void win_fwd_kernel(co
     const long long kst = a.sk.t * (long long)sizeof(T), vst = a.sv.t * (long long)sizeof(T);
     const unsigned lds = (unsigned)(uintptr_t)(LDS_PTR(char))smem;
     auto issue = [&](int j0, unsigned long long valid, int buf) {
-        load_tile<T, DH, BN, NWAVE>(kb + j0 * kst, (unsigned)kst, valid, lds + buf * 2 * TILE, wave, lane);
-        load_tile<T, DH, BN, NWAVE>(vb + j0 * vst, (unsigned)vst, valid, lds + buf * 2 * TILE + TILE, wave, lane);
+        load_tile<T, DH, BN>(kb + j0 * kst, (unsigned)kst, valid, lds + buf * 2 * TILE, wave, nw, lane);
+        load_tile<T, DH, BN>(vb + j0 * vst, (unsigned)vst, valid, lds + buf * 2 * TILE + TILE, wave, nw, lane);
     };
     auto valid_of = [&](int byte, int j0) { return __ballot(byte != 0) & below(min(BN, wk.kvl - j0)); };
 
@@ -223,6 +251,52 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void win_fwd_kernel(co
 #pragma unroll
     for (int d = 0; d < L::ND; ++d) acc[d] = zero16();
     float m = -INFINITY, l = 0.f;
+    // one step over `count` blocks of 32 keys of a tile, from block b0 on
+    auto blocks = [&](auto count, int b0, const char* kt, const char* vt, unsigned long long bits, bool full) {
+        constexpr int C = decltype(count)::value;
+        f32x16 st[C];
+        kt += b0 * L::bytes(32);
+        vt += b0 * L::bytes(32);
+#pragma unroll
+        for (int b = 0; b < C; ++b) {
+            st[b] = zero16();
+#pragma unroll
+            for (int s = 0; s < L::NF; ++s) st[b] = M::mac(row_frag<T, DH>(kt + L::bytes(32 * b), s, lane), qf[s], st[b]);
+        }
+        if (!full) {
+#pragma unroll
+            for (int b = 0; b < C; ++b) {
+                const unsigned w = (unsigned)(bits >> (32 * (b0 + b))) >> (4 * hi);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) st[b][r] = (w >> tok(r, 0)) & 1u ? st[b][r] : -INFINITY;
+            }
+        }
+        float mt = st[0][0];
+#pragma unroll
+        for (int b = 0; b < C; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) mt = fmaxf(mt, st[b][r]);
+        mt = fmaxf(mt, __shfl_xor(mt, 32, 64)) * a.c;
+        // The reference point m of the exponentials follows the running maximum only when that is more than 2^8 above it: the sums are in 32 bits and
+        // P's relative rounding does not depend on its size, and most tiles then leave the accumulators as they are.
+        if (__any(mt > m + 8.f)) {
+            const float mn = fmaxf(m, mt), f = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+            m = mn;
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < L::ND; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[d][r] *= f;
+        }
+        const float mm = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int b = 0; b < C; ++b) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) { st[b][r] = __builtin_amdgcn_exp2f(fmaf(st[b][r], a.c, -mm)); l += st[b][r]; }
+#pragma unroll
+            for (int d = 0; d < L::ND; ++d) acc[d] = M::template mac_t<DH>(vt + L::bytes(32 * b), d, st[b], acc[d], lane);
+        }
+    };
     unsigned long long valid = 0, valid_next = 0;
     int byte = 1;                                             // key_mask of this lane's key in the tile after the next
     if (wk.nt > 0) {
@@ -244,45 +318,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void win_fwd_kernel(co
         const bool full = j0 >= in_lo && j0 + BN <= in_hi && valid == below(BN);
         if (!full) bits = visible(sp, j0) & valid;
         if (wave_rows && (full || __any(bits != 0))) {
-            f32x16 st[NB];
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                st[b] = zero16();
-#pragma unroll
-                for (int s = 0; s < L::NF; ++s) st[b] = M::mac(row_frag<T, DH>(kt, 32 * b + (lane & 31), s, hi), qf[s], st[b]);
-            }
-            if (!full) {
-#pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    const unsigned w = (unsigned)(bits >> (32 * b)) >> (4 * hi);
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) st[b][r] = (w >> tok(r, 0)) & 1u ? st[b][r] : -INFINITY;
-                }
-            }
-            float mt = st[0][0];
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) mt = fmaxf(mt, st[b][r]);
-            mt = fmaxf(mt, __shfl_xor(mt, 32, 64)) * a.c;
-            // The reference point m of the exponentials follows the running maximum only when that is more than 2^8 above it: the sums are in
-            // 32 bits and P's relative rounding does not depend on its size, and most tiles then leave the accumulators as they are.
-            if (__any(mt > m + 8.f)) {
-                const float mn = fmaxf(m, mt), f = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
-                m = mn;
-                l *= f;
-#pragma unroll
-                for (int d = 0; d < L::ND; ++d)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) acc[d][r] *= f;
-            }
-            const float mm = m == -INFINITY ? 0.f : m;
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) { st[b][r] = __builtin_amdgcn_exp2f(fmaf(st[b][r], a.c, -mm)); l += st[b][r]; }
-#pragma unroll
-                for (int d = 0; d < L::ND; ++d) acc[d] = M::template mac_t<DH>(vt, 32 * b, d, st[b], acc[d], lane);
+            // blocks of 32 keys that no row of the wave sees are left out
+            if constexpr (NB == 1) blocks(std::integral_constant<int, 1>(), 0, kt, vt, bits, full);
+            else {
+                const bool first = full || __any((unsigned)bits != 0), second = full || __any((unsigned)(bits >> 32) != 0);
+                if (first && second) blocks(std::integral_constant<int, 2>(), 0, kt, vt, bits, full);
+                else blocks(std::integral_constant<int, 1>(), first ? 0 : 1, kt, vt, bits, full);
             }
         }
         valid = valid_next;
@@ -301,20 +342,20 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void win_fwd_kernel(co
 
 // ------------------------------------------------------------------------------------------------ backward: dq (and delta)
 template <typename T, int DH, int BN>
-__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void win_bwd_dq_kernel(const WinArgs a) {
+__global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 3>)) void win_bwd_dq_kernel(const WinArgs a) {
     using L = Lay<T, DH>;
     using M = Mma<T>;
-    constexpr int NB = BN / 32, TILE = BN * L::ROWB;
+    constexpr int NB = BN / 32, TILE = L::bytes(BN);
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hi = lane >> 5;
-    const int nqt = (a.Tq + BM - 1) / BM;
+    const int nw = blockDim.x >> 6, bm = nw * BQ, nqt = (a.Tq + bm - 1) / bm;
     int item = xcd_item();
     const int g = item % a.G; item /= a.G;
     const int qt = nqt - 1 - item % nqt; item /= nqt;
     const int hk = item % a.Hkv, n = item / a.Hkv, h = hk * a.G + g;
     const Seq sq = sequence(a, n);
-    const int i0 = qt * BM + wave * 32, i = i0 + (lane & 31), ic = min(i, a.Tq - 1);
-    const Walk wk = walk_of(a, sq.pos + qt * BM, sq.pos + min(qt * BM + BM, a.Tq) - 1, sq.kvl, BN);
+    const int i0 = qt * bm + wave * BQ, i = i0 + (lane & 31), ic = min(i, a.Tq - 1);
+    const Walk wk = walk_of(a, sq.pos + qt * bm, sq.pos + min(qt * bm + bm, a.Tq) - 1, sq.kvl, BN);
     const Span sp = span_of(a, sq.pos + ic, sq.kvl);
     const bool wave_rows = i0 < a.Tq;
     const int in_lo = span_of(a, sq.pos + min(i0 + 31, a.Tq - 1), sq.kvl).lo, in_hi = span_of(a, sq.pos + min(i0, a.Tq - 1), sq.kvl).hi;
@@ -341,8 +382,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void win_bwd_dq_kernel
     const long long kst = a.sk.t * (long long)sizeof(T), vst = a.sv.t * (long long)sizeof(T);
     const unsigned lds = (unsigned)(uintptr_t)(LDS_PTR(char))smem;
     auto issue = [&](int j0, unsigned long long valid, int buf) {
-        load_tile<T, DH, BN, NWAVE>(kb + j0 * kst, (unsigned)kst, valid, lds + buf * 2 * TILE, wave, lane);
-        load_tile<T, DH, BN, NWAVE>(vb + j0 * vst, (unsigned)vst, valid, lds + buf * 2 * TILE + TILE, wave, lane);
+        load_tile<T, DH, BN>(kb + j0 * kst, (unsigned)kst, valid, lds + buf * 2 * TILE, wave, nw, lane);
+        load_tile<T, DH, BN>(vb + j0 * vst, (unsigned)vst, valid, lds + buf * 2 * TILE + TILE, wave, nw, lane);
     };
     auto valid_of = [&](int byte, int j0) { return __ballot(byte != 0) & below(min(BN, wk.kvl - j0)); };
     f32x16 acc[L::ND];
@@ -371,11 +412,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void win_bwd_dq_kernel
         if (wave_rows && (full || __any(bits != 0))) {
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
+                if (!full && !__any((unsigned)(bits >> (32 * b)) != 0)) continue;
                 f32x16 st = zero16(), dp = zero16();
 #pragma unroll
                 for (int s = 0; s < L::NF; ++s) {
-                    st = M::mac(row_frag<T, DH>(kt, 32 * b + (lane & 31), s, hi), qf[s], st);
-                    dp = M::mac(row_frag<T, DH>(vt, 32 * b + (lane & 31), s, hi), df[s], dp);
+                    st = M::mac(row_frag<T, DH>(kt + L::bytes(32 * b), s, lane), qf[s], st);
+                    dp = M::mac(row_frag<T, DH>(vt + L::bytes(32 * b), s, lane), df[s], dp);
                 }
                 const unsigned w = (unsigned)(bits >> (32 * b)) >> (4 * hi);
 #pragma unroll
@@ -384,7 +426,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void win_bwd_dq_kernel
                     st[r] = full || ((w >> tok(r, 0)) & 1u) ? p : 0.f;
                 }
 #pragma unroll
-                for (int d = 0; d < L::ND; ++d) acc[d] = M::template mac_t<DH>(kt, 32 * b, d, st, acc[d], lane);
+                for (int d = 0; d < L::ND; ++d) acc[d] = M::template mac_t<DH>(kt + L::bytes(32 * b), d, st, acc[d], lane);
             }
         }
         valid = valid_next;
@@ -400,28 +442,38 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void win_bwd_dq_kernel
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dk, dv
-template <typename T, int DH>
-__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void win_bwd_dkv_kernel(const WinArgs a) {
+// A workgroup owns kg groups of 32 keys and walks the queries that see them, 32 qh at a time: wave w takes key group w % kg and query rows 32 (w / kg).
+// The qh partial sums of a key group are added through LDS at the end.
+// SINK = false: the pairs inside the windows.  SINK = true, launched before it: the pairs of a sink key and a query whose window starts behind it.  Every
+// query has those, so their walk is cut into `chunks` that leave fp32 partial sums in the workspace; the window pass adds them to the sink keys' rows
+// in a fixed order.  (One workgroup that walks all queries for the sinks' tile alone took 1.9 ms where the window pass takes a tenth of that.)
+template <typename T, int DH, bool SINK>
+__global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 3>)) void win_bwd_dkv_kernel(const WinArgs a, int kg, int qh) {
     using L = Lay<T, DH>;
     using M = Mma<T>;
-    constexpr int TILE = BQ * L::ROWB, STAGE = 2 * TILE + 256;        // Q, dout, {lse2, delta} of 32 queries
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hi = lane >> 5;
-    const int nkt = (a.Tk + BM - 1) / BM;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hi = lane >> 5, key_group = wave % kg, row_group = wave / kg, nw = kg * qh;
+    const int bn = kg * BQ, bq = qh * BQ, tile = qh * L::bytes(BQ), stage = 2 * tile + qh * 256;        // Q, dout, statistics of bq queries
+    const int keys = SINK ? a.sink_keys : a.Tk, nkt = (keys + bn - 1) / bn;
     int item = xcd_item();
-    const int kt = item % nkt; item /= nkt;                           // the tile with the sinks first: every query sees it
+    int chunk = 0;
+    if (SINK) { chunk = item % a.chunks; item /= a.chunks; }
+    const int kt = item % nkt; item /= nkt;
     const int hk = item % a.Hkv, n = item / a.Hkv;
     const Seq sq = sequence(a, n);
-    const int jb = kt * BM, j = jb + wave * 32 + (lane & 31), jc = min(j, a.Tk - 1);
-    const bool seen = j < sq.kvl && (!a.key_mask || a.key_mask[(size_t)n * a.Tk + jc]);
-    // rows of queries that see key jj: [lo, hi)
+    const int jb = kt * bn, j = jb + key_group * BQ + (lane & 31), jc = min(j, a.Tk - 1);
+    const bool seen = j < min(sq.kvl, keys) && (!a.key_mask || a.key_mask[(size_t)n * a.Tk + jc]);
+    // rows of queries whose window holds key jj: [first_row, end_row); the rows behind them see it if it is a sink
     auto first_row = [&](int jj) { return a.right < 0 ? 0 : clampi(jj - a.right - sq.pos, 0, a.Tq); };
-    auto end_row = [&](int jj) { return a.left < 0 || jj < a.sinks ? a.Tq : clampi(jj + a.left - sq.pos + 1, 0, a.Tq); };
-    const int lo = seen ? first_row(j) : 0, end = seen ? end_row(j) : 0;
-    const int last = min(jb + BM, sq.kvl) - 1;                        // last key of the tile that exists
+    auto end_row = [&](int jj) { return a.left < 0 || jj < a.near_sinks ? a.Tq : clampi(jj + a.left - sq.pos + 1, 0, a.Tq); };
+    auto behind = [&](int jj) { return max(first_row(jj), end_row(jj)); };
+    const int lo = !seen ? 0 : SINK ? behind(j) : first_row(j), end = !seen ? 0 : SINK ? a.Tq : end_row(j);
+    const int last = min(min(jb + bn, keys), sq.kvl) - 1;                     // last key of the tile that exists
     int r0 = 0, r1 = 0;
-    if (last >= jb) { r0 = first_row(jb) & ~(BQ - 1); r1 = jb < a.sinks ? a.Tq : end_row(last); }
-    const int nq = r1 > r0 ? (r1 - r0 + BQ - 1) / BQ : 0, nt = nq * a.G;
+    if (last >= jb) { r0 = (SINK ? behind(jb) : first_row(jb)) & ~(BQ - 1); r1 = SINK || jb < a.near_sinks ? a.Tq : end_row(last); }
+    const int nq = r1 > r0 ? (r1 - r0 + bq - 1) / bq : 0;
+    int t0 = 0, t1 = nq * a.G;                                                // tiles of queries, head by head
+    if (SINK) { const int per = (t1 + a.chunks - 1) / a.chunks; t0 = min(chunk * per, t1); t1 = min(t0 + per, t1); }
 
     typename M::Frag kf[L::NF], vf[L::NF];
     {
@@ -437,32 +489,38 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void win_bwd_dkv_kerne
     const long long qst = a.sq.t * (long long)sizeof(T), dst = a.sdo.t * (long long)sizeof(T);
     const unsigned lds = (unsigned)(uintptr_t)(LDS_PTR(char))smem;
     auto issue = [&](int t, int buf) {
-        const int h = hk * a.G + t / nq, i0 = r0 + (t % nq) * BQ;
-        const unsigned long long valid = below(a.Tq - i0);
-        const unsigned at = lds + buf * STAGE;
-        load_tile<T, DH, BQ, NWAVE>((const char*)((const T*)a.q + n * a.sq.n + h * a.sq.h) + i0 * qst, (unsigned)qst, valid, at, wave, lane);
-        load_tile<T, DH, BQ, NWAVE>((const char*)((const T*)a.dout + n * a.sdo.n + h * a.sdo.h) + i0 * dst, (unsigned)dst, valid, at + TILE, wave, lane);
-        if (wave == 0) dma4((unsigned)lane * 4u, tile_rsrc(a.stats + stats_at(a, n, h, i0)), at + 2 * TILE);
+        const int h = hk * a.G + t / nq, i0 = r0 + (t % nq) * bq;
+        const unsigned at = lds + buf * stage;
+        for (int r = 0; r < qh; ++r) {                                        // 32 rows at a time
+            const int ir = i0 + r * BQ;
+            if (ir >= a.Tq) break;                                            // (the rows of that group are masked out below)
+            const unsigned long long valid = below(a.Tq - ir);
+            load_tile<T, DH, BQ>((const char*)((const T*)a.q + n * a.sq.n + h * a.sq.h) + ir * qst, (unsigned)qst, valid, at + r * L::bytes(BQ), wave, nw, lane);
+            load_tile<T, DH, BQ>((const char*)((const T*)a.dout + n * a.sdo.n + h * a.sdo.h) + ir * dst, (unsigned)dst, valid, at + tile + r * L::bytes(BQ), wave, nw, lane);
+            if (wave == r % nw) dma4((unsigned)lane * 4u, tile_rsrc(a.stats + stats_at(a, n, h, ir)), at + 2 * tile + r * 256);
+        }
     };
     f32x16 dk[L::ND], dv[L::ND];
 #pragma unroll
     for (int d = 0; d < L::ND; ++d) { dk[d] = zero16(); dv[d] = zero16(); }
-    if (nt > 0) issue(0, 0);
-    for (int t = 0; t < nt; ++t) {
+    if (t0 < t1) issue(t0, 0);
+    for (int t = t0; t < t1; ++t) {
         dma_barrier();
-        if (t + 1 < nt) issue(t + 1, (t + 1) & 1);
-        const char* qt = smem + (t & 1) * STAGE;
-        const char* dt = qt + TILE;
-        const float* st2 = (const float*)(qt + 2 * TILE);
-        const int i0 = r0 + (t % nq) * BQ;
+        const int buf = (t - t0) & 1;
+        if (t + 1 < t1) issue(t + 1, buf ^ 1);
+        const char* qt = smem + buf * stage + row_group * L::bytes(BQ);
+        const char* dt = qt + tile;
+        const float* st2 = (const float*)(smem + buf * stage + 2 * tile + row_group * 256);
+        const int i0 = r0 + (t % nq) * bq + row_group * BQ;
         const unsigned bits = (unsigned)(below(min(end - i0, 32)) & ~below(lo - i0));
         if (__any(bits != 0)) {
             f32x16 s = zero16(), dp = zero16();
 #pragma unroll
             for (int f = 0; f < L::NF; ++f) {
-                s = M::mac(row_frag<T, DH>(qt, lane & 31, f, hi), kf[f], s);
-                dp = M::mac(row_frag<T, DH>(dt, lane & 31, f, hi), vf[f], dp);
+                s = M::mac(row_frag<T, DH>(qt, f, lane), kf[f], s);
+                dp = M::mac(row_frag<T, DH>(dt, f, lane), vf[f], dp);
             }
+            __builtin_amdgcn_sched_barrier(0);
             const unsigned w = bits >> (4 * hi);
 #pragma unroll
             for (int r = 0; r < 16; r += 4) {
@@ -475,14 +533,61 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void win_bwd_dkv_kerne
                     dp[r + e] = on ? p * (dp[r + e] - de[e]) : 0.f;
                 }
             }
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int d = 0; d < L::ND; ++d) {
-                dv[d] = M::template mac_t<DH>(dt, 0, d, s, dv[d], lane);
-                dk[d] = M::template mac_t<DH>(qt, 0, d, dp, dk[d], lane);
+                dv[d] = M::template mac_t<DH>(dt, d, s, dv[d], lane);
+                dk[d] = M::template mac_t<DH>(qt, d, dp, dk[d], lane);
             }
         }
     }
+    if (qh > 1) {                                                             // add the row groups' sums: a lane's 16 ND values lie 64 apart
+        auto add = [&](f32x16 (&acc)[L::ND]) {
+            float* at = (float*)smem + key_group * 64 * 16 * L::ND + lane;
+            const int group = kg * 64 * 16 * L::ND;
+            __syncthreads();
+            if (row_group > 0)
+#pragma unroll
+                for (int d = 0; d < L::ND; ++d)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) at[(row_group - 1) * group + (d * 16 + r) * 64] = acc[d][r];
+            __syncthreads();
+            if (row_group == 0)
+                for (int g = 0; g + 1 < qh; ++g)
+#pragma unroll
+                    for (int d = 0; d < L::ND; ++d)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) acc[d][r] += at[g * group + (d * 16 + r) * 64];
+        };
+        add(dk);
+        add(dv);
+        if (row_group > 0) return;
+    }
+    if (SINK) {
+        if (j < a.sink_rows) {
+            float* o = a.sinks_ws + (((long long)(n * a.Hkv + hk) * a.chunks + chunk) * a.sink_rows + j) * 2 * DH;
+#pragma unroll
+            for (int d = 0; d < L::ND; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; r += 4) {
+                    *(f32x4*)(o + 32 * d + tok(r, hi)) = f32x4{dk[d][r], dk[d][r + 1], dk[d][r + 2], dk[d][r + 3]};
+                    *(f32x4*)(o + DH + 32 * d + tok(r, hi)) = f32x4{dv[d][r], dv[d][r + 1], dv[d][r + 2], dv[d][r + 3]};
+                }
+        }
+        return;
+    }
     if (j < a.Tk) {
+        for (int c = 0; j < a.sink_keys && c < a.chunks; ++c) {
+            const float* o = a.sinks_ws + (((long long)(n * a.Hkv + hk) * a.chunks + c) * a.sink_rows + j) * 2 * DH;
+#pragma unroll
+            for (int d = 0; d < L::ND; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; r += 4) {
+                    const f32x4 x = *(const f32x4*)(o + 32 * d + tok(r, hi)), y = *(const f32x4*)(o + DH + 32 * d + tok(r, hi));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) { dk[d][r + e] += x[e]; dv[d][r + e] += y[e]; }
+                }
+        }
         T* ok = (T*)a.dk + n * a.sdk.n + j * a.sdk.t + hk * a.sdk.h;
         T* ov = (T*)a.dv + n * a.sdv.n + j * a.sdv.t + hk * a.sdv.h;
 #pragma unroll
@@ -495,14 +600,185 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void win_bwd_dkv_kerne
     }
 }
 
+// ------------------------------------------------------------------------------------------------ few query rows against many keys
+// The G Tq <= 32 rows of one key head as one 32-column tile, the keys in 32-row tiles that the workgroup's waves take in turn, each with its own running
+// maximum and sum and its own pair of LDS tiles (no barrier: a wave waits for its own DMA, counted, while the next tile is in flight).  The waves are
+// merged through LDS; with `splits` > 1 several workgroups share the keys and win_merge_kernel joins their partial results.  Bound by memory, so P is kept
+// as the sum of two bf16 numbers: the second product costs nothing.
+constexpr int FEW = 32;
+template <int N> __device__ __forceinline__ void wait_dma() { asm volatile("s_waitcnt vmcnt(%c0)" ::"i"(N) : "memory"); }
+template <typename T, int DH> struct Few {
+    using L = Lay<T, DH>;
+    static constexpr int TILE = L::bytes(FEW), PIECES = 2 * FEW / L::PIECE_ROWS, NW = PIECES <= 16 ? 4 : 2;
+    static constexpr int MERGE = NW * FEW * (DH + 2) * 4, STAGES = NW * 4 * TILE, LDS = MERGE > STAGES ? MERGE : STAGES;
+};
+template <typename T, int DH>
+__global__ __launch_bounds__((64 * Few<T, DH>::NW), 1) void win_few_kernel(const WinArgs a, int splits) {
+    using L = Lay<T, DH>;
+    using M = Mma<T>;
+    using F = Few<T, DH>;
+    constexpr int NW = F::NW, TILE = F::TILE;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hi = lane >> 5, r = lane & 31, rows = a.G * a.Tq;
+    int item = blockIdx.x;
+    const int split = item % splits; item /= splits;
+    const int hk = item % a.Hkv, n = item / a.Hkv;
+    const Seq sq = sequence(a, n);
+    const int rc = min(r, rows - 1), g = rc / a.Tq, i = rc - g * a.Tq, h = hk * a.G + g;
+    Walk wk = walk_of(a, sq.pos, sq.pos + a.Tq - 1, sq.kvl, FEW);
+    Span sp = span_of(a, sq.pos + i, sq.kvl);
+    const Span s0 = span_of(a, sq.pos, sq.kvl), s1 = span_of(a, sq.pos + a.Tq - 1, sq.kvl);           // every row sees [s1.lo, s0.hi)
+    const int per = (wk.nt + splits - 1) / splits, t0 = min(split * per, wk.nt), t1 = min(t0 + per, wk.nt);
+
+    typename M::Frag qf[L::NF];
+    {
+        const char* p = (const char*)((const T*)a.q + n * a.sq.n + i * a.sq.t + h * a.sq.h);
+#pragma unroll
+        for (int s = 0; s < L::NF; ++s) qf[s] = *(const typename M::Frag*)(p + 32 * s + 16 * hi);
+    }
+    const char* kb = (const char*)((const T*)a.k + n * a.sk.n + hk * a.sk.h);
+    const char* vb = (const char*)((const T*)a.v + n * a.sv.n + hk * a.sv.h);
+    const long long kst = a.sk.t * (long long)sizeof(T), vst = a.sv.t * (long long)sizeof(T);
+    char* mine = smem + wave * 4 * TILE;
+    const unsigned lds = (unsigned)(uintptr_t)(LDS_PTR(char))mine;
+    auto valid_of = [&](int byte, int j0) { return __ballot(byte != 0) & below(min(FEW, wk.kvl - j0)); };
+    auto issue = [&](int j0, unsigned long long valid, int buf) {
+        load_tile<T, DH, FEW>(kb + j0 * kst, (unsigned)kst, valid, lds + buf * 2 * TILE, 0, 1, lane);
+        load_tile<T, DH, FEW>(vb + j0 * vst, (unsigned)vst, valid, lds + buf * 2 * TILE + TILE, 0, 1, lane);
+    };
+    f32x16 acc[L::ND];
+#pragma unroll
+    for (int d = 0; d < L::ND; ++d) acc[d] = zero16();
+    float m = -INFINITY, l = 0.f;
+    int t = t0 + wave, buf = 0, byte = 1;
+    unsigned long long valid = 0, next = 0;
+    if (t < t1) {
+        valid = valid_of(mask_byte(a, n, wk.j0(t, FEW) + r), wk.j0(t, FEW));
+        issue(wk.j0(t, FEW), valid, 0);
+        if (t + NW < t1) byte = mask_byte(a, n, wk.j0(t + NW, FEW) + r);
+    }
+    for (; t < t1; t += NW) {
+        const int j0 = wk.j0(t, FEW);
+        const bool more = t + NW < t1;
+        if (more) {
+            next = valid_of(byte, wk.j0(t + NW, FEW));
+            if (t + 2 * NW < t1) byte = mask_byte(a, n, wk.j0(t + 2 * NW, FEW) + r);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");       // this wave has read the tile that is refilled
+            issue(wk.j0(t + NW, FEW), next, buf ^ 1);
+            wait_dma<F::PIECES>();
+        } else wait_dma<0>();
+        const char* kt = mine + buf * 2 * TILE;
+        const char* vt = kt + TILE;
+        f32x16 st = zero16();
+#pragma unroll
+        for (int s = 0; s < L::NF; ++s) st = M::mac(row_frag<T, DH>(kt, s, lane), qf[s], st);
+        if (!(j0 >= s1.lo && j0 + FEW <= s0.hi && valid == below(FEW))) {
+            const unsigned w = (unsigned)(visible(sp, j0) & valid) >> (4 * hi);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) st[e] = (w >> tok(e, 0)) & 1u ? st[e] : -INFINITY;
+        }
+        float mt = st[0];
+#pragma unroll
+        for (int e = 1; e < 16; ++e) mt = fmaxf(mt, st[e]);
+        mt = fmaxf(mt, __shfl_xor(mt, 32, 64)) * a.c;
+        if (__any(mt > m + 8.f)) {
+            const float mn = fmaxf(m, mt), f = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+            m = mn;
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < L::ND; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[d][e] *= f;
+        }
+        const float mm = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) { st[e] = __builtin_amdgcn_exp2f(fmaf(st[e], a.c, -mm)); l += st[e]; }
+#pragma unroll
+        for (int d = 0; d < L::ND; ++d) acc[d] = M::template mac_t<DH>(vt, d, st, acc[d], lane);
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) st[e] -= bf2f(f2bf(st[e]));
+#pragma unroll
+            for (int d = 0; d < L::ND; ++d) acc[d] = M::template mac_t<DH>(vt, d, st, acc[d], lane);
+        }
+        valid = next;
+        buf ^= 1;
+    }
+    l += __shfl_xor(l, 32, 64);
+    __syncthreads();                                                          // the tiles are done with: their LDS takes the waves' results
+    float* part = (float*)smem;                                               // [NW][32][DH], then [NW][32] of m and of l
+    float* pm = part + NW * FEW * DH;
+    float* pl = pm + NW * FEW;
+#pragma unroll
+    for (int d = 0; d < L::ND; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4)
+            *(f32x4*)(part + (wave * FEW + r) * DH + 4 * (((32 * d + tok(e, hi)) >> 2) ^ (r & 7))) = f32x4{acc[d][e], acc[d][e + 1], acc[d][e + 2], acc[d][e + 3]};
+    if (hi == 0) { pm[wave * FEW + r] = m; pl[wave * FEW + r] = l; }
+    __syncthreads();
+    for (int e = threadIdx.x; e < rows * (DH / 4); e += 64 * NW) {
+        const int row = e / (DH / 4), d = e - row * (DH / 4), gg = row / a.Tq, ii = row - gg * a.Tq, hh = hk * a.G + gg;
+        float top = -INFINITY, total = 0.f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) top = fmaxf(top, pm[w * FEW + row]);
+        const float base = top == -INFINITY ? 0.f : top;
+        f32x4 o{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            const float f = __builtin_amdgcn_exp2f(pm[w * FEW + row] - base);
+            total += f * pl[w * FEW + row];
+            o = o + *(const f32x4*)(part + (w * FEW + row) * DH + 4 * (d ^ (row & 7))) * f;
+        }
+        if (splits > 1) {
+            const long long at = (((long long)n * a.Hkv + hk) * splits + split) * rows + row;
+            *(f32x4*)(a.parts + at * DH + 4 * d) = o;
+            if (d == 0) { float* ml = a.parts + (long long)a.N * a.Hkv * splits * rows * DH + 2 * at; ml[0] = top; ml[1] = total; }
+        } else {
+            const float inv = total == 0.f ? 0.f : 1.f / total;
+            M::st4((T*)a.out + n * a.so.n + ii * a.so.t + hh * a.so.h + 4 * d, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+            if (d == 0 && a.lse) a.lse[((long long)n * a.H + hh) * a.Tq + ii] = total == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * LN2;
+        }
+    }
+}
+// one row per wave: the splits' partial results into out and lse
+template <typename T, int DH>
+__global__ __launch_bounds__(256) void win_merge_kernel(const WinArgs a, int splits) {
+    const int lane = threadIdx.x & 63, rows = a.G * a.Tq;
+    const long long units = (long long)a.N * a.Hkv, at = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (at >= units * rows) return;
+    const long long unit = at / rows;
+    const int row = (int)(at - unit * rows), g = row / a.Tq, i = row - g * a.Tq, n = (int)(unit / a.Hkv), h = (int)(unit % a.Hkv) * a.G + g;
+    const float* ml = a.parts + units * splits * rows * DH;
+    float top = -INFINITY, total = 0.f, o[DH / 64];
+    for (int s = 0; s < splits; ++s) top = fmaxf(top, ml[2 * ((unit * splits + s) * rows + row)]);
+    const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int e = 0; e < DH / 64; ++e) o[e] = 0.f;
+    for (int s = 0; s < splits; ++s) {
+        const long long k = (unit * splits + s) * rows + row;
+        const float f = __builtin_amdgcn_exp2f(ml[2 * k] - base);
+        total += f * ml[2 * k + 1];
+#pragma unroll
+        for (int e = 0; e < DH / 64; ++e) o[e] += f * a.parts[k * DH + 64 * e + lane];
+    }
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    T* p = (T*)a.out + n * a.so.n + i * a.so.t + h * a.so.h;
+#pragma unroll
+    for (int e = 0; e < DH / 64; ++e) Elem<T>::st(p + 64 * e + lane, o[e] * inv);
+    if (lane == 0 && a.lse) a.lse[((long long)n * a.H + h) * a.Tq + i] = total == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * LN2;
+}
+
 // ------------------------------------------------------------------------------------------------ host side
-bool fits(const DicStrides& s, long long tokens, int size) {
+// The stride of a dimension of one element is never used, and may be anything.
+Strides st(const DicStrides& s, int N, int T, int H) { return Strides{N > 1 ? s.n : 0, T > 1 ? s.t : 0, H > 1 ? s.h : 0}; }
+bool fits(const DicStrides& d, int N, int T, int H, int size) {
     // 16-byte rows, and 64 rows of a tile inside a descriptor's 31-bit range
-    return s.n % (16 / size) == 0 && s.t % (16 / size) == 0 && s.h % (16 / size) == 0 && s.n >= 0 && s.t >= 0 && s.h >= 0 && (tokens <= 1 || s.t <= (1ll << 24) / size);
+    const Strides s = st(d, N, T, H);
+    const int per = 16 / size;
+    return s.n % per == 0 && s.t % per == 0 && s.h % per == 0 && s.n >= 0 && s.t >= 0 && s.h >= 0 && s.t <= (1ll << 24) / size;
 }
 bool apart(const DicStrides& s, int N, int T, int H, int dh) { return (N <= 1 || s.n >= dh) && (T <= 1 || s.t >= dh) && (H <= 1 || s.h >= dh); }
 bool aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
-Strides st(const DicStrides& s) { return Strides{s.n, s.t, s.h}; }
 
 int check(int dtype, const DicWinAttnParams* p, bool bwd, bool pointers = true) {
     DIC_REQUIRE(p != nullptr, "dic_win_attn: no parameters");
@@ -512,64 +788,142 @@ int check(int dtype, const DicWinAttnParams* p, bool bwd, bool pointers = true) 
     DIC_REQUIRE(p->N >= 0 && p->Tq >= 0 && p->Tk >= 0 && p->Tq <= (1 << 28) && p->Tk <= (1 << 28), "dic_win_attn: sizes out of range");
     DIC_REQUIRE(p->H > 0 && p->Hkv > 0 && p->H % p->Hkv == 0, "dic_win_attn: the number of heads must be a multiple of the number of key heads");
     DIC_REQUIRE(p->sinks >= 0 && std::isfinite(p->scale) && p->scale > 0.f, "dic_win_attn: sinks >= 0 and a positive finite scale are needed");
-    const long long tiles_q = ((long long)p->Tq + BM - 1) / BM, tiles_k = ((long long)p->Tk + BM - 1) / BM;
-    DIC_REQUIRE((long long)p->N * p->H * tiles_q < (1ll << 31) && (long long)p->N * p->Hkv * tiles_k < (1ll << 31), "dic_win_attn: too many tiles for one launch");
+    DIC_REQUIRE((long long)p->N * p->H * (p->Tq / 32 + 1) < (1ll << 31) && (long long)p->N * p->Hkv * (p->Tk / 32 + 1) < (1ll << 31), "dic_win_attn: too many tiles for one launch");
     if (!pointers) return 0;
     const bool nq = p->N && p->Tq, nk = p->N && p->Tk;
     DIC_REQUIRE(!nq || (p->q && (bwd ? p->out && p->lse && p->dout && p->dq : p->out != nullptr)), "dic_win_attn: null query-side pointer");
     DIC_REQUIRE(!nk || (p->k && p->v && (!bwd || (p->dk && p->dv))), "dic_win_attn: null key-side pointer");
     DIC_REQUIRE(aligned(p->q) && aligned(p->k) && aligned(p->v) && aligned(p->out) && (!bwd || (aligned(p->dout) && aligned(p->dq) && aligned(p->dk) && aligned(p->dv))),
                 "dic_win_attn: pointers must be 16-byte aligned");
-    DIC_REQUIRE(fits(p->q_stride, p->Tq, size) && fits(p->out_stride, p->Tq, size) && fits(p->k_stride, p->Tk, size) && fits(p->v_stride, p->Tk, size)
-                && (!bwd || (fits(p->dout_stride, p->Tq, size) && fits(p->dq_stride, p->Tq, size) && fits(p->dk_stride, p->Tk, size) && fits(p->dv_stride, p->Tk, size))),
+    auto rows_q = [&](const DicStrides& d) { return fits(d, p->N, p->Tq, p->H, size); };
+    auto rows_k = [&](const DicStrides& d) { return fits(d, p->N, p->Tk, p->Hkv, size); };
+    DIC_REQUIRE((!nq || (rows_q(p->q_stride) && rows_q(p->out_stride) && (!bwd || (rows_q(p->dout_stride) && rows_q(p->dq_stride)))))
+                && (!nk || (rows_k(p->k_stride) && rows_k(p->v_stride) && (!bwd || (rows_k(p->dk_stride) && rows_k(p->dv_stride))))),
                 "dic_win_attn: strides must be non-negative multiples of 16 bytes, and a token stride at most 16 MiB");
     DIC_REQUIRE(bwd ? apart(p->dq_stride, p->N, p->Tq, p->H, p->dh) && apart(p->dk_stride, p->N, p->Tk, p->Hkv, p->dh) && apart(p->dv_stride, p->N, p->Tk, p->Hkv, p->dh)
                     : apart(p->out_stride, p->N, p->Tq, p->H, p->dh), "dic_win_attn: rows of an output overlap");
     return 0;
 }
+// Query rows in waves of 32: all of them in one workgroup where that takes at most 8 waves (fp32: 4), which then loads the keys once (130 rows x 3072 heads
+// forward: 86 us with 5 waves, 113 us with 4 and a second workgroup for 2 rows); else 4, one to a SIMD (2050 rows: 61 us with 4, 111 us with 5).
+int waves_of(int rows, int most) {
+    const int waves = (rows + BQ - 1) / BQ;
+    return waves <= most ? waves : 4;
+}
+// The dk / dv kernel's workgroup: kg groups of 32 keys and qh groups of 32 query rows.  Few key tiles: fewer keys and more rows to a workgroup.
+struct Shape { int kg, qh; };
+Shape shape_of(const WinArgs& a, int most, int most_rows) {
+    const int waves = (a.Tk + BQ - 1) / BQ;
+    const long long heads = (long long)a.N * a.Hkv;
+    if (waves <= most && heads >= 256) return {waves, 1};
+    for (int kg = 4; kg > 1; kg >>= 1) if (heads * ((waves + kg - 1) / kg) >= 512) return {kg, 4 / kg < most_rows ? 4 / kg : most_rows};
+    return {1, most_rows};
+}
+template <typename T, int DH> constexpr int ROW_GROUPS = Lay<T, DH>::ROWB <= 256 ? 4 : 2;       // at most: two stages of 512-byte rows fill 132 KB of LDS with 2
+// Pieces of the sink pass: about 256 workgroups, and no more than 16 partial sums for the window pass to add.
+void plan_sinks(WinArgs& a) {
+    a.near_sinks = a.left >= 0 ? (a.sinks < a.Tk ? a.sinks : a.Tk) : 0;
+    // The sinks' tile walks Tq rows, another one about left + right + 128 of them: it needs no pass of its own while the card has as much else to do
+    // (130 rows in windows of 129, 3072 heads: that pass took 43 us beside the window pass's 150).
+    const long long others = a.right < 0 ? a.Tq : (long long)a.left + a.right + 128, all = (long long)a.N * a.Hkv * ((a.Tk + 127) / 128) * (others < a.Tq ? others : a.Tq);
+    if (a.near_sinks > 0 && a.Tq > 2 * others && a.Tq > all / 256) { a.sink_keys = a.near_sinks; a.near_sinks = 0; }
+    a.sink_rows = (a.sink_keys + BQ - 1) / BQ * BQ;
+    const long long tiles = (long long)a.N * a.Hkv * (a.sink_rows / BQ), most = (long long)a.G * ((a.Tq + 4 * BQ - 1) / (4 * BQ));
+    const long long want = tiles ? (256 + tiles - 1) / tiles : 1;
+    a.chunks = (int)(want < most ? want : most);
+    if (a.chunks > 16) a.chunks = 16;
+    if (a.chunks < 1) a.chunks = 1;
+}
+long long sink_floats(const WinArgs& a, int dh) { return (long long)a.N * a.Hkv * a.chunks * a.sink_rows * 2 * dh; }
+// Few query rows: one workgroup per key head and sequence, or several that share the keys while that fills the card and leaves each 8 tiles to read.
+bool few_rows(const WinArgs& a) { return a.G * (long long)a.Tq <= FEW && a.Tk > 64; }
+int splits_of(const WinArgs& a) {
+    const long long seen = a.left < 0 || a.right < 0 ? a.Tk : (long long)a.left + a.right + a.Tq + 2 * FEW + (a.sinks < a.Tk ? a.sinks : a.Tk);
+    const long long tiles = ((seen < a.Tk ? seen : a.Tk) + FEW - 1) / FEW, units = (long long)a.N * a.Hkv, want = (512 + units - 1) / units, most = tiles / 8;
+    const long long s = want < most ? want : most;
+    return s > 1 ? (int)s : 1;
+}
+long long parts_floats(const WinArgs& a, int dh) {
+    const int s = few_rows(a) ? splits_of(a) : 1;
+    return s > 1 ? (long long)a.N * a.Hkv * s * a.G * a.Tq * (dh + 2) : 0;
+}
+size_t ws_bytes(const WinArgs& a, int dh, bool backward) {
+    if (!backward) return (size_t)parts_floats(a, dh) * sizeof(float);
+    return (size_t)(stats_floats(a.N, a.H, a.Tq) + sink_floats(a, dh)) * sizeof(float);
+}
+
 WinArgs args_of(const DicWinAttnParams* p) {
     WinArgs a{};
     a.q = p->q; a.k = p->k; a.v = p->v; a.o = p->out; a.out = p->out; a.dout = p->dout;
     a.dq = p->dq; a.dk = p->dk; a.dv = p->dv; a.lse = p->lse;
-    a.sq = st(p->q_stride); a.sk = st(p->k_stride); a.sv = st(p->v_stride); a.so = st(p->out_stride);
-    a.sdo = st(p->dout_stride); a.sdq = st(p->dq_stride); a.sdk = st(p->dk_stride); a.sdv = st(p->dv_stride);
+    auto rows_q = [&](const DicStrides& d) { return st(d, p->N, p->Tq, p->H); };
+    auto rows_k = [&](const DicStrides& d) { return st(d, p->N, p->Tk, p->Hkv); };
+    a.sq = rows_q(p->q_stride); a.sk = rows_k(p->k_stride); a.sv = rows_k(p->v_stride); a.so = rows_q(p->out_stride);
+    a.sdo = rows_q(p->dout_stride); a.sdq = rows_q(p->dq_stride); a.sdk = rows_k(p->dk_stride); a.sdv = rows_k(p->dv_stride);
     a.key_mask = p->key_mask; a.kv_len = p->kv_len; a.q_pos = p->q_pos;
     a.N = p->N; a.Tq = p->Tq; a.Tk = p->Tk; a.H = p->H; a.Hkv = p->Hkv; a.G = p->H / p->Hkv;
     a.left = p->left < 0 ? -1 : (p->left < FAR / 2 ? p->left : FAR / 2);
     a.right = p->right < 0 ? -1 : (p->right < FAR / 2 ? p->right : FAR / 2);
     a.sinks = p->sinks; a.scale = p->scale; a.c = p->scale * LOG2E;
+    plan_sinks(a);
     return a;
 }
-template <typename K> int launch(K kernel, long long blocks, size_t lds, const WinArgs& a, hipStream_t st) {
-    // (set on every launch: the attribute belongs to the current device's copy of the kernel)
-    hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    if (e != hipSuccess) { dic_set_error(hipGetErrorString(e)); return (int)e; }
-    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), lds, st, a);
+template <typename K, typename... More> int launch(K kernel, long long blocks, int threads, size_t lds, hipStream_t st, More... more) {
+    if (lds > (64 << 10)) {                     // once for each device: the attribute belongs to its copy of the kernel
+        static std::atomic<unsigned long long> allowed{0};
+        int dev = 0;
+        hipError_t e = hipGetDevice(&dev);
+        if (e == hipSuccess && !((allowed.load(std::memory_order_relaxed) >> (dev & 63)) & 1)) {
+            e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 160 << 10);
+            if (e == hipSuccess) allowed.fetch_or(1ull << (dev & 63), std::memory_order_relaxed);
+        }
+        if (e != hipSuccess) { dic_set_error(hipGetErrorString(e)); return (int)e; }
+    }
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), lds, st, more...);
     DIC_CHECK_LAUNCH();
     return 0;
 }
 template <typename T, int DH> int fwd(const WinArgs& a, hipStream_t st) {
     constexpr int BN = sizeof(T) == 2 ? 64 : 32;
-    return launch(win_fwd_kernel<T, DH, BN>, (long long)a.N * a.H * ((a.Tq + BM - 1) / BM), (size_t)4 * BN * Lay<T, DH>::ROWB, a, st);
+    if (few_rows(a)) {
+        const int splits = splits_of(a);
+        if (int rc = launch(win_few_kernel<T, DH>, (long long)a.N * a.Hkv * splits, 64 * Few<T, DH>::NW, Few<T, DH>::LDS, st, a, splits)) return rc;
+        return splits > 1 ? launch(win_merge_kernel<T, DH>, ((long long)a.N * a.H * a.Tq + 3) / 4, 256, 0, st, a, splits) : 0;
+    }
+    const int w = waves_of(a.Tq, MOST_WAVES<T>);
+    return launch(win_fwd_kernel<T, DH, BN>, (long long)a.N * a.H * ((a.Tq + w * BQ - 1) / (w * BQ)), 64 * w, (size_t)4 * Lay<T, DH>::bytes(BN), st, a);
+}
+template <typename T, int DH> size_t dkv_lds(int kg, int qh) {
+    const size_t stages = (size_t)2 * qh * (2 * Lay<T, DH>::bytes(BQ) + 256), sums = (size_t)(qh - 1) * kg * BQ * DH * sizeof(float);
+    return stages > sums ? stages : sums;
 }
 template <typename T, int DH> int bwd(const WinArgs& a, hipStream_t st) {
     constexpr int BN = sizeof(T) == 2 ? 64 : 32;
-    if (a.Tq > 0)
-        if (int rc = launch(win_bwd_dq_kernel<T, DH, BN>, (long long)a.N * a.H * ((a.Tq + BM - 1) / BM), (size_t)4 * BN * Lay<T, DH>::ROWB, a, st)) return rc;
-    if (a.Tk > 0) return launch(win_bwd_dkv_kernel<T, DH>, (long long)a.N * a.Hkv * ((a.Tk + BM - 1) / BM), (size_t)2 * (2 * BQ * Lay<T, DH>::ROWB + 256), a, st);
-    return 0;
+    if (a.Tq > 0) {
+        const int w = waves_of(a.Tq, MOST_WAVES<T>);
+        if (int rc = launch(win_bwd_dq_kernel<T, DH, BN>, (long long)a.N * a.H * ((a.Tq + w * BQ - 1) / (w * BQ)), 64 * w, (size_t)4 * Lay<T, DH>::bytes(BN), st, a)) return rc;
+    }
+    if (a.Tk == 0) return 0;
+    if (a.sink_keys > 0)
+        if (int rc = launch(win_bwd_dkv_kernel<T, DH, true>, (long long)a.N * a.Hkv * (a.sink_rows / BQ) * a.chunks, 64 * ROW_GROUPS<T, DH>,
+                            dkv_lds<T, DH>(1, ROW_GROUPS<T, DH>), st, a, 1, ROW_GROUPS<T, DH>)) return rc;
+    const Shape s = shape_of(a, MOST_WAVES<T>, ROW_GROUPS<T, DH>);
+    return launch(win_bwd_dkv_kernel<T, DH, false>, (long long)a.N * a.Hkv * ((a.Tk + s.kg * BQ - 1) / (s.kg * BQ)), 64 * s.kg * s.qh, dkv_lds<T, DH>(s.kg, s.qh), st, a, s.kg, s.qh);
 }
 }  // namespace
 
 extern "C" size_t dic_win_attn_ws_bytes(int dtype, int backward, const DicWinAttnParams* p) {
     if (check(dtype, p, false, false)) return 0;
-    return backward ? (size_t)stats_floats(p->N, p->H, p->Tq) * sizeof(float) : 0;
+    return ws_bytes(args_of(p), p->dh, backward != 0);
 }
 
 extern "C" int dic_win_attn_fwd(int dtype, const DicWinAttnParams* p, void* stream) {
     if (int rc = check(dtype, p, false)) return rc;
     if (p->N == 0 || p->Tq == 0) return 0;
-    const WinArgs a = args_of(p);
+    WinArgs a = args_of(p);
+    const size_t need = ws_bytes(a, p->dh, false);
+    DIC_REQUIRE(need == 0 || (p->ws && aligned(p->ws) && p->ws_bytes >= need), "dic_win_attn_fwd: workspace missing or too small (dic_win_attn_ws_bytes)");
+    a.parts = (float*)p->ws;
     hipStream_t st = (hipStream_t)stream;
     if (dtype == DIC_BF16) return p->dh == 64 ? fwd<bf16_t, 64>(a, st) : fwd<bf16_t, 128>(a, st);
     return p->dh == 64 ? fwd<float, 64>(a, st) : fwd<float, 128>(a, st);
@@ -578,10 +932,11 @@ extern "C" int dic_win_attn_fwd(int dtype, const DicWinAttnParams* p, void* stre
 extern "C" int dic_win_attn_bwd(int dtype, const DicWinAttnParams* p, void* stream) {
     if (int rc = check(dtype, p, true)) return rc;
     if (p->N == 0) return 0;
-    const size_t need = (size_t)stats_floats(p->N, p->H, p->Tq) * sizeof(float);
-    DIC_REQUIRE(need == 0 || (p->ws && aligned(p->ws) && p->ws_bytes >= need), "dic_win_attn_bwd: workspace missing or too small (dic_win_attn_ws_bytes)");
     WinArgs a = args_of(p);
+    const size_t need = ws_bytes(a, p->dh, true);
+    DIC_REQUIRE(need == 0 || (p->ws && aligned(p->ws) && p->ws_bytes >= need), "dic_win_attn_bwd: workspace missing or too small (dic_win_attn_ws_bytes)");
     a.stats = (float*)p->ws;
+    a.sinks_ws = a.stats + stats_floats(p->N, p->H, p->Tq);
     hipStream_t st = (hipStream_t)stream;
     if (dtype == DIC_BF16) return p->dh == 64 ? bwd<bf16_t, 64>(a, st) : bwd<bf16_t, 128>(a, st);
     return p->dh == 64 ? bwd<float, 64>(a, st) : bwd<float, 128>(a, st);

@@ -36,6 +36,16 @@ def test_struct_mirrors_follow_the_header(struct, mirror):
     assert getattr(dic._lib, mirror)._fields_ == want
 
 
+def test_packed_params_have_the_structs_sizes():
+    from importlib import import_module
+    block = import_module("diffusion-image-captioning_amd.block")
+    for packed, mirror in ((block._WIN, dic._lib.WinAttnParams), (block._NORM, dic._lib.GatedNormParams)):
+        assert packed.size == C.sizeof(mirror)
+        values = list(range(1, len(mirror._fields_) + 1))
+        got = mirror.from_buffer_copy(packed.pack(*values))
+        assert [getattr(got, n) for n, _ in mirror._fields_] == values
+
+
 def attn(**kw):
     p = dic._lib.WinAttnParams()
     base = dict(N=2, Tq=8, Tk=8, H=4, Hkv=2, dh=64, left=-1, right=-1, scale=0.125, ws=4096, ws_bytes=1 << 20)
