@@ -27,22 +27,34 @@ struct NormArgs {
     float r, inv_d;
 };
 
-// 4 elements from any whole-element address; `cnt` of them exist
-template <typename T> __device__ __forceinline__ f32x4 ld(const T* p, int cnt) {
-    f32x4 v{0.f, 0.f, 0.f, 0.f};
-    if (cnt == 4) {
-        if constexpr (sizeof(T) == 2) {
-            uint2 u;
-            __builtin_memcpy(&u, p, 8);
-            v[0] = __uint_as_float(u.x << 16); v[1] = __uint_as_float(u.x & 0xffff0000u);
-            v[2] = __uint_as_float(u.y << 16); v[3] = __uint_as_float(u.y & 0xffff0000u);
-        } else __builtin_memcpy(&v, p, 16);
-    } else {
-#pragma unroll
-        for (int e = 0; e < 3; ++e) if (e < cnt) v[e] = Elem<T>::ld(p + e);
+// 4 elements as they lie in memory, at any whole-element address; `cnt` of them exist
+template <typename T> struct Raw;
+template <> struct Raw<bf16_t> {
+    uint2 v;
+    __device__ __forceinline__ void load(const bf16_t* p, int cnt) {
+        v = make_uint2(0u, 0u);
+        if (cnt == 4) __builtin_memcpy(&v, p, 8);
+        else if (cnt > 0) {
+            v.x = p[0] | (cnt > 1 ? (unsigned)p[1] << 16 : 0u);
+            v.y = cnt > 2 ? p[2] : 0u;
+        }
     }
-    return v;
-}
+    __device__ __forceinline__ f32x4 f() const {
+        return f32x4{__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u)};
+    }
+};
+template <> struct Raw<float> {
+    f32x4 v;
+    __device__ __forceinline__ void load(const float* p, int cnt) {
+        v = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (cnt == 4) __builtin_memcpy(&v, p, 16);
+        else {
+#pragma unroll
+            for (int e = 0; e < 3; ++e) if (e < cnt) v[e] = p[e];
+        }
+    }
+    __device__ __forceinline__ f32x4 f() const { return v; }
+};
 template <typename T> __device__ __forceinline__ void stv(T* p, f32x4 v, int cnt) {
     if (cnt == 4) {
         if constexpr (sizeof(T) == 2) { const uint2 u = make_uint2(pack2bf(v[0], v[1]), pack2bf(v[2], v[3])); __builtin_memcpy(p, &u, 8); }
@@ -53,34 +65,52 @@ template <typename T> __device__ __forceinline__ void stv(T* p, f32x4 v, int cnt
     }
 }
 
+// Sums over 16 lanes by lane permutations inside the adds (two neighbours, two pairs, two quads, two eights), over a wave by reading the four sums:
+// a row's statistics are two dependent sums, and through LDS (ds_bpermute) each took six round trips.
+template <int CTRL> __device__ __forceinline__ float dpp(float v) { return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true)); }
+__device__ __forceinline__ float sum16(float v) {
+    v += dpp<0xB1>(v);          // quad_perm 1 0 3 2
+    v += dpp<0x4E>(v);          // quad_perm 2 3 0 1
+    v += dpp<0x141>(v);         // row_half_mirror
+    v += dpp<0x140>(v);         // row_mirror
+    return v;
+}
+__device__ __forceinline__ float sum64(float v) {
+    const int s = __float_as_int(sum16(v));
+    return (__int_as_float(__builtin_amdgcn_readlane(s, 0)) + __int_as_float(__builtin_amdgcn_readlane(s, 16)))
+           + (__int_as_float(__builtin_amdgcn_readlane(s, 32)) + __int_as_float(__builtin_amdgcn_readlane(s, 48)));
+}
+
 template <int TPR, int NV> struct Team {
-    static constexpr int THREADS = TPR > 256 ? TPR : 256, TEAMS = THREADS / TPR, WAVES = TPR / 64;
+    static constexpr int THREADS = TPR > 256 ? TPR : 256, TEAMS = THREADS / TPR, WAVES = TPR / 64, WIDTH = TPR * NV * 4;
     int lane, col[NV], cnt[NV];
     __device__ __forceinline__ Team(int D) {
         lane = threadIdx.x % TPR;
 #pragma unroll
         for (int c = 0; c < NV; ++c) { col[c] = (c * TPR + lane) * 4; cnt[c] = D - col[c] < 0 ? 0 : D - col[c] > 4 ? 4 : D - col[c]; }
     }
-    template <typename T> __device__ __forceinline__ void load(const T* p, f32x4 (&v)[NV]) const {
+    template <typename T> __device__ __forceinline__ void load(const void* p, long long at, Raw<T> (&v)[NV]) const {
 #pragma unroll
-        for (int c = 0; c < NV; ++c) v[c] = ld<T>(p + col[c], cnt[c]);
+        for (int c = 0; c < NV; ++c) v[c].load((const T*)p + at + col[c], cnt[c]);
     }
     __device__ __forceinline__ void load_or(const float* p, float other, f32x4 (&v)[NV]) const {
-        if (p) load<float>(p, v);
-        else {
 #pragma unroll
-            for (int c = 0; c < NV; ++c) v[c] = f32x4{other, other, other, other};
+        for (int c = 0; c < NV; ++c) {
+            Raw<float> r;
+            r.v = f32x4{other, other, other, other};
+            if (p) r.load(p + col[c], cnt[c]);
+            v[c] = r.v;
         }
     }
-    template <typename T> __device__ __forceinline__ void store(T* p, const f32x4 (&v)[NV]) const {
+    template <typename T> __device__ __forceinline__ void store(void* p, long long at, const f32x4 (&v)[NV]) const {
 #pragma unroll
-        for (int c = 0; c < NV; ++c) stv<T>(p + col[c], v[c], cnt[c]);
+        for (int c = 0; c < NV; ++c) stv<T>((T*)p + at + col[c], v[c], cnt[c]);
     }
     // both sums over the team, in every lane.  Teams of several waves: `red` has 2 slots per wave; calls alternate between two halves of it, so that one
     // barrier per call is enough.
     __device__ __forceinline__ void sum2(float& a, float& b, float* red, int& turn) const {
-#pragma unroll
-        for (int o = (TPR < 64 ? TPR : 64) / 2; o > 0; o >>= 1) { a += __shfl_xor(a, o, 64); b += __shfl_xor(b, o, 64); }
+        if constexpr (TPR == 16) { a = sum16(a); b = sum16(b); }
+        else { a = sum64(a); b = sum64(b); }
         if constexpr (TPR > 64) {
             float* at = red + (turn & 1) * 2 * WAVES;
             turn ^= 1;
@@ -89,6 +119,31 @@ template <int TPR, int NV> struct Team {
             a = 0.f; b = 0.f;
 #pragma unroll
             for (int w = 0; w < WAVES; ++w) { a += at[2 * w]; b += at[2 * w + 1]; }
+        }
+    }
+};
+// N vectors of D floats that every row uses.  Several teams in a workgroup: in LDS, since registers are what limits the rows in flight; one team: in its
+// registers, where each thread needs its own columns only.
+template <int TPR, int NV, int N> struct Vectors {
+    using TM = Team<TPR, NV>;
+    static constexpr bool SHARED = TM::TEAMS > 1;
+    f32x4 own[SHARED ? 1 : N][SHARED ? 1 : NV];
+    __device__ __forceinline__ f32x4 get(const float* lds, const TM& tm, int k, int c) const {
+        if constexpr (SHARED) return *(const f32x4*)(lds + k * TM::WIDTH + tm.col[c]);
+        else return own[k][c];
+    }
+    // (shared: every thread of the workgroup calls, with barriers around the calls)
+    __device__ __forceinline__ void set(float* lds, const TM& tm, int k, const float* p, float other, int D, const float* times = nullptr) {
+        if constexpr (SHARED) {
+            for (int i = threadIdx.x; i < TM::WIDTH; i += TM::THREADS) lds[k * TM::WIDTH + i] = i < D ? (p ? p[i] : other) * (times ? times[i] : 1.f) : 0.f;
+        } else {
+            tm.load_or(p, other, own[k]);
+            if (times) {
+                f32x4 t[NV];
+                tm.load_or(times, 1.f, t);
+#pragma unroll
+                for (int c = 0; c < NV; ++c) own[k][c] = own[k][c] * t[c];
+            }
         }
     }
 };
@@ -118,30 +173,41 @@ __device__ __forceinline__ void moments(const Team<TPR, NV>& tm, const f32x4 (&v
 template <typename T, typename TX, int TPR, int NV>
 __global__ __launch_bounds__((Team<TPR, NV>::THREADS)) void gated_norm_fwd_kernel(const NormArgs p) {
     using TM = Team<TPR, NV>;
+    using VS = Vectors<TPR, NV, 4>;
     __shared__ float red[TPR > 64 ? 4 * TM::WAVES : 1];
+    __shared__ __attribute__((aligned(16))) float vec[VS::SHARED ? 4 * TM::WIDTH : 1];
+    enum { W2, B2, W1, B1 };
     const TM tm(p.D);
     int turn = 0;
-    f32x4 w2[NV], b2[NV], w1[NV], b1[NV], g[NV];
-    tm.load_or(p.post.w, 1.f, w2); tm.load_or(p.post.b, 0.f, b2);
-    tm.load_or(p.pre.w, 1.f, w1); tm.load_or(p.pre.b, 0.f, b1);
+    VS vs;
+    vs.set(vec, tm, W2, p.post.w, 1.f, p.D); vs.set(vec, tm, B2, p.post.b, 0.f, p.D);
+    vs.set(vec, tm, W1, p.pre.w, 1.f, p.D); vs.set(vec, tm, B1, p.pre.b, 0.f, p.D);
+    if constexpr (VS::SHARED) __syncthreads();
+    f32x4 g[NV];
     long long seg = -1;
     tm.load_or(nullptr, 1.f, g);
     // consecutive rows stay in a workgroup: the gate row changes rarely
     const long long per = ((p.rows + gridDim.x - 1) / gridDim.x + TM::TEAMS - 1) / TM::TEAMS * TM::TEAMS;
     const long long first = per * blockIdx.x + threadIdx.x / TPR, end = min(per * (blockIdx.x + 1ll), p.rows);
+    Raw<TX> rx[NV];                                          // the next row, on its way while this one is worked on
+    Raw<T> ry[NV];
+    if (first < end) { tm.template load<TX>(p.x, first * p.D, rx); if (p.y) tm.template load<T>(p.y, first * p.D, ry); }
     for (long long row = first; row < end; row += TM::TEAMS) {
         f32x4 v[NV], n[NV];
-        tm.template load<TX>((const TX*)p.x + row * p.D, v);
+#pragma unroll
+        for (int c = 0; c < NV; ++c) { v[c] = rx[c].f(); n[c] = ry[c].f(); }
+        if (p.gate && row / p.seg_rows != seg) { seg = row / p.seg_rows; tm.load_or(p.gate + seg * p.D, 1.f, g); }
+        if (row + TM::TEAMS < end) { tm.template load<TX>(p.x, (row + TM::TEAMS) * p.D, rx); if (p.y) tm.template load<T>(p.y, (row + TM::TEAMS) * p.D, ry); }
         float m2 = 0.f, r2 = 0.f, m1 = 0.f, r1 = 0.f;
-        if (p.y) tm.template load<T>((const T*)p.y + row * p.D, n);
-        if (p.gate && row / p.seg_rows != seg) { seg = row / p.seg_rows; tm.template load<float>(p.gate + seg * p.D, g); }
         if (p.y) {
             if (p.post.kind != DIC_NORM_NONE) {
                 moments(tm, n, p.post, p.inv_d, red, turn, m2, r2);
 #pragma unroll
-                for (int c = 0; c < NV; ++c)
+                for (int c = 0; c < NV; ++c) {
+                    const f32x4 w = vs.get(vec, tm, W2, c), b = vs.get(vec, tm, B2, c);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) n[c][e] = (n[c][e] - m2) * r2 * w2[c][e] + b2[c][e];
+                    for (int e = 0; e < 4; ++e) n[c][e] = (n[c][e] - m2) * r2 * w[e] + b[e];
+                }
             }
 #pragma unroll
             for (int c = 0; c < NV; ++c)
@@ -151,65 +217,101 @@ __global__ __launch_bounds__((Team<TPR, NV>::THREADS)) void gated_norm_fwd_kerne
 #pragma unroll
             for (int c = 0; c < NV; ++c) v[c] = v[c] * p.r;
         }
-        if (p.x_new) tm.template store<TX>((TX*)p.x_new + row * p.D, v);
+        if (p.x_new) tm.template store<TX>(p.x_new, row * p.D, v);
         if (p.pre.kind != DIC_NORM_NONE) {
             moments(tm, v, p.pre, p.inv_d, red, turn, m1, r1);
 #pragma unroll
-            for (int c = 0; c < NV; ++c)
+            for (int c = 0; c < NV; ++c) {
+                const f32x4 w = vs.get(vec, tm, W1, c), b = vs.get(vec, tm, B1, c);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[c][e] = (v[c][e] - m1) * r1 * w1[c][e] + b1[c][e];
-            tm.template store<T>((T*)p.a + row * p.D, v);
+                for (int e = 0; e < 4; ++e) v[c][e] = (v[c][e] - m1) * r1 * w[e] + b[e];
+            }
+            tm.template store<T>(p.a, row * p.D, v);
         }
         if (tm.lane == 0 && p.saved) { p.saved[row] = m2; p.saved[p.rows + row] = r2; p.saved[2 * p.rows + row] = m1; p.saved[3 * p.rows + row] = r1; }
     }
 }
 
-// A workgroup walks consecutive pieces; its teams take the rows of a piece in turn.  Column sums: d and d u over a piece give that piece's share of the
-// gate's gradient (w sum(d u) + b sum(d), folded over the teams through LDS), and, times the gate, of the post norm's weight and bias.
-template <typename T, typename TX, int TPR, int NV>
+// A workgroup walks consecutive pieces (ONE: it has one); its teams take the rows of a piece in turn.  Column sums: d and d u over a piece give that
+// piece's share of the gate's gradient (w sum(d u) + b sum(d), folded over the teams through LDS), and, times the gate, of the post norm's weight and bias.
+template <typename T, typename TX, int TPR, int NV, bool ONE>
 __global__ __launch_bounds__((Team<TPR, NV>::THREADS)) void gated_norm_bwd_kernel(const NormArgs p) {
     using TM = Team<TPR, NV>;
+    using VS = Vectors<TPR, NV, 2>;
     __shared__ float red[TPR > 64 ? 4 * TM::WAVES : 1];
-    extern __shared__ __attribute__((aligned(16))) float fold[];        // [TEAMS][D rounded up to 4]
+    __shared__ __attribute__((aligned(16))) float vec[VS::SHARED ? 2 * TM::WIDTH : 1];
+    __shared__ __attribute__((aligned(16))) float fold[TM::TEAMS > 1 ? TM::TEAMS * TM::WIDTH : 1];
+    enum { W1, GW2 };                                        // pre's weight; the gate times post's
     const TM tm(p.D);
-    const int team = threadIdx.x / TPR, ldf = (p.D + 3) & ~3;
+    const int team = threadIdx.x / TPR;
     int turn = 0;
-    f32x4 w2[NV], w1[NV], g[NV], sdu[NV], sd[NV], sw2[NV], sb2[NV], sw1[NV], sb1[NV];
+    VS vs;
+    f32x4 sdu[NV], sd[NV], sw2[ONE ? 1 : NV], sb2[ONE ? 1 : NV], sw1[NV], sb1[NV], g[NV];
     const f32x4 zero{0.f, 0.f, 0.f, 0.f};
-    tm.load_or(p.post.w, 1.f, w2); tm.load_or(p.pre.w, 1.f, w1); tm.load_or(nullptr, 1.f, g);
+    vs.set(vec, tm, W1, p.pre.w, 1.f, p.D);
 #pragma unroll
-    for (int c = 0; c < NV; ++c) sw2[c] = sb2[c] = sw1[c] = sb1[c] = zero;
+    for (int c = 0; c < NV; ++c) { sw1[c] = sb1[c] = zero; if constexpr (!ONE) sw2[c] = sb2[c] = zero; }
     const bool layer1 = p.pre.kind == DIC_NORM_LAYER, layer2 = p.post.kind == DIC_NORM_LAYER, pre = p.pre.kind != DIC_NORM_NONE, post = p.post.kind != DIC_NORM_NONE;
-    const long long q0 = (long long)blockIdx.x * p.pieces_per_block, q1 = min(q0 + p.pieces_per_block, p.pieces);
+    // sums over the teams, in a fixed order, to out[0 .. D)
+    auto fold_teams = [&](float* out, const f32x4 (&v)[NV]) {
+        if constexpr (TM::TEAMS == 1) tm.template store<float>(out, 0, v);
+        else {
+            tm.template store<float>(fold + team * TM::WIDTH, 0, v);
+            __syncthreads();
+            for (int i = threadIdx.x; i < p.D; i += TM::THREADS) {
+                float s = 0.f;
+#pragma unroll
+                for (int t = 0; t < TM::TEAMS; ++t) s += fold[t * TM::WIDTH + i];
+                out[i] = s;
+            }
+            __syncthreads();
+        }
+    };
+    const long long q0 = ONE ? blockIdx.x : (long long)blockIdx.x * p.pieces_per_block, q1 = ONE ? q0 + 1 : min(q0 + p.pieces_per_block, p.pieces);
     for (long long q = q0; q < q1; ++q) {
         const long long seg = q / p.gate_parts, part = q - seg * p.gate_parts;
         const long long first = seg * p.seg_rows + part * p.piece_rows, end = min(first + p.piece_rows, min((seg + 1) * p.seg_rows, p.rows));
-        if (p.gate) tm.template load<float>(p.gate + seg * p.D, g);
+        const float* gate = p.gate ? p.gate + seg * p.D : nullptr;
+        if (VS::SHARED && !ONE && q > q0 && p.gate) __syncthreads();                 // the last piece's rows are done with
+        if (q == q0 || p.gate) vs.set(vec, tm, GW2, p.post.w, 1.f, p.D, gate);
+        Raw<TX> rd[NV], rx[NV];                              // the next row, on its way while this one is worked on
+        Raw<T> re[NV], ry[NV];
+        auto fetch = [&](long long row) {
+            if (p.dx_new) tm.template load<TX>(p.dx_new, row * p.D, rd);
+            if (pre) { tm.template load<T>(p.da, row * p.D, re); tm.template load<TX>(p.x_new, row * p.D, rx); }
+            if (p.y) tm.template load<T>(p.y, row * p.D, ry);
+        };
+        constexpr bool AHEAD = TPR < 1024;                   // (16 waves to a row have 128 registers each: no room for the next one)
+        if (AHEAD && first + team < end) fetch(first + team);
+        if constexpr (VS::SHARED) { if (q == q0 || p.gate) __syncthreads(); }
 #pragma unroll
         for (int c = 0; c < NV; ++c) sdu[c] = sd[c] = zero;
         for (long long row = first + team; row < end; row += TM::TEAMS) {
             f32x4 d[NV], e[NV], x[NV], y[NV];
-            if (p.dx_new) tm.template load<TX>((const TX*)p.dx_new + row * p.D, d);
-            else {
+            if (!AHEAD) fetch(row);
 #pragma unroll
-                for (int c = 0; c < NV; ++c) d[c] = zero;
+            for (int c = 0; c < NV; ++c) {
+                d[c] = p.dx_new ? rd[c].f() : zero;
+                if (pre) { e[c] = re[c].f(); x[c] = rx[c].f(); }
+                if (p.y) y[c] = ry[c].f();
             }
-            if (pre) { tm.template load<T>((const T*)p.da + row * p.D, e); tm.template load<TX>((const TX*)p.x_new + row * p.D, x); }
-            if (p.y) tm.template load<T>((const T*)p.y + row * p.D, y);
+            if (AHEAD && row + TM::TEAMS < end) fetch(row + TM::TEAMS);
             if (pre) {
                 const float m = p.saved[2 * p.rows + row], rs = p.saved[3 * p.rows + row];
                 float c1 = 0.f, c2 = 0.f;
 #pragma unroll
-                for (int c = 0; c < NV; ++c)
+                for (int c = 0; c < NV; ++c) {
+                    const f32x4 w = vs.get(vec, tm, W1, c);
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         const float u = k < tm.cnt[c] ? (x[c][k] - m) * rs : 0.f;
                         sw1[c][k] += e[c][k] * u;
                         sb1[c][k] += e[c][k];
-                        const float f = e[c][k] * w1[c][k];
+                        const float f = e[c][k] * w[k];
                         c1 += f; c2 += f * u;
                         x[c][k] = u; e[c][k] = f;
                     }
+                }
                 tm.sum2(c1, c2, red, turn);
                 c1 = layer1 ? c1 * p.inv_d : 0.f;
                 c2 *= p.inv_d;
@@ -221,23 +323,25 @@ __global__ __launch_bounds__((Team<TPR, NV>::THREADS)) void gated_norm_bwd_kerne
             if (p.dx) {
 #pragma unroll
                 for (int c = 0; c < NV; ++c) x[c] = d[c] * p.r;
-                tm.template store<TX>((TX*)p.dx + row * p.D, x);
+                tm.template store<TX>(p.dx, row * p.D, x);
             }
             if (p.y) {
                 const float m = post ? p.saved[row] : 0.f, rs = post ? p.saved[p.rows + row] : 1.f;
                 float c1 = 0.f, c2 = 0.f;
 #pragma unroll
-                for (int c = 0; c < NV; ++c)
+                for (int c = 0; c < NV; ++c) {
+                    const f32x4 w = vs.get(vec, tm, GW2, c);
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         const bool in = k < tm.cnt[c];
                         const float u = in ? (y[c][k] - m) * rs : 0.f, dd = in ? d[c][k] : 0.f;
                         sdu[c][k] += dd * u;
                         sd[c][k] += dd;
-                        const float f = dd * g[c][k] * w2[c][k];
+                        const float f = dd * w[k];
                         c1 += f; c2 += f * u;
                         y[c][k] = u; d[c][k] = f;
                     }
+                }
                 if (post) {
                     tm.sum2(c1, c2, red, turn);
                     c1 = layer2 ? c1 * p.inv_d : 0.f;
@@ -247,45 +351,30 @@ __global__ __launch_bounds__((Team<TPR, NV>::THREADS)) void gated_norm_bwd_kerne
 #pragma unroll
                         for (int k = 0; k < 4; ++k) d[c][k] = rs * (d[c][k] - c1 - y[c][k] * c2);
                 }
-                if (p.dy) tm.template store<T>((T*)p.dy + row * p.D, d);
+                if (p.dy) tm.template store<T>(p.dy, row * p.D, d);
             }
         }
+        tm.load_or(gate, 1.f, g);
+        if constexpr (!ONE) {
 #pragma unroll
-        for (int c = 0; c < NV; ++c) { sw2[c] += sdu[c] * g[c]; sb2[c] += sd[c] * g[c]; }
+            for (int c = 0; c < NV; ++c) { sw2[c] += sdu[c] * g[c]; sb2[c] += sd[c] * g[c]; }
+        }
         if (p.dgate) {
-            f32x4 b2[NV];
-            tm.load_or(p.post.b, 0.f, b2);
+            f32x4 w2[NV], b2[NV], share[NV];
+            tm.load_or(p.post.w, 1.f, w2); tm.load_or(p.post.b, 0.f, b2);
 #pragma unroll
-            for (int c = 0; c < NV; ++c) sdu[c] = sdu[c] * w2[c] + sd[c] * b2[c];
-            if constexpr (TM::TEAMS == 1) tm.template store<float>(p.dgate + q * p.D, sdu);
-            else {
-                tm.template store<float>(fold + team * ldf, sdu);
-                __syncthreads();
-                for (int i = threadIdx.x; i < p.D; i += TM::THREADS) {
-                    float s = 0.f;
-                    for (int t = 0; t < TM::TEAMS; ++t) s += fold[t * ldf + i];
-                    p.dgate[q * p.D + i] = s;
-                }
-                __syncthreads();
-            }
+            for (int c = 0; c < NV; ++c) share[c] = sdu[c] * w2[c] + sd[c] * b2[c];
+            fold_teams(p.dgate + q * p.D, share);
         }
     }
     if (!p.cols) return;
     float* out = p.cols + (long long)blockIdx.x * 4 * p.D;
-    auto put = [&](int k, const f32x4 (&v)[NV]) {
-        if constexpr (TM::TEAMS == 1) tm.template store<float>(out + k * p.D, v);
-        else {
-            tm.template store<float>(fold + team * ldf, v);
-            __syncthreads();
-            for (int i = threadIdx.x; i < p.D; i += TM::THREADS) {
-                float s = 0.f;
-                for (int t = 0; t < TM::TEAMS; ++t) s += fold[t * ldf + i];
-                out[k * p.D + i] = s;
-            }
-            __syncthreads();
-        }
-    };
-    put(0, sw2); put(1, sb2); put(2, sw1); put(3, sb1);
+    if constexpr (ONE) {
+#pragma unroll
+        for (int c = 0; c < NV; ++c) { sdu[c] = sdu[c] * g[c]; sd[c] = sd[c] * g[c]; }
+        fold_teams(out, sdu); fold_teams(out + p.D, sd);
+    } else { fold_teams(out, sw2); fold_teams(out + p.D, sb2); }
+    fold_teams(out + 2 * p.D, sw1); fold_teams(out + 3 * p.D, sb1);
 }
 
 // out[c] = sum over k < n of in[k * ld + c]: 32 columns by 32 interleaved groups of rows per workgroup, the groups added in a fixed order
@@ -321,7 +410,7 @@ template <typename F> int by_width(int D, F&& f) {
     if (D <= 768) return f(std::integral_constant<int, 64>(), std::integral_constant<int, 3>());
     if (D <= 1024) return f(std::integral_constant<int, 64>(), std::integral_constant<int, 4>());
     if (D <= 2048) return f(std::integral_constant<int, 256>(), std::integral_constant<int, 2>());
-    if (D <= 4096) return f(std::integral_constant<int, 256>(), std::integral_constant<int, 4>());
+    if (D <= 4096) return f(std::integral_constant<int, 512>(), std::integral_constant<int, 2>());
     return f(std::integral_constant<int, 1024>(), std::integral_constant<int, 2>());
 }
 int teams_of(int D) { return D <= 128 ? 16 : D <= 1024 ? 4 : 1; }
@@ -382,8 +471,8 @@ template <typename T, typename TX> int fwd(const NormArgs& a, hipStream_t st) {
 template <typename T, typename TX> int bwd(const NormArgs& a, long long blocks, hipStream_t st) {
     return by_width(a.D, [&](auto tpr, auto nv) -> int {
         using TM = Team<decltype(tpr)::value, decltype(nv)::value>;
-        const size_t lds = TM::TEAMS == 1 ? 0 : (size_t)TM::TEAMS * ((a.D + 3) & ~3) * sizeof(float);
-        hipLaunchKernelGGL((gated_norm_bwd_kernel<T, TX, decltype(tpr)::value, decltype(nv)::value>), dim3((unsigned)blocks), dim3(TM::THREADS), lds, st, a);
+        if (a.pieces_per_block == 1) hipLaunchKernelGGL((gated_norm_bwd_kernel<T, TX, decltype(tpr)::value, decltype(nv)::value, true>), dim3((unsigned)blocks), dim3(TM::THREADS), 0, st, a);
+        else hipLaunchKernelGGL((gated_norm_bwd_kernel<T, TX, decltype(tpr)::value, decltype(nv)::value, false>), dim3((unsigned)blocks), dim3(TM::THREADS), 0, st, a);
         DIC_CHECK_LAUNCH();
         return 0;
     });
