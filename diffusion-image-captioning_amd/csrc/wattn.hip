@@ -74,20 +74,35 @@ template <typename T> struct Mma;
 template <> struct Mma<bf16_t> {
     typedef bf16x8 Frag;
     __device__ static __forceinline__ f32x16 mac(Frag a, Frag b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
-    // acc[d][col] += sum over 32 tokens of tile[token][32 db + d] * p[token][col], p in accumulator order
-    template <int DH> __device__ static __forceinline__ f32x16 mac_t(const char* tile, int db, const f32x16& p, f32x16 acc, int lane) {
+    // acc[d][col] += sum over 32 tokens of tile[token][32 db + d] * p[token][col], p in accumulator order: the tile's part, p's part, the product
+    struct Turned { bf16x8 f[2]; };
+    struct Right { bf16x8 f[2]; };
+    template <int DH> __device__ static __forceinline__ Turned turned(const char* tile, int db, int lane) {
         using L = Lay<bf16_t, DH>;
         const char* base = tile + L::tr_base(lane) + db * L::SEG;
+        Turned a;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR(s16x4))(base + 2 * s * L::up));
             s16x4 up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR(s16x4))(base + (2 * s + 1) * L::up));
-            s16x8 a = __builtin_shufflevector(lo, up, 0, 1, 2, 3, 4, 5, 6, 7);
+            a.f[s] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, up, 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+        return a;
+    }
+    __device__ static __forceinline__ Right right(const f32x16& p) {
+        Right r;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
             i32x4 b;
 #pragma unroll
             for (int e = 0; e < 4; ++e) b[e] = (int)pack2bf(p[8 * s + 2 * e], p[8 * s + 2 * e + 1]);
-            acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
+            r.f[s] = __builtin_bit_cast(bf16x8, b);
         }
+        return r;
+    }
+    __device__ static __forceinline__ f32x16 mac_t(const Turned& a, const Right& b, f32x16 acc) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.f[s], b.f[s], acc, 0, 0, 0);
         return acc;
     }
     __device__ static __forceinline__ float dot(Frag a, Frag b) {
@@ -105,11 +120,20 @@ template <> struct Mma<float> {
         for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
         return c;
     }
-    template <int DH> __device__ static __forceinline__ f32x16 mac_t(const char* tile, int db, const f32x16& p, f32x16 acc, int lane) {
+    struct Turned { float f[16]; };
+    typedef f32x16 Right;
+    template <int DH> __device__ static __forceinline__ Turned turned(const char* tile, int db, int lane) {
         using L = Lay<float, DH>;
         const char* base = tile + L::el_base(lane) + 2 * db * L::SEG;
+        Turned a;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(*(const float*)(base + L::at(r)), p[r], acc, 0, 0, 0);
+        for (int r = 0; r < 16; ++r) a.f[r] = *(const float*)(base + L::at(r));
+        return a;
+    }
+    __device__ static __forceinline__ Right right(const f32x16& p) { return p; }
+    __device__ static __forceinline__ f32x16 mac_t(const Turned& a, const Right& b, f32x16 acc) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a.f[r], b[r], acc, 0, 0, 0);
         return acc;
     }
     __device__ static __forceinline__ float dot(Frag a, Frag b) { return (a[0] * b[0] + a[1] * b[1]) + (a[2] * b[2] + a[3] * b[3]); }
@@ -127,8 +151,8 @@ __device__ __forceinline__ i32x4 tile_rsrc(const void* base) {
     r[3] = 0x00020000;
     return r;
 }
-__device__ __forceinline__ void dma16(unsigned voff, const i32x4& rsrc, unsigned lds_addr) {           // 64 lanes x 16 B -> 1 KiB at lds_addr
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(rsrc), "s"(__builtin_amdgcn_readfirstlane(lds_addr)) : "memory");
+__device__ __forceinline__ void dma16(unsigned voff, const i32x4& rsrc, unsigned soff, unsigned lds_addr) {   // 64 lanes x 16 B -> 1 KiB at lds_addr
+    asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(voff), "s"(rsrc), "s"(soff), "s"(__builtin_amdgcn_readfirstlane(lds_addr)) : "memory");
 }
 __device__ __forceinline__ void dma4(unsigned voff, const i32x4& rsrc, unsigned lds_addr) {            // 64 lanes x 4 B
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds" ::"v"(voff), "s"(rsrc), "s"(__builtin_amdgcn_readfirstlane(lds_addr)) : "memory");
@@ -136,22 +160,38 @@ __device__ __forceinline__ void dma4(unsigned voff, const i32x4& rsrc, unsigned 
 // this wave's DMA has landed and, behind the barrier, everybody's has; everybody is done with the buffer that is refilled next
 __device__ __forceinline__ void dma_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// ROWS token rows from `base` (row stride st bytes) into a tile; bit r of `valid`: row r is read, else zero.  Waves first, first + step, ... share the pieces.
-template <typename T, int DH, int ROWS>
+// ROWS token rows from `base` (row stride st bytes) into a tile; bit r of `valid`: row r is read, else zero.  NW > 0: the pieces are dealt evenly to that
+// many waves, each the same number; NW = 0: waves first, first + step, ... take them in turn.
+template <typename T, int DH, int ROWS, int NW>
 __device__ __forceinline__ void load_tile(const char* base, unsigned st, unsigned long long valid, unsigned lds, int first, int step, int lane) {
     using L = Lay<T, DH>;
     const i32x4 rs = tile_rsrc(base);
     constexpr int P = ROWS / L::PIECE_ROWS;
-    static_assert(ROWS % L::PIECE_ROWS == 0, "whole pieces");
+    constexpr unsigned long long ALL = ROWS == 64 ? ~0ull : (1ull << (ROWS & 63)) - 1;
+    static_assert(ROWS % L::PIECE_ROWS == 0 && (NW == 0 || P % (NW ? NW : 1) == 0), "whole pieces, the same number for each wave");
+    const unsigned off = (unsigned)L::dma_row(lane) * st + (unsigned)L::dma_chunk(lane) * 16u;
     auto one = [&](int piece, bool all) {
-        const int row = piece * L::PIECE_ROWS + L::dma_row(lane);
-        const unsigned off = (unsigned)row * st + (unsigned)L::dma_chunk(lane) * 16u;
-        dma16(all || ((valid >> row) & 1ull) ? off : 0xfffffff0u, rs, lds + (unsigned)(piece * L::PS));
+        const int row = piece * L::PIECE_ROWS;
+        dma16(all || ((valid >> (row + L::dma_row(lane))) & 1ull) ? off : 0xfffffff0u, rs, (unsigned)row * st, lds + (unsigned)(piece * L::PS));
     };
-    if (P >= 4 && step == 4 && valid == (ROWS == 64 ? ~0ull : (1ull << ROWS % 64) - 1)) {
+    if constexpr (NW > 0) {
+        if (valid == ALL) {
 #pragma unroll
-        for (int j = 0; j < P / 4; ++j) one(4 * j + first, true);
-    } else for (int piece = first; piece < P; piece += step) one(piece, false);
+            for (int j = 0; j < P / NW; ++j) one(j * NW + first, true);
+        } else {
+#pragma unroll
+            for (int j = 0; j < P / NW; ++j) one(j * NW + first, false);
+        }
+    } else if (valid == ALL)
+        for (int piece = first; piece < P; piece += step) one(piece, true);
+    else
+        for (int piece = first; piece < P; piece += step) one(piece, false);
+}
+// The loads of `f` end here.  Left to their first use, inside the loop over tiles, the compiler's wait there would be for every load in flight, the next
+// tiles' DMA among them (which it does not know of), in every turn.
+template <typename F, int N> __device__ __forceinline__ void landed(F (&f)[N]) {
+#pragma unroll
+    for (int s = 0; s < N; ++s) asm volatile("" : "+v"(f[s]));
 }
 template <typename T, int DH>
 __device__ __forceinline__ typename Mma<T>::Frag row_frag(const char* tile, int s, int lane) {
@@ -210,15 +250,73 @@ constexpr int BQ = 32;                          // queries (or keys) per wave, a
 __host__ __device__ __forceinline__ long long stats_floats(long long N, long long H, long long Tq) { return N * H * ((Tq + BQ - 1) / BQ) * 2 * BQ; }
 __device__ __forceinline__ long long stats_at(const WinArgs& a, int n, int h, int i0) { return stats_floats(1, (long long)n * a.H + h, a.Tq) + 2 * i0; }
 
+// The key and value tiles of a workgroup's walk in LDS.  NW > 0: two of them, and that many waves fetch the next one behind the barrier in front of a tile.
+// NW = 0: the walk has at most FEW_TILES, and whatever waves there are fetch all of them at the start.
+constexpr int FEW_TILES = 4, MASK_RUN = 256;
+template <typename T, int DH, int BN, int NW> struct KeyTiles {
+    using L = Lay<T, DH>;
+    static constexpr int TILE = L::bytes(BN), SLOTS = NW ? 2 : FEW_TILES;
+    const WinArgs& a;
+    const Walk wk;
+    const char *kb, *vb, *smem;
+    const long long kst, vst;
+    const int n, wave, nw, lane;
+    unsigned long long* table;                                // with key_mask: the masks of the next tiles, a ring of 2 MASK_RUN
+    __device__ __forceinline__ KeyTiles(const WinArgs& a, const Walk& wk, int n, int hk, char* smem, unsigned long long* table, int wave, int lane)
+        : a(a), wk(wk), kb((const char*)((const T*)a.k + n * a.sk.n + hk * a.sk.h)), vb((const char*)((const T*)a.v + n * a.sv.n + hk * a.sv.h)), smem(smem),
+          kst(a.sk.t * (long long)sizeof(T)), vst(a.sv.t * (long long)sizeof(T)), n(n), wave(wave), nw(NW ? NW : blockDim.x >> 6), lane(lane), table(table) {}
+    // masks of the tiles t .. t + MASK_RUN - 1 (barriers around it)
+    __device__ __forceinline__ void read_masks(int t) {
+        for (int k = t + wave; k < min(t + MASK_RUN, wk.nt); k += nw) {
+            const int j = wk.j0(k, BN) + lane;
+            const unsigned long long v = __ballot(lane < BN && j < a.Tk && a.key_mask[(size_t)n * a.Tk + j] != 0);
+            if (lane == 0) table[k & (2 * MASK_RUN - 1)] = v;
+        }
+    }
+    // bits of the keys of tile t that exist and are not masked
+    __device__ __forceinline__ unsigned long long valid(int t) const {
+        const int there = wk.kvl - wk.j0(t, BN);
+        unsigned long long v = there >= BN ? below(BN) : below(there);
+        if (a.key_mask) {
+            const unsigned long long m = table[t & (2 * MASK_RUN - 1)];
+            v &= (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)m) | (unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((int)(m >> 32)) << 32;
+        }
+        return v;
+    }
+    __device__ __forceinline__ void issue(int t) const {
+        const int j0 = wk.j0(t, BN);
+        const unsigned long long v = valid(t);
+        const unsigned lds = (unsigned)(uintptr_t)(LDS_PTR(const char))smem + (t & (SLOTS - 1)) * 2 * TILE;
+        load_tile<T, DH, BN, NW>(kb + j0 * kst, (unsigned)kst, v, lds, wave, nw, lane);
+        load_tile<T, DH, BN, NW>(vb + j0 * vst, (unsigned)vst, v, lds + TILE, wave, nw, lane);
+    }
+    __device__ __forceinline__ void begin() {
+        if (a.key_mask) { read_masks(0); __syncthreads(); }
+        for (int t = 0; t < min(wk.nt, NW ? 1 : FEW_TILES); ++t) issue(t);
+        if constexpr (NW == 0) dma_barrier();
+    }
+    // tile t is in LDS behind this call, its keys at the address returned and its values TILE bytes further on
+    __device__ __forceinline__ const char* step(int t) {
+        if constexpr (NW > 0) {
+            dma_barrier();
+            if (t + 1 < wk.nt) {
+                if (a.key_mask && ((t + 1) & (MASK_RUN - 1)) == 0) { read_masks(t + 1); __syncthreads(); }
+                issue(t + 1);
+            }
+        }
+        return smem + (t & (SLOTS - 1)) * 2 * TILE;
+    }
+};
+
 // ------------------------------------------------------------------------------------------------ forward
-template <typename T, int DH, int BN>
+template <typename T, int DH, int BN, int NW>
 __global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 4>)) void win_fwd_kernel(const WinArgs a) {
     using L = Lay<T, DH>;
     using M = Mma<T>;
     constexpr int NB = BN / 32, TILE = L::bytes(BN);
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hi = lane >> 5;
-    const int nw = blockDim.x >> 6, bm = nw * BQ, nqt = (a.Tq + bm - 1) / bm;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hi = lane >> 5;
+    const int nw = NW ? NW : blockDim.x >> 6, bm = nw * BQ, nqt = (a.Tq + bm - 1) / bm;
     int item = xcd_item();
     const int g = item % a.G; item /= a.G;
     const int qt = nqt - 1 - item % nqt; item /= nqt;         // long rows first
@@ -236,16 +334,11 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 4>)) void win_
         const char* p = (const char*)((const T*)a.q + n * a.sq.n + ic * a.sq.t + h * a.sq.h);
 #pragma unroll
         for (int s = 0; s < L::NF; ++s) qf[s] = *(const typename M::Frag*)(p + 32 * s + 16 * hi);
+        landed(qf);
     }
-    const char* kb = (const char*)((const T*)a.k + n * a.sk.n + hk * a.sk.h);
-    const char* vb = (const char*)((const T*)a.v + n * a.sv.n + hk * a.sv.h);
-    const long long kst = a.sk.t * (long long)sizeof(T), vst = a.sv.t * (long long)sizeof(T);
-    const unsigned lds = (unsigned)(uintptr_t)(LDS_PTR(char))smem;
-    auto issue = [&](int j0, unsigned long long valid, int buf) {
-        load_tile<T, DH, BN>(kb + j0 * kst, (unsigned)kst, valid, lds + buf * 2 * TILE, wave, nw, lane);
-        load_tile<T, DH, BN>(vb + j0 * vst, (unsigned)vst, valid, lds + buf * 2 * TILE + TILE, wave, nw, lane);
-    };
-    auto valid_of = [&](int byte, int j0) { return __ballot(byte != 0) & below(min(BN, wk.kvl - j0)); };
+    __shared__ unsigned long long table[2 * MASK_RUN];
+    KeyTiles<T, DH, BN, NW> tiles(a, wk, n, hk, smem, table, wave, lane);
+    tiles.begin();
 
     f32x16 acc[L::ND];
 #pragma unroll
@@ -294,26 +387,14 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 4>)) void win_
 #pragma unroll
             for (int r = 0; r < 16; ++r) { st[b][r] = __builtin_amdgcn_exp2f(fmaf(st[b][r], a.c, -mm)); l += st[b][r]; }
 #pragma unroll
-            for (int d = 0; d < L::ND; ++d) acc[d] = M::template mac_t<DH>(vt + L::bytes(32 * b), d, st[b], acc[d], lane);
+            for (int d = 0; d < L::ND; ++d) acc[d] = M::mac_t(M::template turned<DH>(vt + L::bytes(32 * b), d, lane), M::right(st[b]), acc[d]);
         }
     };
-    unsigned long long valid = 0, valid_next = 0;
-    int byte = 1;                                             // key_mask of this lane's key in the tile after the next
-    if (wk.nt > 0) {
-        valid = valid_of(mask_byte(a, n, wk.j0(0, BN) + lane), wk.j0(0, BN));
-        issue(wk.j0(0, BN), valid, 0);
-        if (wk.nt > 1) byte = mask_byte(a, n, wk.j0(1, BN) + lane);
-    }
     for (int t = 0; t < wk.nt; ++t) {
         const int j0 = wk.j0(t, BN);
-        if (t + 1 < wk.nt) {
-            valid_next = valid_of(byte, wk.j0(t + 1, BN));
-            if (t + 2 < wk.nt) byte = mask_byte(a, n, wk.j0(t + 2, BN) + lane);
-        }
-        dma_barrier();
-        if (t + 1 < wk.nt) issue(wk.j0(t + 1, BN), valid_next, (t + 1) & 1);
-        const char* kt = smem + (t & 1) * 2 * TILE;
+        const char* kt = tiles.step(t);
         const char* vt = kt + TILE;
+        const unsigned long long valid = tiles.valid(t);
         unsigned long long bits = ~0ull;
         const bool full = j0 >= in_lo && j0 + BN <= in_hi && valid == below(BN);
         if (!full) bits = visible(sp, j0) & valid;
@@ -326,7 +407,6 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 4>)) void win_
                 else blocks(std::integral_constant<int, 1>(), first ? 0 : 1, kt, vt, bits, full);
             }
         }
-        valid = valid_next;
     }
     l += __shfl_xor(l, 32, 64);
     if (i < a.Tq) {
@@ -341,14 +421,14 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 4>)) void win_
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dq (and delta)
-template <typename T, int DH, int BN>
-__global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 3>)) void win_bwd_dq_kernel(const WinArgs a) {
+template <typename T, int DH, int BN, int NW>
+__global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 4>)) void win_bwd_dq_kernel(const WinArgs a) {
     using L = Lay<T, DH>;
     using M = Mma<T>;
     constexpr int NB = BN / 32, TILE = L::bytes(BN);
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hi = lane >> 5;
-    const int nw = blockDim.x >> 6, bm = nw * BQ, nqt = (a.Tq + bm - 1) / bm;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hi = lane >> 5;
+    const int nw = NW ? NW : blockDim.x >> 6, bm = nw * BQ, nqt = (a.Tq + bm - 1) / bm;
     int item = xcd_item();
     const int g = item % a.G; item /= a.G;
     const int qt = nqt - 1 - item % nqt; item /= nqt;
@@ -373,39 +453,26 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 3>)) void win_
             delta += M::dot(df[s], *(const typename M::Frag*)(po + 32 * s + 16 * hi));
         }
         delta += __shfl_xor(delta, 32, 64);
+        landed(qf);
+        landed(df);
     }
-    const float l2 = a.lse[((long long)n * a.H + h) * a.Tq + ic] * LOG2E;
-    if (i < a.Tq) a.stats[stats_at(a, n, h, i0) + lane] = hi ? delta : l2;
+    // rows that see nothing, and those behind the last that fill a tile of statistics up, get lse = +inf: the dk / dv kernel's exponentials are then zero
+    float l2 = a.lse[((long long)n * a.H + h) * a.Tq + ic] * LOG2E;
+    if (l2 == -INFINITY || i >= a.Tq) l2 = INFINITY;
+    asm volatile("" : "+v"(l2));
+    if (wave_rows) a.stats[stats_at(a, n, h, i0) + lane] = hi ? (i < a.Tq ? delta : 0.f) : l2;
 
-    const char* kb = (const char*)((const T*)a.k + n * a.sk.n + hk * a.sk.h);
-    const char* vb = (const char*)((const T*)a.v + n * a.sv.n + hk * a.sv.h);
-    const long long kst = a.sk.t * (long long)sizeof(T), vst = a.sv.t * (long long)sizeof(T);
-    const unsigned lds = (unsigned)(uintptr_t)(LDS_PTR(char))smem;
-    auto issue = [&](int j0, unsigned long long valid, int buf) {
-        load_tile<T, DH, BN>(kb + j0 * kst, (unsigned)kst, valid, lds + buf * 2 * TILE, wave, nw, lane);
-        load_tile<T, DH, BN>(vb + j0 * vst, (unsigned)vst, valid, lds + buf * 2 * TILE + TILE, wave, nw, lane);
-    };
-    auto valid_of = [&](int byte, int j0) { return __ballot(byte != 0) & below(min(BN, wk.kvl - j0)); };
+    __shared__ unsigned long long table[2 * MASK_RUN];
+    KeyTiles<T, DH, BN, NW> tiles(a, wk, n, hk, smem, table, wave, lane);
+    tiles.begin();
     f32x16 acc[L::ND];
 #pragma unroll
     for (int d = 0; d < L::ND; ++d) acc[d] = zero16();
-    unsigned long long valid = 0, valid_next = 0;
-    int byte = 1;
-    if (wk.nt > 0) {
-        valid = valid_of(mask_byte(a, n, wk.j0(0, BN) + lane), wk.j0(0, BN));
-        issue(wk.j0(0, BN), valid, 0);
-        if (wk.nt > 1) byte = mask_byte(a, n, wk.j0(1, BN) + lane);
-    }
     for (int t = 0; t < wk.nt; ++t) {
         const int j0 = wk.j0(t, BN);
-        if (t + 1 < wk.nt) {
-            valid_next = valid_of(byte, wk.j0(t + 1, BN));
-            if (t + 2 < wk.nt) byte = mask_byte(a, n, wk.j0(t + 2, BN) + lane);
-        }
-        dma_barrier();
-        if (t + 1 < wk.nt) issue(wk.j0(t + 1, BN), valid_next, (t + 1) & 1);
-        const char* kt = smem + (t & 1) * 2 * TILE;
+        const char* kt = tiles.step(t);
         const char* vt = kt + TILE;
+        const unsigned long long valid = tiles.valid(t);
         unsigned long long bits = ~0ull;
         const bool full = j0 >= in_lo && j0 + BN <= in_hi && valid == below(BN);
         if (!full) bits = visible(sp, j0) & valid;
@@ -426,10 +493,9 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 3>)) void win_
                     st[r] = full || ((w >> tok(r, 0)) & 1u) ? p : 0.f;
                 }
 #pragma unroll
-                for (int d = 0; d < L::ND; ++d) acc[d] = M::template mac_t<DH>(kt + L::bytes(32 * b), d, st, acc[d], lane);
+                for (int d = 0; d < L::ND; ++d) acc[d] = M::mac_t(M::template turned<DH>(kt + L::bytes(32 * b), d, lane), M::right(st), acc[d]);
             }
         }
-        valid = valid_next;
     }
     if (i < a.Tq) {
         T* o = (T*)a.dq + n * a.sdq.n + i * a.sdq.t + h * a.sdq.h;
@@ -443,17 +509,18 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 3>)) void win_
 
 // ------------------------------------------------------------------------------------------------ backward: dk, dv
 // A workgroup owns kg groups of 32 keys and walks the queries that see them, 32 qh at a time: wave w takes key group w % kg and query rows 32 (w / kg).
-// The qh partial sums of a key group are added through LDS at the end.
+// The qh partial sums of a key group are added through LDS at the end.  A stage holds u of those row groups for each; all queries in one stage, and one
+// buffer, where they are few.
 // SINK = false: the pairs inside the windows.  SINK = true, launched before it: the pairs of a sink key and a query whose window starts behind it.  Every
 // query has those, so their walk is cut into `chunks` that leave fp32 partial sums in the workspace; the window pass adds them to the sink keys' rows
 // in a fixed order.  (One workgroup that walks all queries for the sinks' tile alone took 1.9 ms where the window pass takes a tenth of that.)
 template <typename T, int DH, bool SINK>
-__global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 3>)) void win_bwd_dkv_kernel(const WinArgs a, int kg, int qh) {
+__global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 3>)) void win_bwd_dkv_kernel(const WinArgs a, int kg, int qh, int u, int buffers) {
     using L = Lay<T, DH>;
     using M = Mma<T>;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hi = lane >> 5, key_group = wave % kg, row_group = wave / kg, nw = kg * qh;
-    const int bn = kg * BQ, bq = qh * BQ, tile = qh * L::bytes(BQ), stage = 2 * tile + qh * 256;        // Q, dout, statistics of bq queries
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hi = lane >> 5, key_group = wave % kg, row_group = wave / kg, nw = kg * qh;
+    const int bn = kg * BQ, groups = qh * u, bq = groups * BQ, tile = groups * L::bytes(BQ), stage = 2 * tile + groups * 256;        // Q, dout, statistics of bq queries
     const int keys = SINK ? a.sink_keys : a.Tk, nkt = (keys + bn - 1) / bn;
     int item = xcd_item();
     int chunk = 0;
@@ -485,18 +552,20 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 3>)) void win_
             kf[s] = seen ? *(const typename M::Frag*)(pk + 32 * s + 16 * hi) : zero;
             vf[s] = seen ? *(const typename M::Frag*)(pv + 32 * s + 16 * hi) : zero;
         }
+        landed(kf);
+        landed(vf);
     }
     const long long qst = a.sq.t * (long long)sizeof(T), dst = a.sdo.t * (long long)sizeof(T);
     const unsigned lds = (unsigned)(uintptr_t)(LDS_PTR(char))smem;
     auto issue = [&](int t, int buf) {
         const int h = hk * a.G + t / nq, i0 = r0 + (t % nq) * bq;
         const unsigned at = lds + buf * stage;
-        for (int r = 0; r < qh; ++r) {                                        // 32 rows at a time
+        for (int r = 0; r < groups; ++r) {                                    // 32 rows at a time
             const int ir = i0 + r * BQ;
             if (ir >= a.Tq) break;                                            // (the rows of that group are masked out below)
             const unsigned long long valid = below(a.Tq - ir);
-            load_tile<T, DH, BQ>((const char*)((const T*)a.q + n * a.sq.n + h * a.sq.h) + ir * qst, (unsigned)qst, valid, at + r * L::bytes(BQ), wave, nw, lane);
-            load_tile<T, DH, BQ>((const char*)((const T*)a.dout + n * a.sdo.n + h * a.sdo.h) + ir * dst, (unsigned)dst, valid, at + tile + r * L::bytes(BQ), wave, nw, lane);
+            load_tile<T, DH, BQ, 0>((const char*)((const T*)a.q + n * a.sq.n + h * a.sq.h) + ir * qst, (unsigned)qst, valid, at + r * L::bytes(BQ), wave, nw, lane);
+            load_tile<T, DH, BQ, 0>((const char*)((const T*)a.dout + n * a.sdo.n + h * a.sdo.h) + ir * dst, (unsigned)dst, valid, at + tile + r * L::bytes(BQ), wave, nw, lane);
             if (wave == r % nw) dma4((unsigned)lane * 4u, tile_rsrc(a.stats + stats_at(a, n, h, ir)), at + 2 * tile + r * 256);
         }
     };
@@ -506,14 +575,15 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 3>)) void win_
     if (t0 < t1) issue(t0, 0);
     for (int t = t0; t < t1; ++t) {
         dma_barrier();
-        const int buf = (t - t0) & 1;
+        const int buf = (t - t0) & (buffers - 1);
         if (t + 1 < t1) issue(t + 1, buf ^ 1);
-        const char* qt = smem + buf * stage + row_group * L::bytes(BQ);
-        const char* dt = qt + tile;
-        const float* st2 = (const float*)(smem + buf * stage + 2 * tile + row_group * 256);
-        const int i0 = r0 + (t % nq) * bq + row_group * BQ;
-        const unsigned bits = (unsigned)(below(min(end - i0, 32)) & ~below(lo - i0));
-        if (__any(bits != 0)) {
+        for (int r = row_group; r < groups; r += qh) {
+            const char* qt = smem + buf * stage + r * L::bytes(BQ);
+            const char* dt = qt + tile;
+            const float* st2 = (const float*)(smem + buf * stage + 2 * tile + r * 256);
+            const int i0 = r0 + (t % nq) * bq + r * BQ;
+            const unsigned bits = (unsigned)(below(min(end - i0, 32)) & ~below(lo - i0));
+            if (!__any(bits != 0)) continue;
             f32x16 s = zero16(), dp = zero16();
 #pragma unroll
             for (int f = 0; f < L::NF; ++f) {
@@ -521,23 +591,25 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 3>)) void win_
                 dp = M::mac(row_frag<T, DH>(dt, f, lane), vf[f], dp);
             }
             __builtin_amdgcn_sched_barrier(0);
-            const unsigned w = bits >> (4 * hi);
+            if (!__all(bits == ~0u)) {
+                const unsigned w = bits >> (4 * hi);
 #pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-                const f32x4 l2 = *(const f32x4*)(st2 + tok(r, hi)), de = *(const f32x4*)(st2 + 32 + tok(r, hi));
+                for (int e = 0; e < 16; ++e) s[e] = (w >> tok(e, 0)) & 1u ? s[e] : -INFINITY;
+            }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const bool on = (w >> tok(r + e, 0)) & 1u;
-                    const float p = on ? __builtin_amdgcn_exp2f(fmaf(s[r + e], a.c, -l2[e])) : 0.f;
-                    s[r + e] = p;
-                    dp[r + e] = on ? p * (dp[r + e] - de[e]) : 0.f;
+            for (int e = 0; e < 16; e += 4) {
+                const f32x4 l2 = *(const f32x4*)(st2 + tok(e, hi)), de = *(const f32x4*)(st2 + 32 + tok(e, hi));
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    s[e + x] = __builtin_amdgcn_exp2f(fmaf(s[e + x], a.c, -l2[x]));
+                    dp[e + x] = s[e + x] * (dp[e + x] - de[x]);
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int d = 0; d < L::ND; ++d) {
-                dv[d] = M::template mac_t<DH>(dt, d, s, dv[d], lane);
-                dk[d] = M::template mac_t<DH>(qt, d, dp, dk[d], lane);
+                dv[d] = M::mac_t(M::template turned<DH>(dt, d, lane), M::right(s), dv[d]);
+                dk[d] = M::mac_t(M::template turned<DH>(qt, d, lane), M::right(dp), dk[d]);
             }
         }
     }
@@ -619,7 +691,7 @@ __global__ __launch_bounds__((64 * Few<T, DH>::NW), 1) void win_few_kernel(const
     using F = Few<T, DH>;
     constexpr int NW = F::NW, TILE = F::TILE;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hi = lane >> 5, r = lane & 31, rows = a.G * a.Tq;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hi = lane >> 5, r = lane & 31, rows = a.G * a.Tq;
     int item = blockIdx.x;
     const int split = item % splits; item /= splits;
     const int hk = item % a.Hkv, n = item / a.Hkv;
@@ -635,6 +707,7 @@ __global__ __launch_bounds__((64 * Few<T, DH>::NW), 1) void win_few_kernel(const
         const char* p = (const char*)((const T*)a.q + n * a.sq.n + i * a.sq.t + h * a.sq.h);
 #pragma unroll
         for (int s = 0; s < L::NF; ++s) qf[s] = *(const typename M::Frag*)(p + 32 * s + 16 * hi);
+        landed(qf);
     }
     const char* kb = (const char*)((const T*)a.k + n * a.sk.n + hk * a.sk.h);
     const char* vb = (const char*)((const T*)a.v + n * a.sv.n + hk * a.sv.h);
@@ -643,8 +716,8 @@ __global__ __launch_bounds__((64 * Few<T, DH>::NW), 1) void win_few_kernel(const
     const unsigned lds = (unsigned)(uintptr_t)(LDS_PTR(char))mine;
     auto valid_of = [&](int byte, int j0) { return __ballot(byte != 0) & below(min(FEW, wk.kvl - j0)); };
     auto issue = [&](int j0, unsigned long long valid, int buf) {
-        load_tile<T, DH, FEW>(kb + j0 * kst, (unsigned)kst, valid, lds + buf * 2 * TILE, 0, 1, lane);
-        load_tile<T, DH, FEW>(vb + j0 * vst, (unsigned)vst, valid, lds + buf * 2 * TILE + TILE, 0, 1, lane);
+        load_tile<T, DH, FEW, 1>(kb + j0 * kst, (unsigned)kst, valid, lds + buf * 2 * TILE, 0, 1, lane);
+        load_tile<T, DH, FEW, 1>(vb + j0 * vst, (unsigned)vst, valid, lds + buf * 2 * TILE + TILE, 0, 1, lane);
     };
     f32x16 acc[L::ND];
 #pragma unroll
@@ -694,12 +767,12 @@ __global__ __launch_bounds__((64 * Few<T, DH>::NW), 1) void win_few_kernel(const
 #pragma unroll
         for (int e = 0; e < 16; ++e) { st[e] = __builtin_amdgcn_exp2f(fmaf(st[e], a.c, -mm)); l += st[e]; }
 #pragma unroll
-        for (int d = 0; d < L::ND; ++d) acc[d] = M::template mac_t<DH>(vt, d, st, acc[d], lane);
+        for (int d = 0; d < L::ND; ++d) acc[d] = M::mac_t(M::template turned<DH>(vt, d, lane), M::right(st), acc[d]);
         if constexpr (sizeof(T) == 2) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) st[e] -= bf2f(f2bf(st[e]));
 #pragma unroll
-            for (int d = 0; d < L::ND; ++d) acc[d] = M::template mac_t<DH>(vt, d, st, acc[d], lane);
+            for (int d = 0; d < L::ND; ++d) acc[d] = M::mac_t(M::template turned<DH>(vt, d, lane), M::right(st), acc[d]);
         }
         valid = next;
         buf ^= 1;
@@ -804,20 +877,16 @@ int check(int dtype, const DicWinAttnParams* p, bool bwd, bool pointers = true) 
                     : apart(p->out_stride, p->N, p->Tq, p->H, p->dh), "dic_win_attn: rows of an output overlap");
     return 0;
 }
-// Query rows in waves of 32: all of them in one workgroup where that takes at most 8 waves (fp32: 4), which then loads the keys once (130 rows x 3072 heads
-// forward: 86 us with 5 waves, 113 us with 4 and a second workgroup for 2 rows); else 4, one to a SIMD (2050 rows: 61 us with 4, 111 us with 5).
-int waves_of(int rows, int most) {
-    const int waves = (rows + BQ - 1) / BQ;
-    return waves <= most ? waves : 4;
-}
-// The dk / dv kernel's workgroup: kg groups of 32 keys and qh groups of 32 query rows.  Few key tiles: fewer keys and more rows to a workgroup.
+// The dk / dv kernel's workgroup: kg groups of 32 keys and qh groups of 32 query rows.  All keys where they are few and the heads many; else 8 waves (one
+// workgroup to a CU) for 128 wide bf16 rows and 4 otherwise, fewer keys and more rows to a workgroup until there is one for every place on the card.
 struct Shape { int kg, qh; };
-Shape shape_of(const WinArgs& a, int most, int most_rows) {
-    const int waves = (a.Tk + BQ - 1) / BQ;
+Shape shape_of(const WinArgs& a, int waves, int most, int most_rows) {
+    const int tiles = (a.Tk + BQ - 1) / BQ;
     const long long heads = (long long)a.N * a.Hkv;
-    if (waves <= most && heads >= 256) return {waves, 1};
-    for (int kg = 4; kg > 1; kg >>= 1) if (heads * ((waves + kg - 1) / kg) >= 512) return {kg, 4 / kg < most_rows ? 4 / kg : most_rows};
-    return {1, most_rows};
+    if (tiles <= most && heads >= 256) return {tiles, 1};
+    int kg = waves;
+    while (kg > 1 && heads * ((tiles + kg - 1) / kg) < 2048 / waves && waves / kg < most_rows) kg >>= 1;
+    return {kg, waves / kg};
 }
 template <typename T, int DH> constexpr int ROW_GROUPS = Lay<T, DH>::ROWB <= 256 ? 4 : 2;       // at most: two stages of 512-byte rows fill 132 KB of LDS with 2
 // Pieces of the sink pass: about 256 workgroups, and no more than 16 partial sums for the window pass to add.
@@ -874,7 +943,7 @@ template <typename K, typename... More> int launch(K kernel, long long blocks, i
         int dev = 0;
         hipError_t e = hipGetDevice(&dev);
         if (e == hipSuccess && !((allowed.load(std::memory_order_relaxed) >> (dev & 63)) & 1)) {
-            e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 160 << 10);
+            e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 150 << 10);
             if (e == hipSuccess) allowed.fetch_or(1ull << (dev & 63), std::memory_order_relaxed);
         }
         if (e != hipSuccess) { dic_set_error(hipGetErrorString(e)); return (int)e; }
@@ -883,6 +952,19 @@ template <typename K, typename... More> int launch(K kernel, long long blocks, i
     DIC_CHECK_LAUNCH();
     return 0;
 }
+constexpr size_t SHARED_CU_LDS = 75 << 10;                       // two workgroups fit a CU's 160 KB
+// The workgroups of a kernel that walks the keys.  Few keys: all of them in LDS at once (unless that keeps a second workgroup off the CU) and the query rows
+// of a sequence in one workgroup where they fit (130 rows x 130 keys x 3072 heads, forward: 5 waves 86 us, 4 waves and a second workgroup 113 us).
+template <typename T, int DH, int BN, typename F> int over_keys(const WinArgs& a, F&& go) {
+    constexpr int MOST = MOST_WAVES<T>;
+    const int rows = (a.Tq + BQ - 1) / BQ, tiles = (a.Tk + BN - 1) / BN;
+    const size_t all = (size_t)tiles * 2 * Lay<T, DH>::bytes(BN);
+    const bool few = tiles <= FEW_TILES && all <= SHARED_CU_LDS;
+    const int waves = few && rows <= MOST ? rows : 4;
+    const long long blocks = (long long)a.N * a.H * ((rows + waves - 1) / waves);
+    if (few) return go(std::integral_constant<int, 0>(), waves, blocks, all);
+    return go(std::integral_constant<int, 4>(), waves, blocks, (size_t)4 * Lay<T, DH>::bytes(BN));
+}
 template <typename T, int DH> int fwd(const WinArgs& a, hipStream_t st) {
     constexpr int BN = sizeof(T) == 2 ? 64 : 32;
     if (few_rows(a)) {
@@ -890,25 +972,29 @@ template <typename T, int DH> int fwd(const WinArgs& a, hipStream_t st) {
         if (int rc = launch(win_few_kernel<T, DH>, (long long)a.N * a.Hkv * splits, 64 * Few<T, DH>::NW, Few<T, DH>::LDS, st, a, splits)) return rc;
         return splits > 1 ? launch(win_merge_kernel<T, DH>, ((long long)a.N * a.H * a.Tq + 3) / 4, 256, 0, st, a, splits) : 0;
     }
-    const int w = waves_of(a.Tq, MOST_WAVES<T>);
-    return launch(win_fwd_kernel<T, DH, BN>, (long long)a.N * a.H * ((a.Tq + w * BQ - 1) / (w * BQ)), 64 * w, (size_t)4 * Lay<T, DH>::bytes(BN), st, a);
+    return over_keys<T, DH, BN>(a, [&](auto nw, int waves, long long blocks, size_t lds) { return launch(win_fwd_kernel<T, DH, BN, decltype(nw)::value>, blocks, 64 * waves, lds, st, a); });
 }
-template <typename T, int DH> size_t dkv_lds(int kg, int qh) {
-    const size_t stages = (size_t)2 * qh * (2 * Lay<T, DH>::bytes(BQ) + 256), sums = (size_t)(qh - 1) * kg * BQ * DH * sizeof(float);
+template <typename T, int DH> size_t dkv_lds(int kg, int qh, int u, int buffers) {
+    const size_t stages = (size_t)buffers * qh * u * (2 * Lay<T, DH>::bytes(BQ) + 256), sums = (size_t)(qh - 1) * kg * BQ * DH * sizeof(float);
     return stages > sums ? stages : sums;
 }
 template <typename T, int DH> int bwd(const WinArgs& a, hipStream_t st) {
     constexpr int BN = sizeof(T) == 2 ? 64 : 32;
-    if (a.Tq > 0) {
-        const int w = waves_of(a.Tq, MOST_WAVES<T>);
-        if (int rc = launch(win_bwd_dq_kernel<T, DH, BN>, (long long)a.N * a.H * ((a.Tq + w * BQ - 1) / (w * BQ)), 64 * w, (size_t)4 * Lay<T, DH>::bytes(BN), st, a)) return rc;
-    }
+    if (a.Tq > 0)
+        if (int rc = over_keys<T, DH, BN>(a, [&](auto nw, int waves, long long blocks, size_t lds) { return launch(win_bwd_dq_kernel<T, DH, BN, decltype(nw)::value>, blocks, 64 * waves, lds, st, a); }))
+            return rc;
     if (a.Tk == 0) return 0;
     if (a.sink_keys > 0)
         if (int rc = launch(win_bwd_dkv_kernel<T, DH, true>, (long long)a.N * a.Hkv * (a.sink_rows / BQ) * a.chunks, 64 * ROW_GROUPS<T, DH>,
-                            dkv_lds<T, DH>(1, ROW_GROUPS<T, DH>), st, a, 1, ROW_GROUPS<T, DH>)) return rc;
-    const Shape s = shape_of(a, MOST_WAVES<T>, ROW_GROUPS<T, DH>);
-    return launch(win_bwd_dkv_kernel<T, DH, false>, (long long)a.N * a.Hkv * ((a.Tk + s.kg * BQ - 1) / (s.kg * BQ)), 64 * s.kg * s.qh, dkv_lds<T, DH>(s.kg, s.qh), st, a, s.kg, s.qh);
+                            dkv_lds<T, DH>(1, ROW_GROUPS<T, DH>, 1, 2), st, a, 1, ROW_GROUPS<T, DH>, 1, 2)) return rc;
+    constexpr int WAVES = 4;
+    const Shape s = shape_of(a, WAVES, MOST_WAVES<T>, ROW_GROUPS<T, DH>);
+    // all queries in one stage where they take no more LDS than lets two workgroups share a CU; else as many to a stage (barriers) as two buffers hold
+    const int all = s.qh == 1 && a.G == 1 ? (a.Tq + BQ - 1) / BQ : 0;
+    int u = WAVES / 2 / s.qh > 1 ? WAVES / 2 / s.qh : 1, buffers = 2;
+    if (all > 0 && dkv_lds<T, DH>(s.kg, 1, all, 1) <= SHARED_CU_LDS) { u = all; buffers = 1; }
+    return launch(win_bwd_dkv_kernel<T, DH, false>, (long long)a.N * a.Hkv * ((a.Tk + s.kg * BQ - 1) / (s.kg * BQ)), 64 * s.kg * s.qh, dkv_lds<T, DH>(s.kg, s.qh, u, buffers), st, a,
+                  s.kg, s.qh, u, buffers);
 }
 }  // namespace
 
