@@ -49,16 +49,20 @@ def _launch(name, code, params, device):
 
 
 def _on(t, like, name, dtypes, shape=None):
+    try:
+        if t.dtype in dtypes and t.get_device() == like.get_device() and (shape is None or t.shape == shape) and not (t.requires_grad and torch.is_grad_enabled()):
+            return
+    except AttributeError:
+        pass
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor")
     if t.dtype not in dtypes:
         raise TypeError(f"{name}: {t.dtype} where {' or '.join(map(str, dtypes))} is needed")
-    if not (t.device == like.device):
+    if t.device != like.device:
         raise ValueError(f"{name} is on {t.device}, not on {like.device}")
     if shape is not None and t.shape != shape:
         raise ValueError(f"{name} has shape {tuple(t.shape)}, not {tuple(shape)}")
-    if t.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{name} asks for a gradient: this package has no autograd, call the operator's _grad function on detached tensors")
+    raise ValueError(f"{name} asks for a gradient: this package has no autograd, call the operator's _grad function on detached tensors")
 
 
 def _ptr(t):
@@ -80,46 +84,60 @@ def _first(t, name):
 def _bound(x, name):
     if x is None:
         return -1
-    if not (x >= 0):
+    if x < 0:
         raise ValueError(f"{name} must be None (no bound) or at least 0")
     return min(int(x), _FAR)
 
 
 def _check_rows(t, like, name, shape):
     _on(t, like, name, (like.dtype,), shape)
-    if not (t.stride(3) == 1):
+    if t.stride(3) != 1:
         raise ValueError(f"the rows of {name} must be contiguous")
 
 
-def _attention(q, k, v, left, right, sinks, key_mask, kv_len, q_pos, scale):
-    """The checked arguments: (tail of the packed struct in front of the workspace, dtype code).  Strides and alignment are the C entry's to check."""
+def _complain(q, k, v):
+    """What is wrong with them, as an exception."""
     _first(q, "q")
-    if not (q.dim() == 4):
+    if q.dim() != 4:
         raise ValueError(f"q has shape {tuple(q.shape)}, not [N, Tq, H, dh]")
     _check_rows(q, q, "q", q.shape)
-    N, Tq, H, dh = q.shape
     _on(k, q, "k", (q.dtype,))
-    if not (k.dim() == 4 and k.shape[0] == N and k.shape[3] == dh):
-        raise ValueError(f"k has shape {tuple(k.shape)}, not [{N}, Tk, Hkv, {dh}]")
+    if k.dim() != 4 or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
+        raise ValueError(f"k has shape {tuple(k.shape)}, not [{q.shape[0]}, Tk, Hkv, {q.shape[3]}]")
     _check_rows(k, q, "k", k.shape)
     _check_rows(v, q, "v", k.shape)
-    Tk, Hkv = k.shape[1], k.shape[2]
+
+
+def _attention(q, k, v, left, right, sinks, key_mask, kv_len, q_pos, scale):
+    """The checked arguments: (strides of q, k and v, tail of the packed struct in front of the workspace, dtype code).  Alignment and what else the C entry
+    checks are left to it."""
+    try:
+        t, at, (N, Tq, H, dh), (Nk, Tk, Hkv, dk) = q.dtype, q.get_device(), q.shape, k.shape
+        sq, sk, sv = q.stride(), k.stride(), v.stride()
+        code = _DTYPES[t]
+        fine = (at >= 0 and k.dtype is t and v.dtype is t and k.get_device() == at and v.get_device() == at and N == Nk and dh == dk and v.shape == k.shape
+                and sq[3] == sk[3] == sv[3] == 1 and not ((q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled()))
+    except Exception:
+        fine = False
+    if not fine:
+        _complain(q, k, v)
+        raise ValueError("q, k and v do not fit together")
     if key_mask is not None:
         _on(key_mask, q, "key_mask", (torch.bool, torch.uint8), (N, Tk))
-        if not (key_mask.is_contiguous()):
+        if not key_mask.is_contiguous():
             raise ValueError("key_mask must be contiguous")
-    for t, name in ((kv_len, "kv_len"), (q_pos, "q_pos")):
-        if t is not None:
-            _on(t, q, name, (torch.int32,), (N,))
-            if not (t.is_contiguous()):
+    for x, name in ((kv_len, "kv_len"), (q_pos, "q_pos")):
+        if x is not None:
+            _on(x, q, name, (torch.int32,), (N,))
+            if not x.is_contiguous():
                 raise ValueError(f"{name} must be contiguous")
     scale = dh ** -0.5 if scale is None else float(scale)
-    if not (0.0 < scale < 3e38):
+    if not 0.0 < scale < 3e38:
         raise ValueError("scale must be positive and finite")
-    return (_ptr(key_mask), _ptr(kv_len), _ptr(q_pos), N, Tq, Tk, H, Hkv, dh, _bound(left, "left"), _bound(right, "right"), _bound(sinks or 0, "sinks"), scale), _DTYPES[q.dtype]
+    return (*sq[:3], *sk[:3], *sv[:3]), (_ptr(key_mask), _ptr(kv_len), _ptr(q_pos), N, Tq, Tk, H, Hkv, dh, _bound(left, "left"), _bound(right, "right"), _bound(sinks or 0, "sinks"), scale), code
 
 
-_NO_STRIDE = (0, 0, 0)
+_NO_STRIDES = (0,) * 12
 
 
 def window_attention(q, k, v, *, left=None, right=None, sinks=0, key_mask=None, kv_len=None, q_pos=None, scale=None, out=None):
@@ -131,14 +149,13 @@ def window_attention(q, k, v, *, left=None, right=None, sinks=0, key_mask=None, 
     no bound.  A row that sees nothing gives zeros and lse = -inf.  `out`: write there instead of into a new tensor.
 
     One new token behind a cache: Tq = 1, kv_len = the cache's lengths with the new key in place, q_pos = kv_len - 1, right = 0."""
-    tail, code = _attention(q, k, v, left, right, sinks, key_mask, kv_len, q_pos, scale)
+    strides, tail, code = _attention(q, k, v, left, right, sinks, key_mask, kv_len, q_pos, scale)
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         _check_rows(out, q, "out", q.shape)
     lse = q.new_empty((tail[3], tail[6], tail[4]), dtype=torch.float32)
-    fields = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), 0, 0, 0, 0, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3],
-              *_NO_STRIDE, *_NO_STRIDE, *_NO_STRIDE, *_NO_STRIDE, *tail)
+    fields = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), 0, 0, 0, 0, *strides, *out.stride()[:3], *_NO_STRIDES, *tail)
     size = _fn("dic_win_attn_ws_bytes")(code, 0, _WIN.pack(*fields, 0, 0))
     ws = q.new_empty(size, dtype=torch.uint8) if size else None
     _launch("dic_win_attn_fwd", code, _WIN.pack(*fields, _ptr(ws), size), q.device)
@@ -148,11 +165,11 @@ def window_attention(q, k, v, *, left=None, right=None, sinks=0, key_mask=None, 
 def window_attention_grad(dout, q, k, v, out, lse, *, left=None, right=None, sinks=0, key_mask=None, kv_len=None, q_pos=None, scale=None, grads=None):
     """(dq, dk, dv) of window_attention for the gradient `dout` of its output; the other arguments as they went into and came out of that call.
     `grads`: three tensors to write them into (views of a packed gradient, say).  dk and dv are summed over the query heads of each key head."""
-    tail, code = _attention(q, k, v, left, right, sinks, key_mask, kv_len, q_pos, scale)
+    strides, tail, code = _attention(q, k, v, left, right, sinks, key_mask, kv_len, q_pos, scale)
     _on(dout, q, "dout", (q.dtype,), q.shape)
     _check_rows(out, q, "out", q.shape)
     _on(lse, q, "lse", (torch.float32,), (tail[3], tail[6], tail[4]))
-    if not (lse.is_contiguous()):
+    if not lse.is_contiguous():
         raise ValueError("lse must be contiguous")
     per = 16 // q.element_size()
     if not dout.is_contiguous() and (dout.stride(3) != 1 or any(s % per for s in dout.stride()[:3])) or dout.data_ptr() % 16:
@@ -164,7 +181,7 @@ def window_attention_grad(dout, q, k, v, out, lse, *, left=None, right=None, sin
         for t, like, name in ((dq, q, "dq"), (dk, k, "dk"), (dv, k, "dv")):
             _check_rows(t, q, name, like.shape)
     fields = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-              *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3], *dout.stride()[:3], *dq.stride()[:3], *dk.stride()[:3], *dv.stride()[:3], *tail)
+              *strides, *out.stride()[:3], *dout.stride()[:3], *dq.stride()[:3], *dk.stride()[:3], *dv.stride()[:3], *tail)
     size = _fn("dic_win_attn_ws_bytes")(code, 1, _WIN.pack(*fields, 0, 0))
     ws = q.new_empty(size, dtype=torch.uint8) if size else None
     _launch("dic_win_attn_bwd", code, _WIN.pack(*fields, _ptr(ws), size), q.device)
@@ -184,12 +201,12 @@ def _norm(norm, like, D, side):
     """The packed fields of one norm."""
     if norm is None:
         return 0, 0, 0, 0.0
-    if not (norm.kind in _KINDS):
+    if norm.kind not in _KINDS:
         raise ValueError(f'{side}: a norm is "layer" or "rms"')
     for t, name in ((norm.weight, "weight"), (norm.bias, "bias")):
         if t is not None:
             _on(t, like, f"{side} {name}", (torch.float32,), (D,))
-            if not (t.is_contiguous()):
+            if not t.is_contiguous():
                 raise ValueError(f"{side} {name} must be contiguous")
     return _ptr(norm.weight), _ptr(norm.bias), _KINDS[norm.kind], float(norm.eps)
 
@@ -213,7 +230,7 @@ def _shapes(x, gate):
 
 def _packed(t, like, name, dtype):
     _on(t, like, name, (dtype,), like.shape)
-    if not (t.is_contiguous()):
+    if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
 
 
@@ -275,7 +292,7 @@ def gated_norm_grad(dx_new, da, x_new, y, saved, *, post=None, gate=None, residu
     rows, D, per_gate = _shapes(x_new, gate)
     sides = *_norm(post, x_new, D, "post"), *_norm(pre, x_new, D, "pre")
     _on(saved, x_new, "saved", (torch.float32,), (4, rows))
-    if not (saved.is_contiguous()):
+    if not saved.is_contiguous():
         raise ValueError("saved must be contiguous")
     got = {"dx": torch.empty_like(x_new)}
     if y is not None:

@@ -184,7 +184,7 @@ __global__ __launch_bounds__((Team<TPR, NV>::THREADS)) void gated_norm_fwd_kerne
     vs.set(vec, tm, W1, p.pre.w, 1.f, p.D); vs.set(vec, tm, B1, p.pre.b, 0.f, p.D);
     if constexpr (VS::SHARED) __syncthreads();
     f32x4 g[NV];
-    long long seg = -1;
+    long long seg_end = 0;
     tm.load_or(nullptr, 1.f, g);
     // consecutive rows stay in a workgroup: the gate row changes rarely
     const long long per = ((p.rows + gridDim.x - 1) / gridDim.x + TM::TEAMS - 1) / TM::TEAMS * TM::TEAMS;
@@ -196,7 +196,11 @@ __global__ __launch_bounds__((Team<TPR, NV>::THREADS)) void gated_norm_fwd_kerne
         f32x4 v[NV], n[NV];
 #pragma unroll
         for (int c = 0; c < NV; ++c) { v[c] = rx[c].f(); n[c] = ry[c].f(); }
-        if (p.gate && row / p.seg_rows != seg) { seg = row / p.seg_rows; tm.load_or(p.gate + seg * p.D, 1.f, g); }
+        if (p.gate && row >= seg_end) {
+            const long long seg = row / p.seg_rows;
+            seg_end = (seg + 1) * p.seg_rows;
+            tm.load_or(p.gate + seg * p.D, 1.f, g);
+        }
         if (row + TM::TEAMS < end) { tm.template load<TX>(p.x, (row + TM::TEAMS) * p.D, rx); if (p.y) tm.template load<T>(p.y, (row + TM::TEAMS) * p.D, ry); }
         float m2 = 0.f, r2 = 0.f, m1 = 0.f, r1 = 0.f;
         if (p.y) {

@@ -508,6 +508,9 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 4>)) void win_
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dk, dv
+// Fragments of a key group's values that stay in LDS instead of registers: at 128 wide bf16 rows the accumulators and both operands take all 256 registers
+// that two waves a SIMD leave each, and one that was reloaded from scratch memory in every turn made the turn wait for the next stage's DMA, too.
+template <typename T, int DH> constexpr int PARKED = sizeof(T) == 2 && DH == 128 ? 4 : 0;
 // A workgroup owns kg groups of 32 keys and walks the queries that see them, 32 qh at a time: wave w takes key group w % kg and query rows 32 (w / kg).
 // The qh partial sums of a key group are added through LDS at the end.  A stage holds u of those row groups for each; all queries in one stage, and one
 // buffer, where they are few.
@@ -542,7 +545,9 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 3>)) void win_
     int t0 = 0, t1 = nq * a.G;                                                // tiles of queries, head by head
     if (SINK) { const int per = (t1 + a.chunks - 1) / a.chunks; t0 = min(chunk * per, t1); t1 = min(t0 + per, t1); }
 
-    typename M::Frag kf[L::NF], vf[L::NF];
+    constexpr int PK = PARKED<T, DH>;
+    typename M::Frag kf[L::NF], vf[L::NF - PK];
+    char* parked = smem + buffers * stage + key_group * PK * 1024 + lane * 16;
     {
         const char* pk = (const char*)((const T*)a.k + n * a.sk.n + jc * a.sk.t + hk * a.sk.h);
         const char* pv = (const char*)((const T*)a.v + n * a.sv.n + jc * a.sv.t + hk * a.sv.h);
@@ -550,7 +555,9 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 3>)) void win_
 #pragma unroll
         for (int s = 0; s < L::NF; ++s) {
             kf[s] = seen ? *(const typename M::Frag*)(pk + 32 * s + 16 * hi) : zero;
-            vf[s] = seen ? *(const typename M::Frag*)(pv + 32 * s + 16 * hi) : zero;
+            const typename M::Frag v = seen ? *(const typename M::Frag*)(pv + 32 * s + 16 * hi) : zero;
+            if (s < L::NF - PK) vf[s < L::NF - PK ? s : 0] = v;
+            else *(typename M::Frag*)(parked + (s - (L::NF - PK)) * 1024) = v;        // (waves of one key group write the same)
         }
         landed(kf);
         landed(vf);
@@ -588,7 +595,7 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 3>)) void win_
 #pragma unroll
             for (int f = 0; f < L::NF; ++f) {
                 s = M::mac(row_frag<T, DH>(qt, f, lane), kf[f], s);
-                dp = M::mac(row_frag<T, DH>(dt, f, lane), vf[f], dp);
+                dp = M::mac(row_frag<T, DH>(dt, f, lane), f < L::NF - PK ? vf[f < L::NF - PK ? f : 0] : *(const typename M::Frag*)(parked + (f - (L::NF - PK)) * 1024), dp);
             }
             __builtin_amdgcn_sched_barrier(0);
             if (!__all(bits == ~0u)) {
@@ -975,7 +982,7 @@ template <typename T, int DH> int fwd(const WinArgs& a, hipStream_t st) {
     return over_keys<T, DH, BN>(a, [&](auto nw, int waves, long long blocks, size_t lds) { return launch(win_fwd_kernel<T, DH, BN, decltype(nw)::value>, blocks, 64 * waves, lds, st, a); });
 }
 template <typename T, int DH> size_t dkv_lds(int kg, int qh, int u, int buffers) {
-    const size_t stages = (size_t)buffers * qh * u * (2 * Lay<T, DH>::bytes(BQ) + 256), sums = (size_t)(qh - 1) * kg * BQ * DH * sizeof(float);
+    const size_t stages = (size_t)buffers * qh * u * (2 * Lay<T, DH>::bytes(BQ) + 256) + kg * PARKED<T, DH> * 1024, sums = (size_t)(qh - 1) * kg * BQ * DH * sizeof(float);
     return stages > sums ? stages : sums;
 }
 template <typename T, int DH> int bwd(const WinArgs& a, hipStream_t st) {
