@@ -299,12 +299,10 @@ def gated_norm_grad(dx_new, da, x_new, y, saved, *, post=None, gate=None, residu
         got["dy"] = torch.empty_like(y)
     if gate is not None:
         got["gate"] = torch.empty_like(gate) if rows else torch.zeros_like(gate)
-    for norm, weight, bias in ((post, "post_weight", "post_bias"), (pre, "pre_weight", "pre_bias")):
-        if norm is not None:
-            if norm.weight is not None:
-                got[weight] = torch.empty_like(norm.weight)
-            if norm.bias is not None:
-                got[bias] = torch.empty_like(norm.bias)
+    names = [name for norm, side in ((post, "post"), (pre, "pre")) if norm is not None
+             for name, t in ((side + "_weight", norm.weight), (side + "_bias", norm.bias)) if t is not None]
+    if names:
+        got.update(zip(names, x_new.new_empty((len(names), D), dtype=torch.float32).unbind(0)))      # (one allocation)
     fields = (0, _ptr(y), x_new.data_ptr(), 0, _ptr(gate), saved.data_ptr(), _ptr(dx_new), _ptr(da), got["dx"].data_ptr(), _ptr(got.get("dy")), _ptr(got.get("gate")),
               _ptr(got.get("post_weight")), _ptr(got.get("post_bias")), _ptr(got.get("pre_weight")), _ptr(got.get("pre_bias")), *sides, rows, per_gate, D, residual_scale)
     size = _fn("dic_gated_norm_ws_bytes")(code, _NORM.pack(*fields, 0, 0))

@@ -122,6 +122,14 @@ CASES = {
     "many keys, few queries": (2, 5, 1000, 8, 1, 128, None, 0, 0),
     "few keys, many queries": (2, 400, 20, 2, 2, 64, 50, None, 2),
     "group of 8": (1, 150, 150, 16, 2, 64, 40, 0, 1),
+    "every query sees far keys": (1, 1500, 1500, 2, 1, 64, 10, 0, 3),
+    "many far keys, wide rows": (2, 1100, 1100, 4, 2, 128, 20, 5, 70),
+    "one query, keys for several workgroups": (1, 1, 3000, 2, 2, 64, None, 0, 0),
+    "32 rows, keys for several workgroups": (1, 8, 2000, 8, 2, 128, 1500, 0, 40),
+    "256 rows and keys": (2, 256, 256, 2, 2, 64, 100, 100, 2),
+    "257 rows and keys": (1, 257, 257, 2, 2, 64, 100, 100, 2),
+    "many short sequences": (300, 40, 40, 2, 1, 64, 12, 12, 1),
+    "many sequences, wide rows": (140, 130, 130, 2, 2, 128, 50, 0, 2),
 }
 
 
@@ -190,6 +198,44 @@ def test_query_positions(dtype):
         out, lse = dic.window_attention(q, k, v, **how)
         for name, t in zip(("out", "lse", "dq", "dk", "dv"), (out, lse, *dic.window_attention_grad(dout, q, k, v, out, lse, **how))):
             holds(name, t, want[name])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("Tq", [2, 60])
+def test_masks_of_more_tiles_than_are_read_at_once(dtype, Tq):
+    """A mask over 35000 keys (547 tiles of 64, 1094 of 32), most of them hidden; the queries stand at the end."""
+    Tk = 35000
+    mask = torch.rand(1, Tk, generator=torch.Generator().manual_seed(9)).cuda() < 0.3
+    pos = torch.tensor([Tk - Tq], dtype=torch.int32, device="cuda")
+    run_both(dtype, (1, Tq, Tk, 1, 1, 64, None, 0, 0), key_mask=mask, q_pos=pos, spoil=True)
+    run_both(dtype, (1, Tq, Tk, 1, 1, 64, 30000, 0, 5), key_mask=mask, q_pos=pos, spoil=True)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "fp32"])
+def test_far_keys_with_masks_lengths_and_positions(dtype):
+    """Keys that all queries see beside windows of 25, where some of them are hidden, or behind a sequence's end, or the queries start elsewhere."""
+    N, T = 3, 900
+    mask = torch.ones(N, T, dtype=torch.bool, device="cuda")
+    mask[1, 3:20] = False
+    lens = torch.tensor([T, 700, 9], dtype=torch.int32, device="cuda")
+    pos = torch.tensor([0, 40, -30], dtype=torch.int32, device="cuda")
+    run_both(dtype, (N, T, T, 2, 1, 64, 20, 4, 40), key_mask=mask, kv_len=lens, q_pos=pos, spoil=True)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("T", [50, 400])
+def test_large_logits(dtype, T):
+    """Logits in the hundreds: the maximum moves far from tile to tile, most probabilities vanish."""
+    g = torch.Generator(device="cuda").manual_seed(T)
+    q, k, v, dout = (torch.randn(1, T, 2, 64, generator=g, device="cuda").to(dtype) for _ in range(4))
+    ramp = torch.linspace(-1, 1, T, device="cuda").view(1, T, 1, 1)
+    k = (k * 4 + 20 * ramp * torch.sign(q.mean(1, keepdim=True))).to(dtype)
+    want = definition(q, k, v, visible(1, T, T, None, 0, 0, None, None, None), 1.0, dout)
+    out, lse = dic.window_attention(q, k, v, right=0, scale=1.0)
+    for name, t in zip(("out", "lse", "dq", "dk", "dv"), (out, lse, *dic.window_attention_grad(dout, q, k, v, out, lse, right=0, scale=1.0))):
+        value, bound = want[name]
+        off = (t.double() - value).abs()
+        assert (off <= bound + 1e-30).all(), (name, float((off - bound).max()))
 
 
 @pytest.mark.parametrize("Tq,Tk", [(0, 5), (5, 0), (0, 0)])
