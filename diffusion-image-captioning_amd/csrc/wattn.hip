@@ -198,6 +198,36 @@ __device__ __forceinline__ typename Mma<T>::Frag row_frag(const char* tile, int 
     return *(const typename Mma<T>::Frag*)(tile + Lay<T, DH>::row_base(lane) + Lay<T, DH>::step(s));
 }
 
+// An accumulated block (lane = row, registers = elements) times `mul` into a tensor: lane's row at `to`.
+template <typename T, int DH> __device__ __forceinline__ void store_row(const f32x16 (&acc)[DH / 32], float mul, T* to, int hi) {
+#pragma unroll
+    for (int d = 0; d < DH / 32; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) Mma<T>::st4(to + 32 * d + tok(r, hi), acc[d][r] * mul, acc[d][r + 1] * mul, acc[d][r + 2] * mul, acc[d][r + 3] * mul);
+}
+// The same through LDS (32 rows of ROWB + 16 bytes, the wave's own) into 32 rows, `rows` of them real: a store instruction then writes whole rows instead of
+// 16 bytes of each of 32.  It takes registers and a barrier, and pays in the dk / dv kernel for 128 wide bf16 rows alone (205 -> 187 us at 2 x 4096 keys, 16
+// heads; 117 -> 126 us for 64 wide rows; forward and dq, any type: no difference).
+template <typename T, int DH> constexpr int OUT_ROW = Lay<T, DH>::ROWB + 16;
+template <typename T, int DH> constexpr bool WHOLE_ROWS = sizeof(T) == 2 && DH == 128;
+template <typename T, int DH>
+__device__ __forceinline__ void store_rows(char* lds, const f32x16 (&acc)[DH / 32], float mul, T* to, long long stride, int rows, int lane) {
+    using L = Lay<T, DH>;
+    const int hi = lane >> 5;
+    char* mine = lds + (lane & 31) * OUT_ROW<T, DH>;
+#pragma unroll
+    for (int d = 0; d < L::ND; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4)
+            Mma<T>::st4((T*)mine + 32 * d + tok(r, hi), acc[d][r] * mul, acc[d][r + 1] * mul, acc[d][r + 2] * mul, acc[d][r + 3] * mul);
+#pragma unroll
+    for (int e = 0; e < 32 * L::CH / 64; ++e) {
+        const int row = (e * 64 + lane) / L::CH, c = (e * 64 + lane) % L::CH;
+        const i32x4 v = *(const i32x4*)(lds + row * OUT_ROW<T, DH> + c * 16);
+        if (row < rows) *(i32x4*)((char*)(to + row * stride) + c * 16) = v;
+    }
+}
+
 __device__ __forceinline__ unsigned long long below(int x) { return x <= 0 ? 0ull : x >= 64 ? ~0ull : (1ull << x) - 1ull; }
 __device__ __forceinline__ int clampi(int x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : x; }
 
@@ -310,7 +340,7 @@ template <typename T, int DH, int BN, int NW> struct KeyTiles {
 
 // ------------------------------------------------------------------------------------------------ forward
 template <typename T, int DH, int BN, int NW>
-__global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 4>)) void win_fwd_kernel(const WinArgs a) {
+__global__ __launch_bounds__(64 * MOST_WAVES<T>, (DH == 128 && BN == 32 && sizeof(T) == 2 ? 3 : RESIDENT<T, DH, 4>)) void win_fwd_kernel(const WinArgs a) {
     using L = Lay<T, DH>;
     using M = Mma<T>;
     constexpr int NB = BN / 32, TILE = L::bytes(BN);
@@ -410,12 +440,7 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 4>)) void win_
     }
     l += __shfl_xor(l, 32, 64);
     if (i < a.Tq) {
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        T* o = (T*)a.out + n * a.so.n + i * a.so.t + h * a.so.h;
-#pragma unroll
-        for (int d = 0; d < L::ND; ++d)
-#pragma unroll
-            for (int r = 0; r < 16; r += 4) M::st4(o + 32 * d + tok(r, hi), acc[d][r] * inv, acc[d][r + 1] * inv, acc[d][r + 2] * inv, acc[d][r + 3] * inv);
+        store_row<T, DH>(acc, l == 0.f ? 0.f : 1.f / l, (T*)a.out + n * a.so.n + i * a.so.t + h * a.so.h, hi);
         if (a.lse && hi == 0) a.lse[((long long)n * a.H + h) * a.Tq + i] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * LN2;
     }
 }
@@ -497,14 +522,7 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 4>)) void win_
             }
         }
     }
-    if (i < a.Tq) {
-        T* o = (T*)a.dq + n * a.sdq.n + i * a.sdq.t + h * a.sdq.h;
-#pragma unroll
-        for (int d = 0; d < L::ND; ++d)
-#pragma unroll
-            for (int r = 0; r < 16; r += 4)
-                M::st4(o + 32 * d + tok(r, hi), acc[d][r] * a.scale, acc[d][r + 1] * a.scale, acc[d][r + 2] * a.scale, acc[d][r + 3] * a.scale);
-    }
+    if (i < a.Tq) store_row<T, DH>(acc, a.scale, (T*)a.dq + n * a.sdq.n + i * a.sdq.t + h * a.sdq.h, hi);
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dk, dv
@@ -640,10 +658,10 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 3>)) void win_
         };
         add(dk);
         add(dv);
-        if (row_group > 0) return;
     }
+    const bool owner = row_group == 0;                                        // has its key group's sums
     if (SINK) {
-        if (j < a.sink_rows) {
+        if (owner && j < a.sink_rows) {
             float* o = a.sinks_ws + (((long long)(n * a.Hkv + hk) * a.chunks + chunk) * a.sink_rows + j) * 2 * DH;
 #pragma unroll
             for (int d = 0; d < L::ND; ++d)
@@ -655,8 +673,8 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 3>)) void win_
         }
         return;
     }
-    if (j < a.Tk) {
-        for (int c = 0; j < a.sink_keys && c < a.chunks; ++c) {
+    if (owner && j < a.sink_keys) {
+        for (int c = 0; c < a.chunks; ++c) {
             const float* o = a.sinks_ws + (((long long)(n * a.Hkv + hk) * a.chunks + c) * a.sink_rows + j) * 2 * DH;
 #pragma unroll
             for (int d = 0; d < L::ND; ++d)
@@ -667,15 +685,20 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 3>)) void win_
                     for (int e = 0; e < 4; ++e) { dk[d][r + e] += x[e]; dv[d][r + e] += y[e]; }
                 }
         }
-        T* ok = (T*)a.dk + n * a.sdk.n + j * a.sdk.t + hk * a.sdk.h;
-        T* ov = (T*)a.dv + n * a.sdv.n + j * a.sdv.t + hk * a.sdv.h;
-#pragma unroll
-        for (int d = 0; d < L::ND; ++d)
-#pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-                M::st4(ok + 32 * d + tok(r, hi), dk[d][r] * a.scale, dk[d][r + 1] * a.scale, dk[d][r + 2] * a.scale, dk[d][r + 3] * a.scale);
-                M::st4(ov + 32 * d + tok(r, hi), dv[d][r], dv[d][r + 1], dv[d][r + 2], dv[d][r + 3]);
-            }
+    }
+    T* ok = (T*)a.dk + n * a.sdk.n + hk * a.sdk.h;
+    T* ov = (T*)a.dv + n * a.sdv.n + hk * a.sdv.h;
+    if constexpr (WHOLE_ROWS<T, DH>) {
+        __syncthreads();                                                      // the stages are done with
+        const int j0 = jb + key_group * BQ;
+        if (owner && j0 < a.Tk) {
+            char* mine = smem + key_group * 32 * OUT_ROW<T, DH>;
+            store_rows<T, DH>(mine, dk, a.scale, ok + j0 * a.sdk.t, a.sdk.t, a.Tk - j0, lane);
+            store_rows<T, DH>(mine, dv, 1.f, ov + j0 * a.sdv.t, a.sdv.t, a.Tk - j0, lane);
+        }
+    } else if (owner && j < a.Tk) {
+        store_row<T, DH>(dk, a.scale, ok + j * a.sdk.t, hi);
+        store_row<T, DH>(dv, 1.f, ov + j * a.sdv.t, hi);
     }
 }
 
@@ -913,8 +936,13 @@ void plan_sinks(WinArgs& a) {
 long long sink_floats(const WinArgs& a, int dh) { return (long long)a.N * a.Hkv * a.chunks * a.sink_rows * 2 * dh; }
 // Few query rows: one workgroup per key head and sequence, or several that share the keys while that fills the card and leaves each 8 tiles to read.
 bool few_rows(const WinArgs& a) { return a.G * (long long)a.Tq <= FEW && a.Tk > 64; }
+// Keys that the rows of one key head see together when they are few, at most (where the host can tell: no lengths, no masks).
+long long span_keys(const WinArgs& a) {
+    const long long seen = a.left < 0 || a.right < 0 ? a.Tk : (long long)a.left + a.right + 1 + (a.sinks < a.Tk ? a.sinks : a.Tk);
+    return seen < a.Tk ? seen : a.Tk;
+}
 int splits_of(const WinArgs& a) {
-    const long long seen = a.left < 0 || a.right < 0 ? a.Tk : (long long)a.left + a.right + a.Tq + 2 * FEW + (a.sinks < a.Tk ? a.sinks : a.Tk);
+    const long long seen = span_keys(a) + a.Tq + 2 * FEW;
     const long long tiles = ((seen < a.Tk ? seen : a.Tk) + FEW - 1) / FEW, units = (long long)a.N * a.Hkv, want = (512 + units - 1) / units, most = tiles / 8;
     const long long s = want < most ? want : most;
     return s > 1 ? (int)s : 1;
@@ -979,11 +1007,18 @@ template <typename T, int DH> int fwd(const WinArgs& a, hipStream_t st) {
         if (int rc = launch(win_few_kernel<T, DH>, (long long)a.N * a.Hkv * splits, 64 * Few<T, DH>::NW, Few<T, DH>::LDS, st, a, splits)) return rc;
         return splits > 1 ? launch(win_merge_kernel<T, DH>, ((long long)a.N * a.H * a.Tq + 3) / 4, 256, 0, st, a, splits) : 0;
     }
+    // 128 wide rows that see many keys: tiles of 32, which take the registers and LDS of three workgroups a CU instead of two (one text of 8192 rows, 4096 keys
+    // each, 16 heads: 249 us against 277; rows of 1024 keys, 2 x 4096 rows: 104 us against 96)
+    if constexpr (sizeof(T) == 2 && DH == 128)
+        if (span_keys(a) >= 2048)
+            return launch(win_fwd_kernel<T, DH, 32, 4>, (long long)a.N * a.H * ((a.Tq + 4 * BQ - 1) / (4 * BQ)), 256, 
+                          (size_t)4 * Lay<T, DH>::bytes(32), st, a);
     return over_keys<T, DH, BN>(a, [&](auto nw, int waves, long long blocks, size_t lds) { return launch(win_fwd_kernel<T, DH, BN, decltype(nw)::value>, blocks, 64 * waves, lds, st, a); });
 }
 template <typename T, int DH> size_t dkv_lds(int kg, int qh, int u, int buffers) {
     const size_t stages = (size_t)buffers * qh * u * (2 * Lay<T, DH>::bytes(BQ) + 256) + kg * PARKED<T, DH> * 1024, sums = (size_t)(qh - 1) * kg * BQ * DH * sizeof(float);
-    return stages > sums ? stages : sums;
+    const size_t out = WHOLE_ROWS<T, DH> ? (size_t)kg * 32 * OUT_ROW<T, DH> : 0, most = stages > sums ? stages : sums;
+    return most > out ? most : out;
 }
 template <typename T, int DH> int bwd(const WinArgs& a, hipStream_t st) {
     constexpr int BN = sizeof(T) == 2 ? 64 : 32;
