@@ -446,6 +446,27 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (DH == 128 && BN == 32 && sizeo
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dq (and delta)
+// acc += the part of dq / scale that 32 keys have; bit of `word`: the lane's query sees that key (`full`: all of them)
+template <typename T, int DH>
+__device__ __forceinline__ void dq_block(const char* kt, const char* vt, const typename Mma<T>::Frag (&qf)[Lay<T, DH>::NF], const typename Mma<T>::Frag (&df)[Lay<T, DH>::NF],
+                                         float c, float l2, float delta, unsigned word, bool full, f32x16 (&acc)[DH / 32], int lane) {
+    using L = Lay<T, DH>;
+    using M = Mma<T>;
+    f32x16 st = zero16(), dp = zero16();
+#pragma unroll
+    for (int s = 0; s < L::NF; ++s) {
+        st = M::mac(row_frag<T, DH>(kt, s, lane), qf[s], st);
+        dp = M::mac(row_frag<T, DH>(vt, s, lane), df[s], dp);
+    }
+    const unsigned w = word >> (4 * (lane >> 5));
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        const float p = __builtin_amdgcn_exp2f(fmaf(st[r], c, -l2)) * (dp[r] - delta);
+        st[r] = full || ((w >> tok(r, 0)) & 1u) ? p : 0.f;
+    }
+#pragma unroll
+    for (int d = 0; d < L::ND; ++d) acc[d] = M::mac_t(M::template turned<DH>(kt, d, lane), M::right(st), acc[d]);
+}
 template <typename T, int DH, int BN, int NW>
 __global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 4>)) void win_bwd_dq_kernel(const WinArgs a) {
     using L = Lay<T, DH>;
@@ -505,20 +526,7 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 4>)) void win_
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 if (!full && !__any((unsigned)(bits >> (32 * b)) != 0)) continue;
-                f32x16 st = zero16(), dp = zero16();
-#pragma unroll
-                for (int s = 0; s < L::NF; ++s) {
-                    st = M::mac(row_frag<T, DH>(kt + L::bytes(32 * b), s, lane), qf[s], st);
-                    dp = M::mac(row_frag<T, DH>(vt + L::bytes(32 * b), s, lane), df[s], dp);
-                }
-                const unsigned w = (unsigned)(bits >> (32 * b)) >> (4 * hi);
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const float p = __builtin_amdgcn_exp2f(fmaf(st[r], a.c, -l2)) * (dp[r] - delta);
-                    st[r] = full || ((w >> tok(r, 0)) & 1u) ? p : 0.f;
-                }
-#pragma unroll
-                for (int d = 0; d < L::ND; ++d) acc[d] = M::mac_t(M::template turned<DH>(kt + L::bytes(32 * b), d, lane), M::right(st), acc[d]);
+                dq_block<T, DH>(kt + L::bytes(32 * b), vt + L::bytes(32 * b), qf, df, a.c, l2, delta, (unsigned)(bits >> (32 * b)), full, acc, lane);
             }
         }
     }
@@ -699,6 +707,143 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 3>)) void win_
     } else if (owner && j < a.Tk) {
         store_row<T, DH>(dk, a.scale, ok + j * a.sdk.t, hi);
         store_row<T, DH>(dv, 1.f, ov + j * a.sdv.t, hi);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ backward of short sequences
+// dk / scale and dv += the parts of 32 queries with the statistics st2; bit of `bits`: that query sees the lane's key.  (The dk / dv kernel above has the
+// same steps in its loop: as a call of this function its 128 wide form spilled 19 registers there and took 237 us for 187.)
+template <typename T, int DH>
+__device__ __forceinline__ void dkv_block(const char* qt, const char* dt, const float* st2, const typename Mma<T>::Frag (&kf)[Lay<T, DH>::NF],
+                                          const typename Mma<T>::Frag (&vf)[Lay<T, DH>::NF - PARKED<T, DH>], const char* parked, float c, unsigned bits, f32x16 (&dk)[DH / 32],
+                                          f32x16 (&dv)[DH / 32], int lane) {
+    using L = Lay<T, DH>;
+    using M = Mma<T>;
+    constexpr int KEPT = L::NF - PARKED<T, DH>;
+    const int hi = lane >> 5;
+    f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+    for (int f = 0; f < L::NF; ++f) {
+        s = M::mac(row_frag<T, DH>(qt, f, lane), kf[f], s);
+        dp = M::mac(row_frag<T, DH>(dt, f, lane), f < KEPT ? vf[f < KEPT ? f : 0] : *(const typename M::Frag*)(parked + (f - KEPT) * 1024), dp);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (!__all(bits == ~0u)) {
+        const unsigned w = bits >> (4 * hi);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] = (w >> tok(e, 0)) & 1u ? s[e] : -INFINITY;
+    }
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+        const f32x4 l2 = *(const f32x4*)(st2 + tok(e, hi)), de = *(const f32x4*)(st2 + 32 + tok(e, hi));
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            s[e + x] = __builtin_amdgcn_exp2f(fmaf(s[e + x], c, -l2[x]));
+            dp[e + x] = s[e + x] * (dp[e + x] - de[x]);
+        }
+    }
+    const typename M::Right ps = M::right(s), pd = M::right(dp);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int d = 0; d < L::ND; ++d) {
+        dv[d] = M::mac_t(M::template turned<DH>(dt, d, lane), ps, dv[d]);
+        dk[d] = M::mac_t(M::template turned<DH>(qt, d, lane), pd, dk[d]);
+    }
+}
+// One workgroup has a head's queries and keys whole, wave w queries 32 w.. and keys 32 w.., and reads them once: keys and values lie in LDS and the wave's
+// query rows in registers for dq; then they change places, and dk and dv follow without another read.  3072 heads of 130 x 64 in bf16: 160 us for the two
+// kernels' 202; 8 tensors of 51 MB at 2.55 TB/s, where loading them alone would take 90 us: of 130 rows the fifth wave's 30 are padding, and two workgroups of
+// five waves share a CU (bounded to 128 registers, for three, it spilled 23 and took 177 us).
+template <typename T, int DH>
+__global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 3>)) void win_bwd_short_kernel(const WinArgs a) {
+    using L = Lay<T, DH>;
+    using M = Mma<T>;
+    constexpr int TILE = L::bytes(BQ), PK = PARKED<T, DH>;
+    extern __shared__ __attribute__((aligned(16))) char smem[];               // of every wave: two tiles, 64 statistics, parked values
+    __shared__ unsigned words[MOST_WAVES<T>];                                 // the keys that exist
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hi = lane >> 5, row = lane & 31, nw = blockDim.x >> 6;
+    const int item = xcd_item(), h = item % a.H, n = item / a.H;
+    const Seq sq = sequence(a, n);
+    const int i0 = wave * BQ, i = i0 + row, ic = min(i, a.Tq - 1);
+    char* const mine = smem + wave * 2 * TILE;
+    float* const stats = (float*)(smem + nw * 2 * TILE);
+    char* const parked = smem + nw * (2 * TILE + 256) + wave * PK * 1024 + lane * 16;
+    unsigned valid = 0;
+    if (i0 < a.Tk) {
+        const unsigned lds = (unsigned)(uintptr_t)(LDS_PTR(char))mine;
+        const long long kst = a.sk.t * (long long)sizeof(T), vst = a.sv.t * (long long)sizeof(T);
+        valid = (unsigned)(__ballot(mask_byte(a, n, i) != 0) & below(min(sq.kvl - i0, BQ)));
+        load_tile<T, DH, BQ, 1>((const char*)((const T*)a.k + n * a.sk.n + h * a.sk.h) + i0 * kst, (unsigned)kst, valid, lds, 0, 1, lane);
+        load_tile<T, DH, BQ, 1>((const char*)((const T*)a.v + n * a.sv.n + h * a.sv.h) + i0 * vst, (unsigned)vst, valid, lds + TILE, 0, 1, lane);
+    }
+    if (lane == 0) words[wave] = valid;
+    f32x16 acc[L::ND];
+    {
+        typename M::Frag qf[L::NF] = {}, df[L::NF] = {};                      // zeros behind the last query: nothing comes of them below
+        float delta = 0.f, l2 = INFINITY;
+        if (i < a.Tq) {
+            const char* p = (const char*)((const T*)a.q + n * a.sq.n + i * a.sq.t + h * a.sq.h);
+            const char* pd = (const char*)((const T*)a.dout + n * a.sdo.n + i * a.sdo.t + h * a.sdo.h);
+            const char* po = (const char*)((const T*)a.o + n * a.so.n + i * a.so.t + h * a.so.h);
+            l2 = a.lse[((long long)n * a.H + h) * a.Tq + i] * LOG2E;
+#pragma unroll
+            for (int s = 0; s < L::NF; ++s) {
+                qf[s] = *(const typename M::Frag*)(p + 32 * s + 16 * hi);
+                df[s] = *(const typename M::Frag*)(pd + 32 * s + 16 * hi);
+                delta += M::dot(df[s], *(const typename M::Frag*)(po + 32 * s + 16 * hi));
+            }
+        }
+        delta += __shfl_xor(delta, 32, 64);
+        if (l2 == -INFINITY) l2 = INFINITY;                                   // the query sees nothing
+        dma_barrier();
+#pragma unroll
+        for (int d = 0; d < L::ND; ++d) acc[d] = zero16();
+        if (i0 < a.Tq) {
+            const Span sp = span_of(a, sq.pos + ic, sq.kvl);
+            const int in_lo = span_of(a, sq.pos + min(i0 + 31, a.Tq - 1), sq.kvl).lo, in_hi = span_of(a, sq.pos + i0, sq.kvl).hi;
+            for (int j0 = 0; j0 < a.Tk; j0 += BQ) {
+                const unsigned there = (unsigned)__builtin_amdgcn_readfirstlane((int)words[j0 / BQ]);
+                const bool full = j0 >= in_lo && j0 + BQ <= in_hi && there == ~0u;
+                const unsigned bits = full ? ~0u : (unsigned)visible(sp, j0) & there;
+                if (!__any(bits != 0)) continue;
+                const char* kt = smem + j0 / BQ * 2 * TILE;
+                dq_block<T, DH>(kt, kt + TILE, qf, df, a.c, l2, delta, bits, full, acc, lane);
+            }
+            if (i < a.Tq) store_row<T, DH>(acc, a.scale, (T*)a.dq + n * a.sdq.n + i * a.sdq.t + h * a.sdq.h, hi);
+        }
+        typename M::Frag kf[L::NF], vf[L::NF - PK];
+#pragma unroll
+        for (int s = 0; s < L::NF; ++s) {
+            kf[s] = row_frag<T, DH>(mine, s, lane);
+            const typename M::Frag v = row_frag<T, DH>(mine + TILE, s, lane);
+            if (s < L::NF - PK) vf[s < L::NF - PK ? s : 0] = v;
+            else *(typename M::Frag*)(parked + (s - (L::NF - PK)) * 1024) = v;
+        }
+        __syncthreads();                                                      // nobody needs the keys' tiles any more
+#pragma unroll
+        for (int s = 0; s < L::NF; ++s) {
+            *(typename M::Frag*)(mine + L::row_base(lane) + L::step(s)) = qf[s];
+            *(typename M::Frag*)(mine + TILE + L::row_base(lane) + L::step(s)) = df[s];
+        }
+        stats[wave * 2 * BQ + lane] = hi ? delta : l2;
+        __syncthreads();
+        if (i0 >= a.Tk) return;
+        const bool seen = (valid >> row) & 1u;
+        const int lo = !seen || a.right < 0 ? 0 : clampi(i - a.right - sq.pos, 0, a.Tq);         // the queries that see key i: [lo, end)
+        const int end = !seen ? 0 : a.left < 0 || i < a.sinks ? a.Tq : clampi(i + a.left - sq.pos + 1, 0, a.Tq);
+        f32x16 dv[L::ND];
+#pragma unroll
+        for (int d = 0; d < L::ND; ++d) { acc[d] = zero16(); dv[d] = zero16(); }
+        for (int r = 0; r < a.Tq; r += BQ) {
+            const unsigned bits = (unsigned)(below(min(end - r, BQ)) & ~below(lo - r));
+            if (!__any(bits != 0)) continue;
+            const char* qt = smem + r / BQ * 2 * TILE;
+            dkv_block<T, DH>(qt, qt + TILE, stats + 2 * r, kf, vf, parked, a.c, bits, acc, dv, lane);
+        }
+        if (i < a.Tk) {
+            store_row<T, DH>(acc, a.scale, (T*)a.dk + n * a.sdk.n + i * a.sdk.t + h * a.sdk.h, hi);
+            store_row<T, DH>(dv, 1.f, (T*)a.dv + n * a.sdv.n + i * a.sdv.t + h * a.sdv.h, hi);
+        }
     }
 }
 
@@ -972,13 +1117,14 @@ WinArgs args_of(const DicWinAttnParams* p) {
     plan_sinks(a);
     return a;
 }
+constexpr int MOST_LDS = 150 << 10;                              // of a workgroup, beside what kernels hold under a name
 template <typename K, typename... More> int launch(K kernel, long long blocks, int threads, size_t lds, hipStream_t st, More... more) {
     if (lds > (64 << 10)) {                     // once for each device: the attribute belongs to its copy of the kernel
         static std::atomic<unsigned long long> allowed{0};
         int dev = 0;
         hipError_t e = hipGetDevice(&dev);
         if (e == hipSuccess && !((allowed.load(std::memory_order_relaxed) >> (dev & 63)) & 1)) {
-            e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 150 << 10);
+            e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, MOST_LDS);
             if (e == hipSuccess) allowed.fetch_or(1ull << (dev & 63), std::memory_order_relaxed);
         }
         if (e != hipSuccess) { dic_set_error(hipGetErrorString(e)); return (int)e; }
@@ -1022,6 +1168,13 @@ template <typename T, int DH> size_t dkv_lds(int kg, int qh, int u, int buffers)
 }
 template <typename T, int DH> int bwd(const WinArgs& a, hipStream_t st) {
     constexpr int BN = sizeof(T) == 2 ? 64 : 32;
+    const int waves = ((a.Tq > a.Tk ? a.Tq : a.Tk) + BQ - 1) / BQ;
+    const size_t whole = (size_t)waves * (2 * Lay<T, DH>::bytes(BQ) + 256 + PARKED<T, DH> * 1024);
+    // A head to a workgroup where there is one for every CU (128 wide bf16 rows, 1024 heads of 146: 131 us against 157 in two passes; 32 heads of 224: 33 against
+    // 28; fp32, 768 heads of 128 x 64: 116 against 142, 24 heads: 39 against 34), and always for rows of 128 bytes, of which a wave holds and multiplies the
+    // least (3072 heads of 130: 160 against 202 us; 12 heads of 146: 15 against 19, of 256: 22.5 against 23).
+    if (a.G == 1 && a.Tq > 0 && a.Tk > 0 && waves <= MOST_WAVES<T> && whole <= MOST_LDS && ((long long)a.N * a.H >= 256 || Lay<T, DH>::ROWB == 128))
+        return launch(win_bwd_short_kernel<T, DH>, (long long)a.N * a.H, 64 * waves, whole, st, a);
     if (a.Tq > 0)
         if (int rc = over_keys<T, DH, BN>(a, [&](auto nw, int waves, long long blocks, size_t lds) { return launch(win_bwd_dq_kernel<T, DH, BN, decltype(nw)::value>, blocks, 64 * waves, lds, st, a); }))
             return rc;

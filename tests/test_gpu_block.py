@@ -130,6 +130,12 @@ CASES = {
     "257 rows and keys": (1, 257, 257, 2, 2, 64, 100, 100, 2),
     "many short sequences": (300, 40, 40, 2, 1, 64, 12, 12, 1),
     "many sequences, wide rows": (140, 130, 130, 2, 2, 128, 50, 0, 2),
+    "heads of one workgroup": (130, 100, 70, 2, 2, 64, 20, 30, 1),
+    "heads of one workgroup, 128 rows": (128, 128, 128, 2, 2, 64, None, None, 0),
+    "heads of one workgroup, wide rows": (86, 200, 224, 3, 3, 128, 60, 0, 2),
+    "heads of one workgroup, few queries": (256, 3, 120, 1, 1, 128, None, 100, 0),
+    "wide rows, many keys": (1, 70, 2100, 2, 1, 128, None, None, 0),
+    "wide rows, windows over 2000 keys": (1, 2300, 2300, 1, 1, 128, 2060, 0, 3),
 }
 
 
@@ -182,6 +188,21 @@ def test_keys_that_nobody_may_see_are_not_read_into_results(dtype, Tq):
     for key_mask, kv_len in ((mask, None), (None, lens), (mask.to(torch.uint8), lens)):
         for left, right in ((None, None), (20, 0), (9, 30)):
             run_both(dtype, (N, Tq, Tk, 4, 2, 64, left, right, 2), key_mask=key_mask, kv_len=kv_len, spoil=True)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("Tq,Tk,dh", [(1, 40, 64), (60, 128, 64), (100, 33, 128), (128, 96, 128)])
+def test_heads_of_one_workgroup_with_masks_lengths_and_positions(dtype, Tq, Tk, dh):
+    """As many heads as let a workgroup take one whole in the backward pass, views of packed tensors, keys hidden in every way."""
+    N = 132
+    g = torch.Generator().manual_seed(Tq)
+    lens = torch.randint(0, Tk + 40, (N,), generator=g, dtype=torch.int32).cuda()
+    mask = (torch.rand(N, Tk, generator=g) < 0.7).cuda()
+    mask[5] = False
+    pos = torch.randint(-60, 60, (N,), generator=g, dtype=torch.int32).cuda()
+    run_both(dtype, (N, Tq, Tk, 2, 2, dh, 20, 10, 3), key_mask=mask, kv_len=lens, q_pos=pos, views=True, spoil=True)
+    run_both(dtype, (N, Tq, Tk, 2, 2, dh, None, None, 0), key_mask=mask, views=True, spoil=True)
+    run_both(dtype, (N, Tq, Tk, 2, 2, dh, 30, None, 50), kv_len=lens, q_pos=pos, spoil=True)
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "fp32"])
