@@ -231,12 +231,15 @@ __device__ __forceinline__ void store_rows(char* lds, const f32x16 (&acc)[DH / 3
 __device__ __forceinline__ unsigned long long below(int x) { return x <= 0 ? 0ull : x >= 64 ? ~0ull : (1ull << x) - 1ull; }
 __device__ __forceinline__ int clampi(int x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : x; }
 
-// The keys of one sequence that exist, and the position of its first query.
-struct Seq { int kvl, pos; };
+// The position of a sequence's first query, and the keys that none of its queries sees, which count as absent: those from kvl on (they do not exist, or
+// lie in front of everybody), and [sinks, from), behind everybody's window.
+struct Seq { int kvl, pos, from; };
 __device__ __forceinline__ Seq sequence(const WinArgs& a, int n) {
     Seq s;
     s.kvl = a.kv_len ? clampi(a.kv_len[n], 0, a.Tk) : a.Tk;
     s.pos = a.q_pos ? clampi(a.q_pos[n], -FAR / 2, FAR / 2) : 0;
+    if (a.right >= 0) s.kvl = clampi(s.pos + a.Tq + a.right, 0, s.kvl);
+    s.from = a.left < 0 ? 0 : max(0, s.pos - a.left);
     return s;
 }
 // Query at position t sees the keys [lo, hi) and [0, sk).
@@ -250,16 +253,20 @@ __device__ __forceinline__ Span span_of(const WinArgs& a, int t, int kvl) {
 }
 __device__ __forceinline__ unsigned long long visible(const Span& s, int j0) { return (below(s.hi - j0) & ~below(s.lo - j0)) | below(s.sk - j0); }
 
+// bits of the keys j0 .. j0 + 63 that somebody may see
+__device__ __forceinline__ unsigned long long there(const WinArgs& a, int kvl, int from, int j0) { return below(kvl - j0) & (~below(from - j0) | below(a.sinks - j0)); }
+
 // The key tiles that the queries at positions t0..t1 need: those of the sinks, then those of the windows.
 struct Walk {
-    int ns, w0, nt, kvl;
+    int ns, w0, nt, kvl, from;
     __device__ __forceinline__ int j0(int t, int bn) const { return (t < ns ? t : w0 + t - ns) * bn; }
 };
-__device__ __forceinline__ Walk walk_of(const WinArgs& a, int t0, int t1, int kvl, int bn) {
+__device__ __forceinline__ Walk walk_of(const WinArgs& a, int t0, int t1, const Seq& sq, int bn) {
     Walk w;
-    const int lo = span_of(a, t0, kvl).lo;
-    const Span e = span_of(a, t1, kvl);
-    w.kvl = kvl;
+    const int lo = span_of(a, t0, sq.kvl).lo;
+    const Span e = span_of(a, t1, sq.kvl);
+    w.kvl = sq.kvl;
+    w.from = sq.from;
     w.ns = (e.sk + bn - 1) / bn;
     w.w0 = max(lo / bn, w.ns);
     w.nt = w.ns + max(0, (e.hi + bn - 1) / bn - w.w0);
@@ -305,8 +312,7 @@ template <typename T, int DH, int BN, int NW> struct KeyTiles {
     }
     // bits of the keys of tile t that exist and are not masked
     __device__ __forceinline__ unsigned long long valid(int t) const {
-        const int there = wk.kvl - wk.j0(t, BN);
-        unsigned long long v = there >= BN ? below(BN) : below(there);
+        unsigned long long v = there(a, wk.kvl, wk.from, wk.j0(t, BN)) & below(BN);
         if (a.key_mask) {
             const unsigned long long m = table[t & (2 * MASK_RUN - 1)];
             v &= (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)m) | (unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((int)(m >> 32)) << 32;
@@ -353,7 +359,7 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (DH == 128 && BN == 32 && sizeo
     const int hk = item % a.Hkv, n = item / a.Hkv, h = hk * a.G + g;
     const Seq sq = sequence(a, n);
     const int i0 = qt * bm + wave * BQ, i = i0 + (lane & 31), ic = min(i, a.Tq - 1);
-    const Walk wk = walk_of(a, sq.pos + qt * bm, sq.pos + min(qt * bm + bm, a.Tq) - 1, sq.kvl, BN);
+    const Walk wk = walk_of(a, sq.pos + qt * bm, sq.pos + min(qt * bm + bm, a.Tq) - 1, sq, BN);
     const Span sp = span_of(a, sq.pos + ic, sq.kvl);
     const bool wave_rows = i0 < a.Tq;
     // what every row of this wave sees: [in_lo, in_hi)
@@ -481,7 +487,7 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 4>)) void win_
     const int hk = item % a.Hkv, n = item / a.Hkv, h = hk * a.G + g;
     const Seq sq = sequence(a, n);
     const int i0 = qt * bm + wave * BQ, i = i0 + (lane & 31), ic = min(i, a.Tq - 1);
-    const Walk wk = walk_of(a, sq.pos + qt * bm, sq.pos + min(qt * bm + bm, a.Tq) - 1, sq.kvl, BN);
+    const Walk wk = walk_of(a, sq.pos + qt * bm, sq.pos + min(qt * bm + bm, a.Tq) - 1, sq, BN);
     const Span sp = span_of(a, sq.pos + ic, sq.kvl);
     const bool wave_rows = i0 < a.Tq;
     const int in_lo = span_of(a, sq.pos + min(i0 + 31, a.Tq - 1), sq.kvl).lo, in_hi = span_of(a, sq.pos + min(i0, a.Tq - 1), sq.kvl).hi;
@@ -558,7 +564,7 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 3>)) void win_
     const int hk = item % a.Hkv, n = item / a.Hkv;
     const Seq sq = sequence(a, n);
     const int jb = kt * bn, j = jb + key_group * BQ + (lane & 31), jc = min(j, a.Tk - 1);
-    const bool seen = j < min(sq.kvl, keys) && (!a.key_mask || a.key_mask[(size_t)n * a.Tk + jc]);
+    const bool seen = j < min(sq.kvl, keys) && (j >= sq.from || j < a.sinks) && (!a.key_mask || a.key_mask[(size_t)n * a.Tk + jc]);
     // rows of queries whose window holds key jj: [first_row, end_row); the rows behind them see it if it is a sink
     auto first_row = [&](int jj) { return a.right < 0 ? 0 : clampi(jj - a.right - sq.pos, 0, a.Tq); };
     auto end_row = [&](int jj) { return a.left < 0 || jj < a.near_sinks ? a.Tq : clampi(jj + a.left - sq.pos + 1, 0, a.Tq); };
@@ -772,7 +778,7 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 3>)) void win_
     if (i0 < a.Tk) {
         const unsigned lds = (unsigned)(uintptr_t)(LDS_PTR(char))mine;
         const long long kst = a.sk.t * (long long)sizeof(T), vst = a.sv.t * (long long)sizeof(T);
-        valid = (unsigned)(__ballot(mask_byte(a, n, i) != 0) & below(min(sq.kvl - i0, BQ)));
+        valid = (unsigned)(__ballot(mask_byte(a, n, i) != 0) & there(a, sq.kvl, sq.from, i0));
         load_tile<T, DH, BQ, 1>((const char*)((const T*)a.k + n * a.sk.n + h * a.sk.h) + i0 * kst, (unsigned)kst, valid, lds, 0, 1, lane);
         load_tile<T, DH, BQ, 1>((const char*)((const T*)a.v + n * a.sv.n + h * a.sv.h) + i0 * vst, (unsigned)vst, valid, lds + TILE, 0, 1, lane);
     }
@@ -802,9 +808,9 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 3>)) void win_
             const Span sp = span_of(a, sq.pos + ic, sq.kvl);
             const int in_lo = span_of(a, sq.pos + min(i0 + 31, a.Tq - 1), sq.kvl).lo, in_hi = span_of(a, sq.pos + i0, sq.kvl).hi;
             for (int j0 = 0; j0 < a.Tk; j0 += BQ) {
-                const unsigned there = (unsigned)__builtin_amdgcn_readfirstlane((int)words[j0 / BQ]);
-                const bool full = j0 >= in_lo && j0 + BQ <= in_hi && there == ~0u;
-                const unsigned bits = full ? ~0u : (unsigned)visible(sp, j0) & there;
+                const unsigned keys = (unsigned)__builtin_amdgcn_readfirstlane((int)words[j0 / BQ]);
+                const bool full = j0 >= in_lo && j0 + BQ <= in_hi && keys == ~0u;
+                const unsigned bits = full ? ~0u : (unsigned)visible(sp, j0) & keys;
                 if (!__any(bits != 0)) continue;
                 const char* kt = smem + j0 / BQ * 2 * TILE;
                 dq_block<T, DH>(kt, kt + TILE, qf, df, a.c, l2, delta, bits, full, acc, lane);
@@ -872,7 +878,7 @@ __global__ __launch_bounds__((64 * Few<T, DH>::NW), 1) void win_few_kernel(const
     const int hk = item % a.Hkv, n = item / a.Hkv;
     const Seq sq = sequence(a, n);
     const int rc = min(r, rows - 1), g = rc / a.Tq, i = rc - g * a.Tq, h = hk * a.G + g;
-    Walk wk = walk_of(a, sq.pos, sq.pos + a.Tq - 1, sq.kvl, FEW);
+    Walk wk = walk_of(a, sq.pos, sq.pos + a.Tq - 1, sq, FEW);
     Span sp = span_of(a, sq.pos + i, sq.kvl);
     const Span s0 = span_of(a, sq.pos, sq.kvl), s1 = span_of(a, sq.pos + a.Tq - 1, sq.kvl);           // every row sees [s1.lo, s0.hi)
     const int per = (wk.nt + splits - 1) / splits, t0 = min(split * per, wk.nt), t1 = min(t0 + per, wk.nt);
@@ -889,7 +895,7 @@ __global__ __launch_bounds__((64 * Few<T, DH>::NW), 1) void win_few_kernel(const
     const long long kst = a.sk.t * (long long)sizeof(T), vst = a.sv.t * (long long)sizeof(T);
     char* mine = smem + wave * 4 * TILE;
     const unsigned lds = (unsigned)(uintptr_t)(LDS_PTR(char))mine;
-    auto valid_of = [&](int byte, int j0) { return __ballot(byte != 0) & below(min(FEW, wk.kvl - j0)); };
+    auto valid_of = [&](int byte, int j0) { return __ballot(byte != 0) & there(a, wk.kvl, wk.from, j0) & below(FEW); };
     auto issue = [&](int j0, unsigned long long valid, int buf) {
         load_tile<T, DH, FEW, 1>(kb + j0 * kst, (unsigned)kst, valid, lds + buf * 2 * TILE, 0, 1, lane);
         load_tile<T, DH, FEW, 1>(vb + j0 * vst, (unsigned)vst, valid, lds + buf * 2 * TILE + TILE, 0, 1, lane);
@@ -1048,6 +1054,11 @@ int check(int dtype, const DicWinAttnParams* p, bool bwd, bool pointers = true) 
     DIC_REQUIRE((!nq || (rows_q(p->q_stride) && rows_q(p->out_stride) && (!bwd || (rows_q(p->dout_stride) && rows_q(p->dq_stride)))))
                 && (!nk || (rows_k(p->k_stride) && rows_k(p->v_stride) && (!bwd || (rows_k(p->dk_stride) && rows_k(p->dv_stride))))),
                 "dic_win_attn: strides must be non-negative multiples of 16 bytes, and a token stride at most 16 MiB");
+    const void *in[5] = {p->q, p->k, p->v, bwd ? p->out : nullptr, bwd ? p->dout : nullptr}, *written[3] = {bwd ? p->dq : p->out, bwd ? p->dk : nullptr, bwd ? p->dv : nullptr};
+    for (int i = 0; i < 3; ++i) {
+        for (const void* x : in) DIC_REQUIRE(!written[i] || written[i] != x, "dic_win_attn: an output in place of an input");
+        DIC_REQUIRE(!written[i] || (written[i] != written[(i + 1) % 3]), "dic_win_attn: two outputs in one place");
+    }
     DIC_REQUIRE(bwd ? apart(p->dq_stride, p->N, p->Tq, p->H, p->dh) && apart(p->dk_stride, p->N, p->Tk, p->Hkv, p->dh) && apart(p->dv_stride, p->N, p->Tk, p->Hkv, p->dh)
                     : apart(p->out_stride, p->N, p->Tq, p->H, p->dh), "dic_win_attn: rows of an output overlap");
     return 0;
@@ -1118,18 +1129,18 @@ WinArgs args_of(const DicWinAttnParams* p) {
     return a;
 }
 constexpr int MOST_LDS = 150 << 10;                              // of a workgroup, beside what kernels hold under a name
-template <typename K, typename... More> int launch(K kernel, long long blocks, int threads, size_t lds, hipStream_t st, More... more) {
+template <auto KERNEL, typename... More> int launch(long long blocks, int threads, size_t lds, hipStream_t st, More... more) {
     if (lds > (64 << 10)) {                     // once for each device: the attribute belongs to its copy of the kernel
         static std::atomic<unsigned long long> allowed{0};
         int dev = 0;
         hipError_t e = hipGetDevice(&dev);
         if (e == hipSuccess && !((allowed.load(std::memory_order_relaxed) >> (dev & 63)) & 1)) {
-            e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, MOST_LDS);
+            e = hipFuncSetAttribute((const void*)KERNEL, hipFuncAttributeMaxDynamicSharedMemorySize, MOST_LDS);
             if (e == hipSuccess) allowed.fetch_or(1ull << (dev & 63), std::memory_order_relaxed);
         }
         if (e != hipSuccess) { dic_set_error(hipGetErrorString(e)); return (int)e; }
     }
-    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), lds, st, more...);
+    hipLaunchKernelGGL(KERNEL, dim3((unsigned)blocks), dim3(threads), lds, st, more...);
     DIC_CHECK_LAUNCH();
     return 0;
 }
@@ -1150,16 +1161,16 @@ template <typename T, int DH> int fwd(const WinArgs& a, hipStream_t st) {
     constexpr int BN = sizeof(T) == 2 ? 64 : 32;
     if (few_rows(a)) {
         const int splits = splits_of(a);
-        if (int rc = launch(win_few_kernel<T, DH>, (long long)a.N * a.Hkv * splits, 64 * Few<T, DH>::NW, Few<T, DH>::LDS, st, a, splits)) return rc;
-        return splits > 1 ? launch(win_merge_kernel<T, DH>, ((long long)a.N * a.H * a.Tq + 3) / 4, 256, 0, st, a, splits) : 0;
+        if (int rc = launch<win_few_kernel<T, DH>>((long long)a.N * a.Hkv * splits, 64 * Few<T, DH>::NW, Few<T, DH>::LDS, st, a, splits)) return rc;
+        return splits > 1 ? launch<win_merge_kernel<T, DH>>(((long long)a.N * a.H * a.Tq + 3) / 4, 256, 0, st, a, splits) : 0;
     }
     // 128 wide rows that see many keys: tiles of 32, which take the registers and LDS of three workgroups a CU instead of two (one text of 8192 rows, 4096 keys
     // each, 16 heads: 249 us against 277; rows of 1024 keys, 2 x 4096 rows: 104 us against 96)
     if constexpr (sizeof(T) == 2 && DH == 128)
         if (span_keys(a) >= 2048)
-            return launch(win_fwd_kernel<T, DH, 32, 4>, (long long)a.N * a.H * ((a.Tq + 4 * BQ - 1) / (4 * BQ)), 256, 
+            return launch<win_fwd_kernel<T, DH, 32, 4>>((long long)a.N * a.H * ((a.Tq + 4 * BQ - 1) / (4 * BQ)), 256, 
                           (size_t)4 * Lay<T, DH>::bytes(32), st, a);
-    return over_keys<T, DH, BN>(a, [&](auto nw, int waves, long long blocks, size_t lds) { return launch(win_fwd_kernel<T, DH, BN, decltype(nw)::value>, blocks, 64 * waves, lds, st, a); });
+    return over_keys<T, DH, BN>(a, [&](auto nw, int waves, long long blocks, size_t lds) { return launch<win_fwd_kernel<T, DH, BN, decltype(nw)::value>>(blocks, 64 * waves, lds, st, a); });
 }
 template <typename T, int DH> size_t dkv_lds(int kg, int qh, int u, int buffers) {
     const size_t stages = (size_t)buffers * qh * u * (2 * Lay<T, DH>::bytes(BQ) + 256) + kg * PARKED<T, DH> * 1024, sums = (size_t)(qh - 1) * kg * BQ * DH * sizeof(float);
@@ -1174,13 +1185,13 @@ template <typename T, int DH> int bwd(const WinArgs& a, hipStream_t st) {
     // 28; fp32, 768 heads of 128 x 64: 116 against 142, 24 heads: 39 against 34), and always for rows of 128 bytes, of which a wave holds and multiplies the
     // least (3072 heads of 130: 160 against 202 us; 12 heads of 146: 15 against 19, of 256: 22.5 against 23).
     if (a.G == 1 && a.Tq > 0 && a.Tk > 0 && waves <= MOST_WAVES<T> && whole <= MOST_LDS && ((long long)a.N * a.H >= 256 || Lay<T, DH>::ROWB == 128))
-        return launch(win_bwd_short_kernel<T, DH>, (long long)a.N * a.H, 64 * waves, whole, st, a);
+        return launch<win_bwd_short_kernel<T, DH>>((long long)a.N * a.H, 64 * waves, whole, st, a);
     if (a.Tq > 0)
-        if (int rc = over_keys<T, DH, BN>(a, [&](auto nw, int waves, long long blocks, size_t lds) { return launch(win_bwd_dq_kernel<T, DH, BN, decltype(nw)::value>, blocks, 64 * waves, lds, st, a); }))
+        if (int rc = over_keys<T, DH, BN>(a, [&](auto nw, int waves, long long blocks, size_t lds) { return launch<win_bwd_dq_kernel<T, DH, BN, decltype(nw)::value>>(blocks, 64 * waves, lds, st, a); }))
             return rc;
     if (a.Tk == 0) return 0;
     if (a.sink_keys > 0)
-        if (int rc = launch(win_bwd_dkv_kernel<T, DH, true>, (long long)a.N * a.Hkv * (a.sink_rows / BQ) * a.chunks, 64 * ROW_GROUPS<T, DH>,
+        if (int rc = launch<win_bwd_dkv_kernel<T, DH, true>>((long long)a.N * a.Hkv * (a.sink_rows / BQ) * a.chunks, 64 * ROW_GROUPS<T, DH>,
                             dkv_lds<T, DH>(1, ROW_GROUPS<T, DH>, 1, 2), st, a, 1, ROW_GROUPS<T, DH>, 1, 2)) return rc;
     constexpr int WAVES = 4;
     const Shape s = shape_of(a, WAVES, MOST_WAVES<T>, ROW_GROUPS<T, DH>);
@@ -1188,7 +1199,7 @@ template <typename T, int DH> int bwd(const WinArgs& a, hipStream_t st) {
     const int all = s.qh == 1 && a.G == 1 ? (a.Tq + BQ - 1) / BQ : 0;
     int u = WAVES / 2 / s.qh > 1 ? WAVES / 2 / s.qh : 1, buffers = 2;
     if (all > 0 && dkv_lds<T, DH>(s.kg, 1, all, 1) <= SHARED_CU_LDS) { u = all; buffers = 1; }
-    return launch(win_bwd_dkv_kernel<T, DH, false>, (long long)a.N * a.Hkv * ((a.Tk + s.kg * BQ - 1) / (s.kg * BQ)), 64 * s.kg * s.qh, dkv_lds<T, DH>(s.kg, s.qh, u, buffers), st, a,
+    return launch<win_bwd_dkv_kernel<T, DH, false>>((long long)a.N * a.Hkv * ((a.Tk + s.kg * BQ - 1) / (s.kg * BQ)), 64 * s.kg * s.qh, dkv_lds<T, DH>(s.kg, s.qh, u, buffers), st, a,
                   s.kg, s.qh, u, buffers);
 }
 }  // namespace

@@ -296,10 +296,11 @@ int dic_attn_bwd(int dtype, const void* qkv, const uint8_t* key_mask, const void
  *     j < kv_len[n] (Tk without kv_len)   and   key_mask[n][j] != 0 (with key_mask [N][Tk])   and   j <= t + right (right >= 0)   and
  *     (j >= t - left (left >= 0)  or  j < sinks);                      left / right < 0: no bound on that side.
  * fwd: out = softmax(scale q k^T over the visible keys) v, lse [N][H][Tq] (optional) = the logarithm of the softmax's denominator.  A row that sees
- *     nothing gets out = 0 and lse = -inf.  Keys behind kv_len or masked by key_mask are never read into a result, whatever their rows hold.
+ *     nothing gets out = 0 and lse = -inf.  A key that no row of its sequence sees (behind kv_len, masked by key_mask, outside of every window) reaches no
+ *     result, whatever its rows of k and v hold.  (A row of q, k, v or dout that takes part and is not finite may reach results of other rows near it.)
  *     Sums, maxima and lse are fp32; with DIC_BF16 the probabilities are rounded to bf16 in front of the product with v.
  * bwd: dq, dk, dv from dout and the forward's out and lse; every row is written (zeros where nothing is seen).  Deterministic, no atomics.
- * kv_len is read as clamped to [0, Tk], q_pos to +-2^29.  ws: dic_win_attn_ws_bytes(dtype, backward, p) bytes, 16-byte aligned, private to the call
+ * No output may lie in place of an input or of another output.  kv_len is read as clamped to [0, Tk], q_pos to +-2^29.  ws: dic_win_attn_ws_bytes(dtype, backward, p) bytes, 16-byte aligned, private to the call
  * until it has run; N, Tq or Tk may be 0.                                                                                                    */
 typedef struct DicStrides { int64_t n, t, h; } DicStrides;            /* elements between sequences, tokens, heads */
 typedef struct DicWinAttnParams {

@@ -49,7 +49,7 @@ def test_packed_params_have_the_structs_sizes():
 def attn(**kw):
     p = dic._lib.WinAttnParams()
     base = dict(N=2, Tq=8, Tk=8, H=4, Hkv=2, dh=64, left=-1, right=-1, scale=0.125, ws=4096, ws_bytes=1 << 20)
-    base.update({n: 4096 for n in ("q", "k", "v", "out", "lse", "dout", "dq", "dk", "dv")})
+    base.update({n: 4096 * (i + 1) for i, n in enumerate(("q", "k", "v", "out", "lse", "dout", "dq", "dk", "dv"))})
     for n in ("q", "out", "dout", "dq"):
         base.update({f"{n}_stride_n": 8 * 256, f"{n}_stride_t": 256, f"{n}_stride_h": 64})
     for n in ("k", "v", "dk", "dv"):
@@ -72,6 +72,19 @@ def test_attention_refuses(kw):
     backward = {k: ({"out": "dq", "out_stride_t": "dq_stride_t"}.get(k, k)) for k in kw}
     assert L.dic_win_attn_fwd(1, C.byref(p), None) == 1001 and L.dic_last_error().startswith(b"dic_win_attn")
     assert L.dic_win_attn_bwd(1, C.byref(attn(**{backward[k]: v for k, v in kw.items()})), None) == 1001
+
+
+def test_attention_refuses_outputs_in_place_of_anything_else():
+    L = dic._lib.lib()
+    at = {n: getattr(attn(), n) for n in ("q", "k", "v", "out", "dout", "dq", "dk", "dv")}
+    for x in ("q", "k", "v"):
+        assert L.dic_win_attn_fwd(1, C.byref(attn(out=at[x])), None) == 1001 and b"in place of" in L.dic_last_error()
+    for y in ("dq", "dk", "dv"):
+        for x in ("q", "k", "v", "out", "dout"):
+            assert L.dic_win_attn_bwd(1, C.byref(attn(**{y: at[x]})), None) == 1001 and b"in place of" in L.dic_last_error()
+        for z in ("dq", "dk", "dv"):
+            if z != y:
+                assert L.dic_win_attn_bwd(1, C.byref(attn(**{y: at[z]})), None) == 1001 and b"in one place" in L.dic_last_error()
 
 
 def test_attention_refuses_other_types_and_missing_workspaces():

@@ -191,6 +191,25 @@ def test_keys_that_nobody_may_see_are_not_read_into_results(dtype, Tq):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("Tq,H,Hkv", [(1, 4, 2), (5, 2, 2), (40, 2, 2), (40, 4, 2), (150, 2, 1)])
+def test_keys_outside_of_every_window_are_not_read_into_results(dtype, Tq, H, Hkv):
+    """Rows of a cache in front of its newest token, and between the first keys and the oldest window, hold anything."""
+    N, Tk = 4, 333
+    pos = torch.tensor([0, 40, 170, Tk - Tq], dtype=torch.int32, device="cuda")
+    for left, right, sinks in ((None, 0, 0), (20, 0, 3), (70, 7, 40), (9, None, 2), (0, 0, 0)):
+        g = torch.Generator(device="cuda").manual_seed(Tq)
+        q, k, v, dout = (torch.randn(N, t, h, 64, generator=g, device="cuda").to(dtype) for t, h in ((Tq, H), (Tk, Hkv), (Tk, Hkv), (Tq, H)))
+        see = visible(N, Tq, Tk, left, right, sinks, None, None, pos.long())
+        want = definition(q, k, v, see, 0.125, dout)
+        dead = ~see.any(1)
+        k[dead], v[dead] = math.nan, INF
+        how = dict(left=left, right=right, sinks=sinks, q_pos=pos)
+        out, lse = dic.window_attention(q, k, v, **how)
+        for name, t in zip(("out", "lse", "dq", "dk", "dv"), (out, lse, *dic.window_attention_grad(dout, q, k, v, out, lse, **how))):
+            holds(name, t, want[name])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("Tq,Tk,dh", [(1, 40, 64), (60, 128, 64), (100, 33, 128), (128, 96, 128)])
 def test_heads_of_one_workgroup_with_masks_lengths_and_positions(dtype, Tq, Tk, dh):
     """As many heads as let a workgroup take one whole in the backward pass, views of packed tensors, keys hidden in every way."""
