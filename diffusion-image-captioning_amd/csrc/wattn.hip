@@ -452,29 +452,49 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (DH == 128 && BN == 32 && sizeo
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dq (and delta)
-// acc += the part of dq / scale that 32 keys have; bit of `word`: the lane's query sees that key (`full`: all of them)
-template <typename T, int DH>
-__device__ __forceinline__ void dq_block(const char* kt, const char* vt, const typename Mma<T>::Frag (&qf)[Lay<T, DH>::NF], const typename Mma<T>::Frag (&df)[Lay<T, DH>::NF],
-                                         float c, float l2, float delta, unsigned word, bool full, f32x16 (&acc)[DH / 32], int lane) {
+template <int ND> __device__ __forceinline__ float exactly(f32x16 (&acc)[ND], const f32x16 (&mean)[ND], float off) {        // acc with the exact delta; returns off of the row
+    off += __shfl_xor(off, 32, 64);
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[d][r] = fmaf(-off, mean[d][r], acc[d][r]);
+    return off;
+}
+// acc += the part of dq / scale that 32 keys have; bit of `word`: the lane's query sees that key (`full`: all of them).
+// EXACT: delta is dout . out with the ROUNDED out, off by e_i; where few keys share a row's weight that outweighs what rounding ds costs (windows of 3 keys in
+// bf16: dq and dk 3.7e-3 off, in norm, of which rounding the results themselves is 1.7e-3).  Then `off` sums ds in 32 bits over the lane's keys, which is
+// -e_i as the p_ij of a row sum to 1, and `mean` the rows p_ij k_j, so that dq = acc - off mean is what the exact delta gives (2.35e-3; a third more products:
+// 4 texts of 2048 x 12 heads, windows of 256: 63 us for the backward pass, 61 without).
+// With KEPT < NF the rest of the lane's dout row lies in LDS, 1 KiB apart.
+template <typename T, int DH, bool EXACT, int KEPT>
+__device__ __forceinline__ void dq_block(const char* kt, const char* vt, const typename Mma<T>::Frag (&qf)[Lay<T, DH>::NF], const typename Mma<T>::Frag (&df)[KEPT],
+                                         const char* parked, float c, float l2, float delta, unsigned word, bool full, f32x16 (&acc)[DH / 32], f32x16 (&mean)[EXACT ? DH / 32 : 1], float& off, int lane) {
     using L = Lay<T, DH>;
     using M = Mma<T>;
     f32x16 st = zero16(), dp = zero16();
 #pragma unroll
     for (int s = 0; s < L::NF; ++s) {
         st = M::mac(row_frag<T, DH>(kt, s, lane), qf[s], st);
-        dp = M::mac(row_frag<T, DH>(vt, s, lane), df[s], dp);
+        dp = M::mac(row_frag<T, DH>(vt, s, lane), s < KEPT ? df[s < KEPT ? s : 0] : *(const typename M::Frag*)(parked + (s - KEPT) * 1024), dp);
     }
+    if constexpr (EXACT) __builtin_amdgcn_sched_barrier(0);
     const unsigned w = word >> (4 * (lane >> 5));
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-        const float p = __builtin_amdgcn_exp2f(fmaf(st[r], c, -l2)) * (dp[r] - delta);
+        const float p = __builtin_amdgcn_exp2f(fmaf(st[r], c, -l2));
         st[r] = full || ((w >> tok(r, 0)) & 1u) ? p : 0.f;
+        dp[r] = st[r] * (dp[r] - delta);
+        if constexpr (EXACT) off += dp[r];
     }
 #pragma unroll
-    for (int d = 0; d < L::ND; ++d) acc[d] = M::mac_t(M::template turned<DH>(kt, d, lane), M::right(st), acc[d]);
+    for (int d = 0; d < L::ND; ++d) {
+        const typename M::Turned t = M::template turned<DH>(kt, d, lane);
+        acc[d] = M::mac_t(t, M::right(dp), acc[d]);
+        if constexpr (EXACT) mean[d] = M::mac_t(t, M::right(st), mean[d]);
+    }
 }
-template <typename T, int DH, int BN, int NW>
-__global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 4>)) void win_bwd_dq_kernel(const WinArgs a) {
+template <typename T, int DH, int BN, int NW, bool EXACT>
+__global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, EXACT ? 3 : 4>)) void win_bwd_dq_kernel(const WinArgs a) {
     using L = Lay<T, DH>;
     using M = Mma<T>;
     constexpr int NB = BN / 32, TILE = L::bytes(BN);
@@ -512,14 +532,17 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 4>)) void win_
     float l2 = a.lse[((long long)n * a.H + h) * a.Tq + ic] * LOG2E;
     if (l2 == -INFINITY || i >= a.Tq) l2 = INFINITY;
     asm volatile("" : "+v"(l2));
-    if (wave_rows) a.stats[stats_at(a, n, h, i0) + lane] = hi ? (i < a.Tq ? delta : 0.f) : l2;
+    if (!EXACT && wave_rows) a.stats[stats_at(a, n, h, i0) + lane] = hi ? (i < a.Tq ? delta : 0.f) : l2;
 
     __shared__ unsigned long long table[2 * MASK_RUN];
     KeyTiles<T, DH, BN, NW> tiles(a, wk, n, hk, smem, table, wave, lane);
     tiles.begin();
-    f32x16 acc[L::ND];
+    f32x16 acc[L::ND], mean[EXACT ? L::ND : 1];
+    float off = 0.f;
 #pragma unroll
     for (int d = 0; d < L::ND; ++d) acc[d] = zero16();
+#pragma unroll
+    for (int d = 0; d < (EXACT ? L::ND : 1); ++d) mean[d] = zero16();
     for (int t = 0; t < wk.nt; ++t) {
         const int j0 = wk.j0(t, BN);
         const char* kt = tiles.step(t);
@@ -532,15 +555,19 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 4>)) void win_
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 if (!full && !__any((unsigned)(bits >> (32 * b)) != 0)) continue;
-                dq_block<T, DH>(kt + L::bytes(32 * b), vt + L::bytes(32 * b), qf, df, a.c, l2, delta, (unsigned)(bits >> (32 * b)), full, acc, lane);
+                dq_block<T, DH, EXACT, L::NF>(kt + L::bytes(32 * b), vt + L::bytes(32 * b), qf, df, nullptr, a.c, l2, delta, (unsigned)(bits >> (32 * b)), full, acc, mean, off, lane);
             }
         }
+    }
+    if constexpr (EXACT) {
+        delta += exactly(acc, mean, off);
+        if (wave_rows) a.stats[stats_at(a, n, h, i0) + lane] = hi ? (i < a.Tq ? delta : 0.f) : l2;
     }
     if (i < a.Tq) store_row<T, DH>(acc, a.scale, (T*)a.dq + n * a.sdq.n + i * a.sdq.t + h * a.sdq.h, hi);
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dk, dv
-// Fragments of a key group's values that stay in LDS instead of registers: at 128 wide bf16 rows the accumulators and both operands take all 256 registers
+// Fragments of a key group's values (in the short kernel below: also of dout's rows) that stay in LDS instead of registers: at 128 wide bf16 rows the accumulators and both operands take all 256 registers
 // that two waves a SIMD leave each, and one that was reloaded from scratch memory in every turn made the turn wait for the next stage's DMA, too.
 template <typename T, int DH> constexpr int PARKED = sizeof(T) == 2 && DH == 128 ? 4 : 0;
 // A workgroup owns kg groups of 32 keys and walks the queries that see them, 32 qh at a time: wave w takes key group w % kg and query rows 32 (w / kg).
@@ -757,14 +784,15 @@ __device__ __forceinline__ void dkv_block(const char* qt, const char* dt, const 
     }
 }
 // One workgroup has a head's queries and keys whole, wave w queries 32 w.. and keys 32 w.., and reads them once: keys and values lie in LDS and the wave's
-// query rows in registers for dq; then they change places, and dk and dv follow without another read.  3072 heads of 130 x 64 in bf16: 160 us for the two
-// kernels' 202; 8 tensors of 51 MB at 2.55 TB/s, where loading them alone would take 90 us: of 130 rows the fifth wave's 30 are padding, and two workgroups of
-// five waves share a CU (bounded to 128 registers, for three, it spilled 23 and took 177 us).
+// query rows in registers for dq; then they change places, and dk and dv follow without another read.  3072 heads of 130 x 64 in bf16: 168 us (160
+// without the exact delta) for the two kernels' 202; 8 tensors of 51 MB at 2.4 TB/s, where moving them alone would take 90 us: of 130 rows the fifth wave's 30
+// are padding, and two workgroups of five waves share a CU (bounded to 128 registers, for three, it spilled 23 and was 17 us slower).
 template <typename T, int DH>
 __global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 3>)) void win_bwd_short_kernel(const WinArgs a) {
     using L = Lay<T, DH>;
     using M = Mma<T>;
     constexpr int TILE = L::bytes(BQ), PK = PARKED<T, DH>;
+    constexpr bool EXACT = sizeof(T) == 2;                                    // (fp32: out's rounding is as small as that of the sums)
     extern __shared__ __attribute__((aligned(16))) char smem[];               // of every wave: two tiles, 64 statistics, parked values
     __shared__ unsigned words[MOST_WAVES<T>];                                 // the keys that exist
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hi = lane >> 5, row = lane & 31, nw = blockDim.x >> 6;
@@ -785,7 +813,7 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 3>)) void win_
     if (lane == 0) words[wave] = valid;
     f32x16 acc[L::ND];
     {
-        typename M::Frag qf[L::NF] = {}, df[L::NF] = {};                      // zeros behind the last query: nothing comes of them below
+        typename M::Frag qf[L::NF] = {}, df[L::NF - PK] = {}, df_rest[PK ? PK : 1] = {};        // zeros behind the last query: nothing comes of them below
         float delta = 0.f, l2 = INFINITY;
         if (i < a.Tq) {
             const char* p = (const char*)((const T*)a.q + n * a.sq.n + i * a.sq.t + h * a.sq.h);
@@ -795,16 +823,24 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 3>)) void win_
 #pragma unroll
             for (int s = 0; s < L::NF; ++s) {
                 qf[s] = *(const typename M::Frag*)(p + 32 * s + 16 * hi);
-                df[s] = *(const typename M::Frag*)(pd + 32 * s + 16 * hi);
-                delta += M::dot(df[s], *(const typename M::Frag*)(po + 32 * s + 16 * hi));
+                const typename M::Frag d = *(const typename M::Frag*)(pd + 32 * s + 16 * hi);
+                delta += M::dot(d, *(const typename M::Frag*)(po + 32 * s + 16 * hi));
+                if (s < L::NF - PK) df[s < L::NF - PK ? s : 0] = d;
+                else df_rest[s < L::NF - PK ? 0 : s - (L::NF - PK)] = d;
             }
         }
+#pragma unroll
+        for (int s = 0; s < PK; ++s) *(typename M::Frag*)(parked + s * 1024) = df_rest[s];
         delta += __shfl_xor(delta, 32, 64);
         if (l2 == -INFINITY) l2 = INFINITY;                                   // the query sees nothing
         dma_barrier();
 #pragma unroll
         for (int d = 0; d < L::ND; ++d) acc[d] = zero16();
+        float off = 0.f;
         if (i0 < a.Tq) {
+            f32x16 mean[EXACT ? L::ND : 1];
+#pragma unroll
+            for (int d = 0; d < (EXACT ? L::ND : 1); ++d) mean[d] = zero16();
             const Span sp = span_of(a, sq.pos + ic, sq.kvl);
             const int in_lo = span_of(a, sq.pos + min(i0 + 31, a.Tq - 1), sq.kvl).lo, in_hi = span_of(a, sq.pos + i0, sq.kvl).hi;
             for (int j0 = 0; j0 < a.Tk; j0 += BQ) {
@@ -813,10 +849,13 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 3>)) void win_
                 const unsigned bits = full ? ~0u : (unsigned)visible(sp, j0) & keys;
                 if (!__any(bits != 0)) continue;
                 const char* kt = smem + j0 / BQ * 2 * TILE;
-                dq_block<T, DH>(kt, kt + TILE, qf, df, a.c, l2, delta, bits, full, acc, lane);
+                dq_block<T, DH, EXACT, L::NF - PK>(kt, kt + TILE, qf, df, parked, a.c, l2, delta, bits, full, acc, mean, off, lane);
             }
+            if constexpr (EXACT) delta += exactly(acc, mean, off);
             if (i < a.Tq) store_row<T, DH>(acc, a.scale, (T*)a.dq + n * a.sdq.n + i * a.sdq.t + h * a.sdq.h, hi);
         }
+#pragma unroll
+        for (int s = 0; s < PK; ++s) df_rest[s] = *(const typename M::Frag*)(parked + s * 1024);
         typename M::Frag kf[L::NF], vf[L::NF - PK];
 #pragma unroll
         for (int s = 0; s < L::NF; ++s) {
@@ -829,7 +868,7 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 3>)) void win_
 #pragma unroll
         for (int s = 0; s < L::NF; ++s) {
             *(typename M::Frag*)(mine + L::row_base(lane) + L::step(s)) = qf[s];
-            *(typename M::Frag*)(mine + TILE + L::row_base(lane) + L::step(s)) = df[s];
+            *(typename M::Frag*)(mine + TILE + L::row_base(lane) + L::step(s)) = s < L::NF - PK ? df[s < L::NF - PK ? s : 0] : df_rest[s < L::NF - PK ? 0 : s - (L::NF - PK)];
         }
         stats[wave * 2 * BQ + lane] = hi ? delta : l2;
         __syncthreads();
@@ -1181,14 +1220,21 @@ template <typename T, int DH> int bwd(const WinArgs& a, hipStream_t st) {
     constexpr int BN = sizeof(T) == 2 ? 64 : 32;
     const int waves = ((a.Tq > a.Tk ? a.Tq : a.Tk) + BQ - 1) / BQ;
     const size_t whole = (size_t)waves * (2 * Lay<T, DH>::bytes(BQ) + 256 + PARKED<T, DH> * 1024);
-    // A head to a workgroup where there is one for every CU (128 wide bf16 rows, 1024 heads of 146: 131 us against 157 in two passes; 32 heads of 224: 33 against
+    // A head to a workgroup where there is one for every CU (128 wide bf16 rows, 1024 heads of 146: 137 us against 157 in two passes; 32 heads of 224: 33 against
     // 28; fp32, 768 heads of 128 x 64: 116 against 142, 24 heads: 39 against 34), and always for rows of 128 bytes, of which a wave holds and multiplies the
-    // least (3072 heads of 130: 160 against 202 us; 12 heads of 146: 15 against 19, of 256: 22.5 against 23).
+    // least (3072 heads of 130: 168 against 202 us; 12 heads of 146: 16 against 19, of 256: 23.5 against 23).
     if (a.G == 1 && a.Tq > 0 && a.Tk > 0 && waves <= MOST_WAVES<T> && whole <= MOST_LDS && ((long long)a.N * a.H >= 256 || Lay<T, DH>::ROWB == 128))
         return launch<win_bwd_short_kernel<T, DH>>((long long)a.N * a.H, 64 * waves, whole, st, a);
-    if (a.Tq > 0)
-        if (int rc = over_keys<T, DH, BN>(a, [&](auto nw, int waves, long long blocks, size_t lds) { return launch<win_bwd_dq_kernel<T, DH, BN, decltype(nw)::value>>(blocks, 64 * waves, lds, st, a); }))
-            return rc;
+    if (a.Tq > 0) {
+        const auto dq = [&](auto exact) {
+            return over_keys<T, DH, BN>(a, [&](auto nw, int waves, long long blocks, size_t lds) {
+                return launch<win_bwd_dq_kernel<T, DH, BN, decltype(nw)::value, decltype(exact)::value>>(blocks, 64 * waves, lds, st, a);
+            });
+        };
+        // dq from the exact delta where few keys share a row's weight, and out is rounded to 16 bits: beyond 256 keys the difference is a tenth of the rounding
+        const int rc = sizeof(T) == 2 && span_keys(a) <= 256 ? dq(std::integral_constant<bool, sizeof(T) == 2>()) : dq(std::false_type());
+        if (rc) return rc;
+    }
     if (a.Tk == 0) return 0;
     if (a.sink_keys > 0)
         if (int rc = launch<win_bwd_dkv_kernel<T, DH, true>>((long long)a.N * a.Hkv * (a.sink_rows / BQ) * a.chunks, 64 * ROW_GROUPS<T, DH>,
