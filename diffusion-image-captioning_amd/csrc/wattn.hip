@@ -452,6 +452,11 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (DH == 128 && BN == 32 && sizeo
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dq (and delta)
+// Rows that see at most FEW_KEYS keys get the exact delta (dq_block): those of narrow windows and the first ones of a causal text, whose gradients are the
+// largest.  Beyond that it changes less than a tenth of the rounding errors, and costs a third more products.  Carrying both forms costs the plain one its best
+// schedule: 139 us for 130 (2 x 4096 rows, 16 heads of 128, windows of 1024), where a branch inside of one loop took 153.
+template <typename T> constexpr bool BF16 = sizeof(T) == 2;
+constexpr int FEW_KEYS = 256;
 template <int ND> __device__ __forceinline__ float exactly(f32x16 (&acc)[ND], const f32x16 (&mean)[ND], float off) {        // acc with the exact delta; returns off of the row
     off += __shfl_xor(off, 32, 64);
 #pragma unroll
@@ -461,7 +466,7 @@ template <int ND> __device__ __forceinline__ float exactly(f32x16 (&acc)[ND], co
     return off;
 }
 // acc += the part of dq / scale that 32 keys have; bit of `word`: the lane's query sees that key (`full`: all of them).
-// EXACT: delta is dout . out with the ROUNDED out, off by e_i; where few keys share a row's weight that outweighs what rounding ds costs (windows of 3 keys in
+// EXACT (bf16): delta is dout . out with the ROUNDED out, off by e_i; where few keys share a row's weight that outweighs what rounding ds costs (windows of 3 keys in
 // bf16: dq and dk 3.7e-3 off, in norm, of which rounding the results themselves is 1.7e-3).  Then `off` sums ds in 32 bits over the lane's keys, which is
 // -e_i as the p_ij of a row sum to 1, and `mean` the rows p_ij k_j, so that dq = acc - off mean is what the exact delta gives (2.35e-3; a third more products:
 // 4 texts of 2048 x 12 heads, windows of 256: 63 us for the backward pass, 61 without).
@@ -493,19 +498,13 @@ __device__ __forceinline__ void dq_block(const char* kt, const char* vt, const t
         if constexpr (EXACT) mean[d] = M::mac_t(t, M::right(st), mean[d]);
     }
 }
+// the rows of one workgroup: query tile qt of query head h, key head hk, sequence n
 template <typename T, int DH, int BN, int NW, bool EXACT>
-__global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, EXACT ? 3 : 4>)) void win_bwd_dq_kernel(const WinArgs a) {
+__device__ __forceinline__ void dq_rows(const WinArgs& a, int n, int hk, int h, int qt, const Seq& sq, char* smem, unsigned long long* table) {
     using L = Lay<T, DH>;
     using M = Mma<T>;
     constexpr int NB = BN / 32, TILE = L::bytes(BN);
-    extern __shared__ __attribute__((aligned(16))) char smem[];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hi = lane >> 5;
-    const int nw = NW ? NW : blockDim.x >> 6, bm = nw * BQ, nqt = (a.Tq + bm - 1) / bm;
-    int item = xcd_item();
-    const int g = item % a.G; item /= a.G;
-    const int qt = nqt - 1 - item % nqt; item /= nqt;
-    const int hk = item % a.Hkv, n = item / a.Hkv, h = hk * a.G + g;
-    const Seq sq = sequence(a, n);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hi = lane >> 5, bm = (NW ? NW : blockDim.x >> 6) * BQ;
     const int i0 = qt * bm + wave * BQ, i = i0 + (lane & 31), ic = min(i, a.Tq - 1);
     const Walk wk = walk_of(a, sq.pos + qt * bm, sq.pos + min(qt * bm + bm, a.Tq) - 1, sq, BN);
     const Span sp = span_of(a, sq.pos + ic, sq.kvl);
@@ -532,9 +531,7 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, EXACT ? 3 : 4>
     float l2 = a.lse[((long long)n * a.H + h) * a.Tq + ic] * LOG2E;
     if (l2 == -INFINITY || i >= a.Tq) l2 = INFINITY;
     asm volatile("" : "+v"(l2));
-    if (!EXACT && wave_rows) a.stats[stats_at(a, n, h, i0) + lane] = hi ? (i < a.Tq ? delta : 0.f) : l2;
 
-    __shared__ unsigned long long table[2 * MASK_RUN];
     KeyTiles<T, DH, BN, NW> tiles(a, wk, n, hk, smem, table, wave, lane);
     tiles.begin();
     f32x16 acc[L::ND], mean[EXACT ? L::ND : 1];
@@ -559,11 +556,23 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, EXACT ? 3 : 4>
             }
         }
     }
-    if constexpr (EXACT) {
-        delta += exactly(acc, mean, off);
-        if (wave_rows) a.stats[stats_at(a, n, h, i0) + lane] = hi ? (i < a.Tq ? delta : 0.f) : l2;
-    }
+    if constexpr (EXACT) delta += exactly(acc, mean, off);
+    if (wave_rows) a.stats[stats_at(a, n, h, i0) + lane] = hi ? (i < a.Tq ? delta : 0.f) : l2;
     if (i < a.Tq) store_row<T, DH>(acc, a.scale, (T*)a.dq + n * a.sdq.n + i * a.sdq.t + h * a.sdq.h, hi);
+}
+template <typename T, int DH, int BN, int NW>
+__global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 3>)) void win_bwd_dq_kernel(const WinArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    __shared__ unsigned long long table[2 * MASK_RUN];
+    const int bm = (NW ? NW : blockDim.x >> 6) * BQ, nqt = (a.Tq + bm - 1) / bm;
+    int item = xcd_item();
+    const int g = item % a.G; item /= a.G;
+    const int qt = nqt - 1 - item % nqt; item /= nqt;
+    const int hk = item % a.Hkv, n = item / a.Hkv, h = hk * a.G + g;
+    const Seq sq = sequence(a, n);
+    const Span s0 = span_of(a, sq.pos + qt * bm, sq.kvl), s1 = span_of(a, sq.pos + min(qt * bm + bm, a.Tq) - 1, sq.kvl);
+    if (BF16<T> && min(s0.hi - s0.lo + s0.sk, s1.hi - s1.lo + s1.sk) <= FEW_KEYS) dq_rows<T, DH, BN, NW, BF16<T>>(a, n, hk, h, qt, sq, smem, table);
+    else dq_rows<T, DH, BN, NW, false>(a, n, hk, h, qt, sq, smem, table);
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dk, dv
@@ -792,7 +801,6 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 3>)) void win_
     using L = Lay<T, DH>;
     using M = Mma<T>;
     constexpr int TILE = L::bytes(BQ), PK = PARKED<T, DH>;
-    constexpr bool EXACT = sizeof(T) == 2;                                    // (fp32: out's rounding is as small as that of the sums)
     extern __shared__ __attribute__((aligned(16))) char smem[];               // of every wave: two tiles, 64 statistics, parked values
     __shared__ unsigned words[MOST_WAVES<T>];                                 // the keys that exist
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hi = lane >> 5, row = lane & 31, nw = blockDim.x >> 6;
@@ -838,9 +846,9 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 3>)) void win_
         for (int d = 0; d < L::ND; ++d) acc[d] = zero16();
         float off = 0.f;
         if (i0 < a.Tq) {
-            f32x16 mean[EXACT ? L::ND : 1];
+            f32x16 mean[BF16<T> ? L::ND : 1];
 #pragma unroll
-            for (int d = 0; d < (EXACT ? L::ND : 1); ++d) mean[d] = zero16();
+            for (int d = 0; d < (BF16<T> ? L::ND : 1); ++d) mean[d] = zero16();
             const Span sp = span_of(a, sq.pos + ic, sq.kvl);
             const int in_lo = span_of(a, sq.pos + min(i0 + 31, a.Tq - 1), sq.kvl).lo, in_hi = span_of(a, sq.pos + i0, sq.kvl).hi;
             for (int j0 = 0; j0 < a.Tk; j0 += BQ) {
@@ -849,9 +857,9 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 3>)) void win_
                 const unsigned bits = full ? ~0u : (unsigned)visible(sp, j0) & keys;
                 if (!__any(bits != 0)) continue;
                 const char* kt = smem + j0 / BQ * 2 * TILE;
-                dq_block<T, DH, EXACT, L::NF - PK>(kt, kt + TILE, qf, df, parked, a.c, l2, delta, bits, full, acc, mean, off, lane);
+                dq_block<T, DH, BF16<T>, L::NF - PK>(kt, kt + TILE, qf, df, parked, a.c, l2, delta, bits, full, acc, mean, off, lane);
             }
-            if constexpr (EXACT) delta += exactly(acc, mean, off);
+            if constexpr (BF16<T>) delta += exactly(acc, mean, off);
             if (i < a.Tq) store_row<T, DH>(acc, a.scale, (T*)a.dq + n * a.sdq.n + i * a.sdq.t + h * a.sdq.h, hi);
         }
 #pragma unroll
@@ -1225,16 +1233,9 @@ template <typename T, int DH> int bwd(const WinArgs& a, hipStream_t st) {
     // least (3072 heads of 130: 168 against 202 us; 12 heads of 146: 16 against 19, of 256: 23.5 against 23).
     if (a.G == 1 && a.Tq > 0 && a.Tk > 0 && waves <= MOST_WAVES<T> && whole <= MOST_LDS && ((long long)a.N * a.H >= 256 || Lay<T, DH>::ROWB == 128))
         return launch<win_bwd_short_kernel<T, DH>>((long long)a.N * a.H, 64 * waves, whole, st, a);
-    if (a.Tq > 0) {
-        const auto dq = [&](auto exact) {
-            return over_keys<T, DH, BN>(a, [&](auto nw, int waves, long long blocks, size_t lds) {
-                return launch<win_bwd_dq_kernel<T, DH, BN, decltype(nw)::value, decltype(exact)::value>>(blocks, 64 * waves, lds, st, a);
-            });
-        };
-        // dq from the exact delta where few keys share a row's weight, and out is rounded to 16 bits: beyond 256 keys the difference is a tenth of the rounding
-        const int rc = sizeof(T) == 2 && span_keys(a) <= 256 ? dq(std::integral_constant<bool, sizeof(T) == 2>()) : dq(std::false_type());
-        if (rc) return rc;
-    }
+    if (a.Tq > 0)
+        if (int rc = over_keys<T, DH, BN>(a, [&](auto nw, int waves, long long blocks, size_t lds) { return launch<win_bwd_dq_kernel<T, DH, BN, decltype(nw)::value>>(blocks, 64 * waves, lds, st, a); }))
+            return rc;
     if (a.Tk == 0) return 0;
     if (a.sink_keys > 0)
         if (int rc = launch<win_bwd_dkv_kernel<T, DH, true>>((long long)a.N * a.Hkv * (a.sink_rows / BQ) * a.chunks, 64 * ROW_GROUPS<T, DH>,
