@@ -197,18 +197,19 @@ class NormParams(NamedTuple):
     eps: float = 1e-12
 
 
+_WEIGHT, _BIAS = {"post": "post weight", "pre": "pre weight"}, {"post": "post bias", "pre": "pre bias"}
+
+
 def _norm(norm, like, D, side):
     """The packed fields of one norm."""
     if norm is None:
         return 0, 0, 0, 0.0
     if norm.kind not in _KINDS:
         raise ValueError(f'{side}: a norm is "layer" or "rms"')
-    for t, name in ((norm.weight, "weight"), (norm.bias, "bias")):
+    for t, name in ((norm.weight, _WEIGHT[side]), (norm.bias, _BIAS[side])):
         if t is not None:
-            _on(t, like, f"{side} {name}", (torch.float32,), (D,))
-            if not t.is_contiguous():
-                raise ValueError(f"{side} {name} must be contiguous")
-    return _ptr(norm.weight), _ptr(norm.bias), _KINDS[norm.kind], float(norm.eps)
+            _packed(t, like, name, torch.float32, (D,))
+    return _ptr(norm.weight), _ptr(norm.bias), _KINDS[norm.kind], norm.eps
 
 
 def _shapes(x, gate):
@@ -228,10 +229,14 @@ def _shapes(x, gate):
     return rows, D, max(rows // max(n, 1), 1)
 
 
-def _packed(t, like, name, dtype):
-    _on(t, like, name, (dtype,), like.shape)
-    if not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous")
+def _packed(t, like, name, dtype, shape):
+    try:                                                             # (the whole check in one expression: a call on one caption's rows is all host time)
+        if t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.get_device() == like.get_device() and not (t.requires_grad and torch.is_grad_enabled()):
+            return
+    except AttributeError:
+        pass
+    _on(t, like, name, (dtype,), shape)
+    raise ValueError(f"{name} must be contiguous")
 
 
 def _norm_code(stream, inner):
@@ -250,9 +255,9 @@ def gated_norm(x, y=None, *, post=None, gate=None, residual_scale=1.0, pre=None,
     _first(x, "x")
     inner = y.dtype if isinstance(y, torch.Tensor) else (dtype or x.dtype)
     code = _norm_code(x.dtype, inner)
-    _packed(x, x, "x", x.dtype)
+    _packed(x, x, "x", x.dtype, x.shape)
     if y is not None:
-        _packed(y, x, "y", inner)
+        _packed(y, x, "y", inner, x.shape)
         if not (dtype in (None, inner)):
             raise ValueError("dtype is the type of a without y")
     else:
@@ -275,25 +280,24 @@ def gated_norm_grad(dx_new, da, x_new, y, saved, *, post=None, gate=None, residu
     given = y if y is not None else da
     inner = given.dtype if isinstance(given, torch.Tensor) else x_new.dtype
     code = _norm_code(x_new.dtype, inner)
-    _packed(x_new, x_new, "x_new", x_new.dtype)
+    shape = x_new.shape
+    _packed(x_new, x_new, "x_new", x_new.dtype, shape)
     if not ((da is None) == (pre is None)):
         raise ValueError("da is the gradient of pre's output: both or neither")
     if not (dx_new is not None or da is not None):
         raise ValueError("neither output has a gradient")
     if dx_new is not None:
-        _packed(dx_new, x_new, "dx_new", x_new.dtype)
+        _packed(dx_new, x_new, "dx_new", x_new.dtype, shape)
     if da is not None:
-        _packed(da, x_new, "da", inner)
+        _packed(da, x_new, "da", inner, shape)
     if y is not None:
-        _packed(y, x_new, "y", inner)
+        _packed(y, x_new, "y", inner, shape)
     else:
         if not (post is None and gate is None and pre is not None):
             raise ValueError("without y there is a pre norm and nothing else")
     rows, D, per_gate = _shapes(x_new, gate)
     sides = *_norm(post, x_new, D, "post"), *_norm(pre, x_new, D, "pre")
-    _on(saved, x_new, "saved", (torch.float32,), (4, rows))
-    if not saved.is_contiguous():
-        raise ValueError("saved must be contiguous")
+    _packed(saved, x_new, "saved", torch.float32, (4, rows))
     got = {"dx": torch.empty_like(x_new)}
     if y is not None:
         got["dy"] = torch.empty_like(y)
