@@ -374,6 +374,8 @@ NORMS = [
     (2, 65, 1003, "sequence", "layer", "layer", True), (2, 6, 1024, "shared", "rms", "layer", True), (3, 50, 1500, "sequence", "layer", "layer", True), (1, 3, 2048, "shared", "layer", "layer", True),
     (2, 40, 4095, "sequence", "rms", "layer", True), (2, 3, 4096, None, "layer", "layer", True), (2, 30, 8191, "sequence", "layer", "rms", True), (1, 1300, 8192, "shared", "layer", "layer", False),
     (3000, 1, 96, "sequence", "layer", "layer", True), (1, 20000, 40, "shared", "layer", "rms", True), (9, 1111, 120, "sequence", "rms", "layer", True),
+    (1100, 3, 200, "sequence", "layer", "layer", True), (700, 2, 770, "sequence", "layer", "rms", True), (520, 3, 1500, "sequence", "rms", "layer", True), (300, 2, 2500, "sequence", "layer", "layer", True),
+    (260, 1, 5000, "sequence", "rms", "rms", True),
 ]
 TYPES = [(F32, F32), (BF16, BF16), (F32, BF16)]
 
