@@ -281,8 +281,8 @@ __device__ __forceinline__ int xcd_item() {
 __device__ __forceinline__ int mask_byte(const WinArgs& a, int n, int j) { return a.key_mask && j >= 0 && j < a.Tk ? a.key_mask[(size_t)n * a.Tk + j] : 1; }
 
 template <typename T> constexpr int MOST_WAVES = sizeof(T) == 2 ? 8 : 4;      // of a workgroup: fp32 operands need more than half of a SIMD's registers
-// waves that a SIMD is to hold at once: what the registers of bf16 rows of 64 allow, 2 for rows of 128, 1 for fp32
-template <typename T, int DH, int MOST> constexpr int RESIDENT = sizeof(T) == 4 ? 1 : DH == 64 ? MOST : 2;
+// waves that a SIMD is to hold at once: what the registers of bf16 rows of 64 allow, 2 for rows of 256 bytes, 1 for rows of 512
+template <typename T, int DH, int MOST> constexpr int RESIDENT = sizeof(T) * DH > 256 ? 1 : sizeof(T) * DH == 256 ? 2 : MOST;
 constexpr int BQ = 32;                          // queries (or keys) per wave, and rows of a statistics tile
 __host__ __device__ __forceinline__ long long stats_floats(long long N, long long H, long long Tq) { return N * H * ((Tq + BQ - 1) / BQ) * 2 * BQ; }
 __device__ __forceinline__ long long stats_at(const WinArgs& a, int n, int h, int i0) { return stats_floats(1, (long long)n * a.H + h, a.Tq) + 2 * i0; }
@@ -1121,7 +1121,9 @@ Shape shape_of(const WinArgs& a, int waves, int most, int most_rows) {
     while (kg > 1 && heads * ((tiles + kg - 1) / kg) < 2048 / waves && waves / kg < most_rows) kg >>= 1;
     return {kg, waves / kg};
 }
-template <typename T, int DH> constexpr int ROW_GROUPS = Lay<T, DH>::ROWB <= 256 ? 4 : 2;       // at most: two stages of 512-byte rows fill 132 KB of LDS with 2
+// Row groups at most: with 2, the stages of fp32 rows of 256 bytes let two workgroups share a CU (4 x 513 rows, 12 heads: 75 us, with 4 87), and those of 512
+// bytes fit at all.
+template <typename T, int DH> constexpr int ROW_GROUPS = sizeof(T) == 2 ? 4 : 2;
 // Pieces of the sink pass: about 256 workgroups, and no more than 16 partial sums for the window pass to add.
 void plan_sinks(WinArgs& a) {
     a.near_sinks = a.left >= 0 ? (a.sinks < a.Tk ? a.sinks : a.Tk) : 0;
