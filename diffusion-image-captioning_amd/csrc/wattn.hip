@@ -287,12 +287,13 @@ constexpr int BQ = 32;                          // queries (or keys) per wave, a
 __host__ __device__ __forceinline__ long long stats_floats(long long N, long long H, long long Tq) { return N * H * ((Tq + BQ - 1) / BQ) * 2 * BQ; }
 __device__ __forceinline__ long long stats_at(const WinArgs& a, int n, int h, int i0) { return stats_floats(1, (long long)n * a.H + h, a.Tq) + 2 * i0; }
 
-// The key and value tiles of a workgroup's walk in LDS.  NW > 0: two of them, and that many waves fetch the next one behind the barrier in front of a tile.
+// The key and value tiles of a workgroup's walk in LDS.  NW > 0: two turns of KS tiles, and that many waves fetch the next turn behind the barrier in front of
+// one.  KS = 2: the first half of the waves takes the even tiles, the second the odd ones, for the same rows; they add up their results at the end.
 // NW = 0: the walk has at most FEW_TILES, and whatever waves there are fetch all of them at the start.
 constexpr int FEW_TILES = 4, MASK_RUN = 256;
-template <typename T, int DH, int BN, int NW> struct KeyTiles {
+template <typename T, int DH, int BN, int NW, int KS> struct KeyTiles {
     using L = Lay<T, DH>;
-    static constexpr int TILE = L::bytes(BN), SLOTS = NW ? 2 : FEW_TILES;
+    static constexpr int TILE = L::bytes(BN), SLOTS = NW ? 2 * KS : FEW_TILES;
     const WinArgs& a;
     const Walk wk;
     const char *kb, *vb, *smem;
@@ -328,37 +329,42 @@ template <typename T, int DH, int BN, int NW> struct KeyTiles {
     }
     __device__ __forceinline__ void begin() {
         if (a.key_mask) { read_masks(0); __syncthreads(); }
-        for (int t = 0; t < min(wk.nt, NW ? 1 : FEW_TILES); ++t) issue(t);
+        for (int t = 0; t < min(wk.nt, NW ? KS : FEW_TILES); ++t) issue(t);
         if constexpr (NW == 0) dma_barrier();
     }
-    // tile t is in LDS behind this call, its keys at the address returned and its values TILE bytes further on
-    __device__ __forceinline__ const char* step(int t) {
+    // the turn's tiles t .. t + KS - 1, as far as there are, are in LDS behind this call
+    __device__ __forceinline__ void step(int t) {
         if constexpr (NW > 0) {
             dma_barrier();
-            if (t + 1 < wk.nt) {
-                if (a.key_mask && ((t + 1) & (MASK_RUN - 1)) == 0) { read_masks(t + 1); __syncthreads(); }
-                issue(t + 1);
+            if (t + KS < wk.nt) {
+                if (a.key_mask && ((t + KS) & (MASK_RUN - 1)) == 0) { read_masks(t + KS); __syncthreads(); }
+#pragma unroll
+                for (int k = 0; k < KS; ++k)
+                    if (k == 0 || t + KS + k < wk.nt) issue(t + KS + k);
             }
         }
-        return smem + (t & (SLOTS - 1)) * 2 * TILE;
     }
+    // the keys of tile t; its values lie TILE bytes further on
+    __device__ __forceinline__ const char* at(int t) const { return smem + (t & (SLOTS - 1)) * 2 * TILE; }
 };
 
 // ------------------------------------------------------------------------------------------------ forward
-template <typename T, int DH, int BN, int NW>
+template <typename T, int DH, int BN, int NW, int KS>
 __global__ __launch_bounds__(64 * MOST_WAVES<T>, (DH == 128 && BN == 32 && sizeof(T) == 2 ? 3 : RESIDENT<T, DH, 4>)) void win_fwd_kernel(const WinArgs a) {
     using L = Lay<T, DH>;
     using M = Mma<T>;
     constexpr int NB = BN / 32, TILE = L::bytes(BN);
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hi = lane >> 5;
-    const int nw = NW ? NW : blockDim.x >> 6, bm = nw * BQ, nqt = (a.Tq + bm - 1) / bm;
+    constexpr int ROWS = NW / KS;                             // waves with rows of their own, or 0: all
+    const int row_wave = KS > 1 ? wave % ROWS : wave, half = KS > 1 ? wave / ROWS : 0;
+    const int bm = (NW ? ROWS : blockDim.x >> 6) * BQ, nqt = (a.Tq + bm - 1) / bm;
     int item = xcd_item();
     const int g = item % a.G; item /= a.G;
     const int qt = nqt - 1 - item % nqt; item /= nqt;         // long rows first
     const int hk = item % a.Hkv, n = item / a.Hkv, h = hk * a.G + g;
     const Seq sq = sequence(a, n);
-    const int i0 = qt * bm + wave * BQ, i = i0 + (lane & 31), ic = min(i, a.Tq - 1);
+    const int i0 = qt * bm + row_wave * BQ, i = i0 + (lane & 31), ic = min(i, a.Tq - 1);
     const Walk wk = walk_of(a, sq.pos + qt * bm, sq.pos + min(qt * bm + bm, a.Tq) - 1, sq, BN);
     const Span sp = span_of(a, sq.pos + ic, sq.kvl);
     const bool wave_rows = i0 < a.Tq;
@@ -373,7 +379,7 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (DH == 128 && BN == 32 && sizeo
         landed(qf);
     }
     __shared__ unsigned long long table[2 * MASK_RUN];
-    KeyTiles<T, DH, BN, NW> tiles(a, wk, n, hk, smem, table, wave, lane);
+    KeyTiles<T, DH, BN, NW, KS> tiles(a, wk, n, hk, smem, table, wave, lane);
     tiles.begin();
 
     f32x16 acc[L::ND];
@@ -426,9 +432,12 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (DH == 128 && BN == 32 && sizeo
             for (int d = 0; d < L::ND; ++d) acc[d] = M::mac_t(M::template turned<DH>(vt + L::bytes(32 * b), d, lane), M::right(st[b]), acc[d]);
         }
     };
-    for (int t = 0; t < wk.nt; ++t) {
+    for (int t0 = 0; t0 < wk.nt; t0 += KS) {
+        tiles.step(t0);
+        const int t = t0 + half;
+        if (KS > 1 && t >= wk.nt) break;                      // (the last turn)
         const int j0 = wk.j0(t, BN);
-        const char* kt = tiles.step(t);
+        const char* kt = tiles.at(t);
         const char* vt = kt + TILE;
         const unsigned long long valid = tiles.valid(t);
         unsigned long long bits = ~0ull;
@@ -443,6 +452,28 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (DH == 128 && BN == 32 && sizeo
                 else blocks(std::integral_constant<int, 1>(), first ? 0 : 1, kt, vt, bits, full);
             }
         }
+    }
+    if constexpr (KS > 1) {
+        float* const to = (float*)smem + row_wave * (L::ND * 16 + 2) * 64 + lane;
+        __syncthreads();                                      // the tiles are done with
+        if (half) {
+#pragma unroll
+            for (int d = 0; d < L::ND; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) to[(d * 16 + r) * 64] = acc[d][r];
+            to[L::ND * 16 * 64] = m;
+            to[(L::ND * 16 + 1) * 64] = l;
+        }
+        __syncthreads();
+        if (half) return;
+        const float m1 = to[L::ND * 16 * 64], mn = fmaxf(m, m1), mm = mn == -INFINITY ? 0.f : mn;
+        const float f0 = __builtin_amdgcn_exp2f(m - mm), f1 = __builtin_amdgcn_exp2f(m1 - mm);
+        m = mn;
+        l = l * f0 + to[(L::ND * 16 + 1) * 64] * f1;
+#pragma unroll
+        for (int d = 0; d < L::ND; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[d][r] = acc[d][r] * f0 + to[(d * 16 + r) * 64] * f1;
     }
     l += __shfl_xor(l, 32, 64);
     if (i < a.Tq) {
@@ -499,13 +530,15 @@ __device__ __forceinline__ void dq_block(const char* kt, const char* vt, const t
     }
 }
 // the rows of one workgroup: query tile qt of query head h, key head hk, sequence n
-template <typename T, int DH, int BN, int NW, bool EXACT>
+template <typename T, int DH, int BN, int NW, int KS, bool EXACT>
 __device__ __forceinline__ void dq_rows(const WinArgs& a, int n, int hk, int h, int qt, const Seq& sq, char* smem, unsigned long long* table) {
     using L = Lay<T, DH>;
     using M = Mma<T>;
     constexpr int NB = BN / 32, TILE = L::bytes(BN);
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hi = lane >> 5, bm = (NW ? NW : blockDim.x >> 6) * BQ;
-    const int i0 = qt * bm + wave * BQ, i = i0 + (lane & 31), ic = min(i, a.Tq - 1);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hi = lane >> 5;
+    constexpr int ROWS = NW / KS;
+    const int row_wave = KS > 1 ? wave % ROWS : wave, half = KS > 1 ? wave / ROWS : 0, bm = (NW ? ROWS : blockDim.x >> 6) * BQ;
+    const int i0 = qt * bm + row_wave * BQ, i = i0 + (lane & 31), ic = min(i, a.Tq - 1);
     const Walk wk = walk_of(a, sq.pos + qt * bm, sq.pos + min(qt * bm + bm, a.Tq) - 1, sq, BN);
     const Span sp = span_of(a, sq.pos + ic, sq.kvl);
     const bool wave_rows = i0 < a.Tq;
@@ -532,7 +565,7 @@ __device__ __forceinline__ void dq_rows(const WinArgs& a, int n, int hk, int h, 
     if (l2 == -INFINITY || i >= a.Tq) l2 = INFINITY;
     asm volatile("" : "+v"(l2));
 
-    KeyTiles<T, DH, BN, NW> tiles(a, wk, n, hk, smem, table, wave, lane);
+    KeyTiles<T, DH, BN, NW, KS> tiles(a, wk, n, hk, smem, table, wave, lane);
     tiles.begin();
     f32x16 acc[L::ND], mean[EXACT ? L::ND : 1];
     float off = 0.f;
@@ -540,9 +573,12 @@ __device__ __forceinline__ void dq_rows(const WinArgs& a, int n, int hk, int h, 
     for (int d = 0; d < L::ND; ++d) acc[d] = zero16();
 #pragma unroll
     for (int d = 0; d < (EXACT ? L::ND : 1); ++d) mean[d] = zero16();
-    for (int t = 0; t < wk.nt; ++t) {
+    for (int t0 = 0; t0 < wk.nt; t0 += KS) {
+        tiles.step(t0);
+        const int t = t0 + half;
+        if (KS > 1 && t >= wk.nt) break;                      // (the last turn)
         const int j0 = wk.j0(t, BN);
-        const char* kt = tiles.step(t);
+        const char* kt = tiles.at(t);
         const char* vt = kt + TILE;
         const unsigned long long valid = tiles.valid(t);
         unsigned long long bits = ~0ull;
@@ -556,23 +592,49 @@ __device__ __forceinline__ void dq_rows(const WinArgs& a, int n, int hk, int h, 
             }
         }
     }
+    if constexpr (KS > 1) {                                   // the halves' sums, one accumulator at a time
+        float* const to = (float*)smem + row_wave * L::ND * 16 * 64 + lane;
+        auto add = [&](auto& sums, int n) {
+            __syncthreads();
+            if (half)
+#pragma unroll
+                for (int d = 0; d < n; ++d)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) to[(d * 16 + r) * 64] = sums[d][r];
+            __syncthreads();
+            if (!half)
+#pragma unroll
+                for (int d = 0; d < n; ++d)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) sums[d][r] += to[(d * 16 + r) * 64];
+        };
+        add(acc, L::ND);
+        if constexpr (EXACT) {
+            add(mean, L::ND);
+            __syncthreads();
+            if (half) *to = off;
+            __syncthreads();
+            if (!half) off += *to;
+        }
+        if (half) return;
+    }
     if constexpr (EXACT) delta += exactly(acc, mean, off);
     if (wave_rows) a.stats[stats_at(a, n, h, i0) + lane] = hi ? (i < a.Tq ? delta : 0.f) : l2;
     if (i < a.Tq) store_row<T, DH>(acc, a.scale, (T*)a.dq + n * a.sdq.n + i * a.sdq.t + h * a.sdq.h, hi);
 }
-template <typename T, int DH, int BN, int NW>
+template <typename T, int DH, int BN, int NW, int KS>
 __global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 3>)) void win_bwd_dq_kernel(const WinArgs a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     __shared__ unsigned long long table[2 * MASK_RUN];
-    const int bm = (NW ? NW : blockDim.x >> 6) * BQ, nqt = (a.Tq + bm - 1) / bm;
+    const int bm = (NW ? NW / KS : blockDim.x >> 6) * BQ, nqt = (a.Tq + bm - 1) / bm;
     int item = xcd_item();
     const int g = item % a.G; item /= a.G;
     const int qt = nqt - 1 - item % nqt; item /= nqt;
     const int hk = item % a.Hkv, n = item / a.Hkv, h = hk * a.G + g;
     const Seq sq = sequence(a, n);
     const Span s0 = span_of(a, sq.pos + qt * bm, sq.kvl), s1 = span_of(a, sq.pos + min(qt * bm + bm, a.Tq) - 1, sq.kvl);
-    if (BF16<T> && min(s0.hi - s0.lo + s0.sk, s1.hi - s1.lo + s1.sk) <= FEW_KEYS) dq_rows<T, DH, BN, NW, BF16<T>>(a, n, hk, h, qt, sq, smem, table);
-    else dq_rows<T, DH, BN, NW, false>(a, n, hk, h, qt, sq, smem, table);
+    if (BF16<T> && min(s0.hi - s0.lo + s0.sk, s1.hi - s1.lo + s1.sk) <= FEW_KEYS) dq_rows<T, DH, BN, NW, KS, BF16<T>>(a, n, hk, h, qt, sq, smem, table);
+    else dq_rows<T, DH, BN, NW, KS, false>(a, n, hk, h, qt, sq, smem, table);
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dk, dv
@@ -1193,6 +1255,10 @@ template <auto KERNEL, typename... More> int launch(long long blocks, int thread
     DIC_CHECK_LAUNCH();
     return 0;
 }
+// With that few workgroups of 128 rows (a CU has one at most, a SIMD one wave) a workgroup takes 64 rows instead, and its wave pairs share the keys of 32: one
+// text of 4096 rows read from left to right, 8 heads of 128, forward: 72 us for 142, backward 240 for 292; 4 x 513 rows in windows of 257, 12 heads, fp32: 30
+// for 37 and 96 for 104.  With 512 workgroups, 128 wide, it fills the LDS of a CU by itself: 54 us for 33 (2 x 2048 rows, windows of 501, 16 heads).
+constexpr long long SPLIT = 256;
 constexpr size_t SHARED_CU_LDS = 75 << 10;                       // two workgroups fit a CU's 160 KB
 // The workgroups of a kernel that walks the keys.  Few keys: all of them in LDS at once (unless that keeps a second workgroup off the CU) and the query rows
 // of a sequence in one workgroup where they fit (130 rows x 130 keys x 3072 heads, forward: 5 waves 86 us, 4 waves and a second workgroup 113 us).
@@ -1202,9 +1268,14 @@ template <typename T, int DH, int BN, typename F> int over_keys(const WinArgs& a
     const size_t all = (size_t)tiles * 2 * Lay<T, DH>::bytes(BN);
     const bool few = tiles <= FEW_TILES && all <= SHARED_CU_LDS;
     const int waves = few && rows <= MOST ? rows : 4;
-    const long long blocks = (long long)a.N * a.H * ((rows + waves - 1) / waves);
-    if (few) return go(std::integral_constant<int, 0>(), waves, blocks, all);
-    return go(std::integral_constant<int, 4>(), waves, blocks, (size_t)4 * Lay<T, DH>::bytes(BN));
+    const long long heads = (long long)a.N * a.H, blocks = heads * ((rows + waves - 1) / waves);
+    constexpr std::integral_constant<int, 1> one;
+    constexpr std::integral_constant<int, 2> two;
+    if (few) return go(std::integral_constant<int, 0>(), one, waves, blocks, all);
+    constexpr std::integral_constant<int, 4> four;
+    const size_t turns = (size_t)4 * Lay<T, DH>::bytes(BN), sums = (size_t)2 * (DH / 2 + 2) * 256;
+    if (blocks <= SPLIT) return go(four, two, 4, heads * ((rows + 1) / 2), 2 * turns > sums ? 2 * turns : sums);
+    return go(four, one, 4, blocks, turns);
 }
 template <typename T, int DH> int fwd(const WinArgs& a, hipStream_t st) {
     constexpr int BN = sizeof(T) == 2 ? 64 : 32;
@@ -1216,10 +1287,10 @@ template <typename T, int DH> int fwd(const WinArgs& a, hipStream_t st) {
     // 128 wide rows that see many keys: tiles of 32, which take the registers and LDS of three workgroups a CU instead of two (one text of 8192 rows, 4096 keys
     // each, 16 heads: 249 us against 277; rows of 1024 keys, 2 x 4096 rows: 104 us against 96)
     if constexpr (sizeof(T) == 2 && DH == 128)
-        if (span_keys(a) >= 2048)
-            return launch<win_fwd_kernel<T, DH, 32, 4>>((long long)a.N * a.H * ((a.Tq + 4 * BQ - 1) / (4 * BQ)), 256, 
+        if (span_keys(a) >= 2048 && (long long)a.N * a.H * ((a.Tq + 4 * BQ - 1) / (4 * BQ)) > SPLIT)
+            return launch<win_fwd_kernel<T, DH, 32, 4, 1>>((long long)a.N * a.H * ((a.Tq + 4 * BQ - 1) / (4 * BQ)), 256, 
                           (size_t)4 * Lay<T, DH>::bytes(32), st, a);
-    return over_keys<T, DH, BN>(a, [&](auto nw, int waves, long long blocks, size_t lds) { return launch<win_fwd_kernel<T, DH, BN, decltype(nw)::value>>(blocks, 64 * waves, lds, st, a); });
+    return over_keys<T, DH, BN>(a, [&](auto nw, auto ks, int waves, long long blocks, size_t lds) { return launch<win_fwd_kernel<T, DH, BN, decltype(nw)::value, decltype(ks)::value>>(blocks, 64 * waves, lds, st, a); });
 }
 template <typename T, int DH> size_t dkv_lds(int kg, int qh, int u, int buffers) {
     const size_t stages = (size_t)buffers * qh * u * (2 * Lay<T, DH>::bytes(BQ) + 256) + kg * PARKED<T, DH> * 1024, sums = (size_t)(qh - 1) * kg * BQ * DH * sizeof(float);
@@ -1236,7 +1307,7 @@ template <typename T, int DH> int bwd(const WinArgs& a, hipStream_t st) {
     if (a.G == 1 && a.Tq > 0 && a.Tk > 0 && waves <= MOST_WAVES<T> && whole <= MOST_LDS && ((long long)a.N * a.H >= 256 || Lay<T, DH>::ROWB == 128))
         return launch<win_bwd_short_kernel<T, DH>>((long long)a.N * a.H, 64 * waves, whole, st, a);
     if (a.Tq > 0)
-        if (int rc = over_keys<T, DH, BN>(a, [&](auto nw, int waves, long long blocks, size_t lds) { return launch<win_bwd_dq_kernel<T, DH, BN, decltype(nw)::value>>(blocks, 64 * waves, lds, st, a); }))
+        if (int rc = over_keys<T, DH, BN>(a, [&](auto nw, auto ks, int waves, long long blocks, size_t lds) { return launch<win_bwd_dq_kernel<T, DH, BN, decltype(nw)::value, decltype(ks)::value>>(blocks, 64 * waves, lds, st, a); }))
             return rc;
     if (a.Tk == 0) return 0;
     if (a.sink_keys > 0)

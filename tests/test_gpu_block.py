@@ -135,6 +135,9 @@ CASES = {
     "heads of one workgroup, wide rows": (86, 200, 224, 3, 3, 128, 60, 0, 2),
     "heads of one workgroup, few queries": (256, 3, 120, 1, 1, 128, None, 100, 0),
     "wide rows, many keys": (1, 70, 2100, 2, 1, 128, None, None, 0),
+    "many workgroups": (20, 290, 290, 8, 4, 64, 60, 0, 2),
+    "many workgroups, wide rows": (16, 300, 300, 8, 2, 128, 100, 20, 1),
+    "many workgroups, many keys": (5, 140, 2100, 26, 13, 128, None, None, 0),
     "wide rows, windows over 2000 keys": (1, 2300, 2300, 1, 1, 128, 2060, 0, 3),
 }
 
@@ -188,6 +191,21 @@ def test_keys_that_nobody_may_see_are_not_read_into_results(dtype, Tq):
     for key_mask, kv_len in ((mask, None), (None, lens), (mask.to(torch.uint8), lens)):
         for left, right in ((None, None), (20, 0), (9, 30)):
             run_both(dtype, (N, Tq, Tk, 4, 2, 64, left, right, 2), key_mask=key_mask, kv_len=kv_len, spoil=True)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("N,H,dh", [(24, 8, 64), (24, 6, 128), (3, 2, 64), (3, 2, 128)])
+def test_many_and_few_workgroups_with_masks_lengths_and_positions(dtype, N, H, dh):
+    """Odd numbers of key tiles, for workgroups that share them between their waves and for those that do not."""
+    T = 310
+    g = torch.Generator().manual_seed(N + dh)
+    lens = torch.randint(0, T + 1, (N,), generator=g, dtype=torch.int32).cuda()
+    mask = (torch.rand(N, T, generator=g) < 0.7).cuda()
+    mask[1] = False
+    pos = torch.randint(-100, 100, (N,), generator=g, dtype=torch.int32).cuda()
+    run_both(dtype, (N, T, T, H, 2, dh, 70, 30, 5), key_mask=mask, kv_len=lens, q_pos=pos, spoil=True)
+    run_both(dtype, (N, T, T, H, 2, dh, None, 0, 0), key_mask=mask, spoil=True)
+    run_both(dtype, (N, T, 300, H, 2, dh, None, None, 0), kv_len=lens, spoil=True)
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "fp32"])
