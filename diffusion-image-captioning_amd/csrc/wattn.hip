@@ -1182,15 +1182,17 @@ int check(int dtype, const DicWinAttnParams* p, bool bwd, bool pointers = true) 
                     : apart(p->out_stride, p->N, p->Tq, p->H, p->dh), "dic_win_attn: rows of an output overlap");
     return 0;
 }
-// The dk / dv kernel's workgroup: kg groups of 32 keys and qh groups of 32 query rows.  All keys where they are few and the heads many; else 8 waves (one
-// workgroup to a CU) for 128 wide bf16 rows and 4 otherwise, fewer keys and more rows to a workgroup until there is one for every place on the card.
+// The dk / dv kernel's workgroup: kg groups of 32 keys and qh groups of 32 query rows.  All keys where they are few and the heads many (600 key heads of 200
+// x 128: 242 us, cut in two 270); else four waves, as 4 x 1, 2 x 2 or 1 x 4 as there are workgroups for two, or most of one, on every CU: whole backward passes
+// of 128 wide rows, 4 x 2048 rows, 16 query and 4 key heads: 589 / 527 us with 256 / 512 workgroups of 4 x 1 / 2 x 2; 1 x 2048, 12 heads: 197 / 181 / 245 with
+// 192 / 384 / 768; 2 x 700, 8 heads: 63 / 55 / 71 with 96 / 176 / 352; 1 x 700, 8 heads: 52 / 47 for 2 x 2 / 1 x 4 with 88 / 176.
 struct Shape { int kg, qh; };
 Shape shape_of(const WinArgs& a, int waves, int most, int most_rows) {
     const int tiles = (a.Tk + BQ - 1) / BQ;
     const long long heads = (long long)a.N * a.Hkv;
     if (tiles <= most && heads >= 256) return {tiles, 1};
     int kg = waves;
-    while (kg > 1 && heads * ((tiles + kg - 1) / kg) < 2048 / waves && waves / kg < most_rows) kg >>= 1;
+    while (kg > 1 && heads * ((tiles + kg - 1) / kg) < (kg > 2 ? 512 : 160) && waves / kg < most_rows) kg >>= 1;
     return {kg, waves / kg};
 }
 // Row groups at most: with 2, the stages of fp32 rows of 256 bytes let two workgroups share a CU (4 x 513 rows, 12 heads: 75 us, with 4 87), and those of 512
@@ -1211,7 +1213,9 @@ void plan_sinks(WinArgs& a) {
     if (a.chunks < 1) a.chunks = 1;
 }
 long long sink_floats(const WinArgs& a, int dh) { return (long long)a.N * a.Hkv * a.chunks * a.sink_rows * 2 * dh; }
-// Few query rows: one workgroup per key head and sequence, or several that share the keys while that fills the card and leaves each 8 tiles to read.
+// Few query rows: one workgroup per key head and sequence, or several that share the keys while that fills the card and leaves each 8 tiles to read.  One token,
+// 32 query and 8 key heads of 128: 64 sequences of 1000 keys 44 us, a wave for each query head's tile 114, of 128 keys 11 and 29; one sequence of 16384 keys
+// 43 us in 64 pieces, 173 in one workgroup a head.
 bool few_rows(const WinArgs& a) { return a.G * (long long)a.Tq <= FEW && a.Tk > 64; }
 // Keys that the rows of one key head see together when they are few, at most (where the host can tell: no lengths, no masks).
 long long span_keys(const WinArgs& a) {
