@@ -1202,7 +1202,7 @@ template <typename T, int DH> constexpr int ROW_GROUPS = sizeof(T) == 2 ? 4 : 2;
 void plan_sinks(WinArgs& a) {
     a.near_sinks = a.left >= 0 ? (a.sinks < a.Tk ? a.sinks : a.Tk) : 0;
     // The sinks' tile walks Tq rows, another one about left + right + 128 of them: it needs no pass of its own while the card has as much else to do
-    // (130 rows in windows of 129, 3072 heads: that pass took 43 us beside the window pass's 150).
+    // (130 rows in windows of 129, 3072 heads, before other steps: that pass took 43 us beside the window pass of 150).
     const long long others = a.right < 0 ? a.Tq : (long long)a.left + a.right + 128, all = (long long)a.N * a.Hkv * ((a.Tk + 127) / 128) * (others < a.Tq ? others : a.Tq);
     if (a.near_sinks > 0 && a.Tq > 2 * others && a.Tq > all / 256) { a.sink_keys = a.near_sinks; a.near_sinks = 0; }
     a.sink_rows = (a.sink_keys + BQ - 1) / BQ * BQ;
@@ -1275,7 +1275,7 @@ template <auto KERNEL, typename... More> int launch(long long blocks, int thread
 constexpr long long SPLIT = 256;
 constexpr size_t SHARED_CU_LDS = 75 << 10;                       // two workgroups fit a CU's 160 KB
 // The workgroups of a kernel that walks the keys.  Few keys: all of them in LDS at once (unless that keeps a second workgroup off the CU) and the query rows
-// of a sequence in one workgroup where they fit (130 rows x 130 keys x 3072 heads, forward: 5 waves 86 us, 4 waves and a second workgroup 113 us).
+// of a sequence in one workgroup where they fit (130 rows x 130 keys x 3072 heads, forward, before its other steps: 5 waves 86 us, 4 waves and a second workgroup 113).
 template <typename T, int DH, int BN, typename F> int over_keys(const WinArgs& a, F&& go) {
     constexpr int MOST = MOST_WAVES<T>;
     const int rows = (a.Tq + BQ - 1) / BQ, tiles = (a.Tk + BN - 1) / BN;
