@@ -346,6 +346,27 @@ def test_window_attention_gradients_are_differences_of_the_output():
         assert abs(slope - float((grads[which].double() * u).sum())) < 1e-4 * (1 + abs(slope))      # 2e-5 of the norm, and e^2 of the differences
 
 
+@pytest.mark.parametrize("Tq,Tk,Hq", [(1, 300, 4), (200, 300, 2), (100, 230, 1), (290, 300, 1)])
+def test_rows_of_a_cache_far_apart(Tq, Tk, Hq):
+    """Tokens 16 MiB apart, so that offsets pass 2^32 bytes: the results of the same rows side by side, bit for bit."""
+    step = 1 << 23                                                           # bf16 elements
+    g = torch.Generator(device="cuda").manual_seed(Tk)
+    q, dout = (torch.randn(1, Tq, Hq, 64, generator=g, device="cuda").to(BF16) for _ in range(2))
+    k, v = (torch.randn(1, Tk, 1, 64, generator=g, device="cuda").to(BF16) for _ in range(2))
+    room = torch.empty(step * (Tk - 1) + 256, dtype=BF16, device="cuda")
+    far = [room.as_strided((1, Tk, 1, 64), (0, step, 0, 1), 64 * i) for i in range(4)]
+    far[0].copy_(k)
+    far[1].copy_(v)
+    for how in (dict(left=120, right=0, sinks=3, q_pos=torch.tensor([Tk - Tq], dtype=torch.int32, device="cuda")), dict()):
+        out, lse = dic.window_attention(q, k, v, **how)
+        dq, dk, dv = dic.window_attention_grad(dout, q, k, v, out, lse, **how)
+        o2, l2 = dic.window_attention(q, *far[:2], **how)
+        d2 = torch.empty_like(q)
+        dic.window_attention_grad(dout, q, *far[:2], o2, l2, grads=(d2, far[2], far[3]), **how)
+        for name, x, y in (("out", out, o2), ("lse", lse, l2), ("dq", dq, d2), ("dk", dk, far[2]), ("dv", dv, far[3])):
+            assert torch.equal(x, y), name
+
+
 def test_outputs_can_be_views_and_nothing_else_is_written():
     N, T, Hq, Hkv, dh = 2, 70, 4, 2, 64
     qkv = torch.randn(N, T, Hq + 2 * Hkv, dh, device="cuda").to(BF16)
