@@ -353,7 +353,7 @@ template <typename T, int DH, int BN, int NW, int KS> struct KeyTiles {
 // Long spans are bound by the issue of matrix and vector instructions together (a 32 x 32 block is 16 of the former at 32 cycles a SIMD, and some 450 cycles of
 // exponentials, masks, maxima and conversions; two or three waves a SIMD overlap them in part): 8192 rows that see 4096 keys, 16 heads of 128: 240 us, 860
 // TFLOP/s of visible pairs, where a library matrix product reaches 1350; in windows of 1024, 2 x 4096 rows: 95 us, 630.  Short ones are bound by moving their
-// rows with little to compute meanwhile: 3072 heads of 130 x 64: 197 MB in 67 us, 2.9 TB/s.  8 x 2050 rows in windows of 513, 12 heads of 64: 51 us.
+// rows with little to compute meanwhile: 256 x 12 heads of 130 x 64: 197 MB in 67 us, 2.9 TB/s.  8 x 2050 rows in windows of 513, 12 heads of 64: 51 us.
 template <typename T, int DH, int BN, int NW, int KS>
 __global__ __launch_bounds__(64 * MOST_WAVES<T>, (DH == 128 && BN == 32 && sizeof(T) == 2 ? 3 : RESIDENT<T, DH, 4>)) void win_fwd_kernel(const WinArgs a) {
     using L = Lay<T, DH>;
@@ -864,7 +864,7 @@ __device__ __forceinline__ void dkv_block(const char* qt, const char* dt, const 
     }
 }
 // One workgroup has a head's queries and keys whole, wave w queries 32 w.. and keys 32 w.., and reads them once: keys and values lie in LDS and the wave's
-// query rows in registers for dq; then they change places, and dk and dv follow without another read.  3072 heads of 130 x 64 in bf16: 168 us (160
+// query rows in registers for dq; then they change places, and dk and dv follow without another read.  256 x 12 heads of 130 x 64 in bf16: 168 us (160
 // without the exact delta) for the two kernels' 202; 8 tensors of 51 MB at 2.4 TB/s, where moving them alone would take 90 us: of 130 rows the fifth wave's 30
 // are padding, and two workgroups of five waves share a CU (bounded to 128 registers, for three, it spilled 23 and was 17 us slower).
 template <typename T, int DH>
@@ -1202,7 +1202,7 @@ template <typename T, int DH> constexpr int ROW_GROUPS = sizeof(T) == 2 ? 4 : 2;
 void plan_sinks(WinArgs& a) {
     a.near_sinks = a.left >= 0 ? (a.sinks < a.Tk ? a.sinks : a.Tk) : 0;
     // The sinks' tile walks Tq rows, another one about left + right + 128 of them: it needs no pass of its own while the card has as much else to do
-    // (130 rows in windows of 129, 3072 heads, before other steps: that pass took 43 us beside the window pass of 150).
+    // (130 rows in windows of 129, 256 x 12 heads, before other steps: that pass took 43 us beside the window pass of 150).
     const long long others = a.right < 0 ? a.Tq : (long long)a.left + a.right + 128, all = (long long)a.N * a.Hkv * ((a.Tk + 127) / 128) * (others < a.Tq ? others : a.Tq);
     if (a.near_sinks > 0 && a.Tq > 2 * others && a.Tq > all / 256) { a.sink_keys = a.near_sinks; a.near_sinks = 0; }
     a.sink_rows = (a.sink_keys + BQ - 1) / BQ * BQ;
@@ -1275,7 +1275,7 @@ template <auto KERNEL, typename... More> int launch(long long blocks, int thread
 constexpr long long SPLIT = 256;
 constexpr size_t SHARED_CU_LDS = 75 << 10;                       // two workgroups fit a CU's 160 KB
 // The workgroups of a kernel that walks the keys.  Few keys: all of them in LDS at once (unless that keeps a second workgroup off the CU) and the query rows
-// of a sequence in one workgroup where they fit (130 rows x 130 keys x 3072 heads, forward, before its other steps: 5 waves 86 us, 4 waves and a second workgroup 113).
+// of a sequence in one workgroup where they fit (130 rows x 130 keys x 12 heads x 256 sequences, forward, before its other steps: 5 waves 86 us, 4 waves and a second workgroup 113).
 template <typename T, int DH, int BN, typename F> int over_keys(const WinArgs& a, F&& go) {
     constexpr int MOST = MOST_WAVES<T>;
     const int rows = (a.Tq + BQ - 1) / BQ, tiles = (a.Tk + BN - 1) / BN;
@@ -1317,7 +1317,7 @@ template <typename T, int DH> int bwd(const WinArgs& a, hipStream_t st) {
     const size_t whole = (size_t)waves * (2 * Lay<T, DH>::bytes(BQ) + 256 + PARKED<T, DH> * 1024);
     // A head to a workgroup where there is one for every CU (128 wide bf16 rows, 1024 heads of 146: 137 us against 157 in two passes; 32 heads of 224: 33 against
     // 28; fp32, 768 heads of 128 x 64: 116 against 142, 24 heads: 39 against 34), and always for rows of 128 bytes, of which a wave holds and multiplies the
-    // least (3072 heads of 130: 168 against 202 us; 12 heads of 146: 16 against 19, of 256: 23.5 against 23).
+    // least (256 x 12 heads of 130: 168 against 202 us; 12 heads of 146: 16 against 19, of 256: 23.5 against 23).
     if (a.G == 1 && a.Tq > 0 && a.Tk > 0 && waves <= MOST_WAVES<T> && whole <= MOST_LDS && ((long long)a.N * a.H >= 256 || Lay<T, DH>::ROWB == 128))
         return launch<win_bwd_short_kernel<T, DH>>((long long)a.N * a.H, 64 * waves, whole, st, a);
     if (a.Tq > 0)
