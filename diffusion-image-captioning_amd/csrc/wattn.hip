@@ -16,7 +16,9 @@
 namespace {
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
-constexpr int FAR = (1 << 30) - 2;              // positions and bounds are clamped to +-FAR: sums of two stay inside 32 bits
+// Positions are clamped to +-FAR_POS and bounds to FAR, which is behind every key from every position (there are at most 2^28 rows), so that a finite bound
+// never cuts where the unclamped one would not; position + rows + bound stays inside 32 bits.
+constexpr int FAR_POS = 1 << 29, FAR = (1 << 30) - 2;
 
 struct Strides { long long n, t, h; };
 struct WinArgs {
@@ -237,7 +239,7 @@ struct Seq { int kvl, pos, from; };
 __device__ __forceinline__ Seq sequence(const WinArgs& a, int n) {
     Seq s;
     s.kvl = a.kv_len ? clampi(a.kv_len[n], 0, a.Tk) : a.Tk;
-    s.pos = a.q_pos ? clampi(a.q_pos[n], -FAR / 2, FAR / 2) : 0;
+    s.pos = a.q_pos ? clampi(a.q_pos[n], -FAR_POS, FAR_POS) : 0;
     if (a.right >= 0) s.kvl = clampi(s.pos + a.Tq + a.right, 0, s.kvl);
     s.from = a.left < 0 ? 0 : max(0, s.pos - a.left);
     return s;
@@ -1247,8 +1249,8 @@ WinArgs args_of(const DicWinAttnParams* p) {
     a.sdo = rows_q(p->dout_stride); a.sdq = rows_q(p->dq_stride); a.sdk = rows_k(p->dk_stride); a.sdv = rows_k(p->dv_stride);
     a.key_mask = p->key_mask; a.kv_len = p->kv_len; a.q_pos = p->q_pos;
     a.N = p->N; a.Tq = p->Tq; a.Tk = p->Tk; a.H = p->H; a.Hkv = p->Hkv; a.G = p->H / p->Hkv;
-    a.left = p->left < 0 ? -1 : (p->left < FAR / 2 ? p->left : FAR / 2);
-    a.right = p->right < 0 ? -1 : (p->right < FAR / 2 ? p->right : FAR / 2);
+    a.left = p->left < 0 ? -1 : (p->left < FAR ? p->left : FAR);
+    a.right = p->right < 0 ? -1 : (p->right < FAR ? p->right : FAR);
     a.sinks = p->sinks; a.scale = p->scale; a.c = p->scale * LOG2E;
     plan_sinks(a);
     return a;

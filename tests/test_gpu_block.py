@@ -259,6 +259,23 @@ def test_query_positions(dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("Tq,Hq,Hkv", [(2, 4, 2), (50, 4, 2), (50, 2, 2)])
+def test_bounds_as_far_as_the_farthest_positions(dtype, Tq, Hq, Hkv):
+    """Finite bounds beside positions of +-2^29: they cut where they say, and larger ones nowhere."""
+    pos = torch.tensor([2 ** 29, 2 ** 29 - 7, 2 ** 31 - 1, 0, -2 ** 29, 7 - 2 ** 29, -2 ** 31], dtype=torch.int32, device="cuda")
+    clamped = pos.clamp(-2 ** 29, 2 ** 29)
+    N, Tk = len(pos), 260
+    g = torch.Generator(device="cuda").manual_seed(7)
+    q, k, v, dout = (torch.randn(N, t, n, 64, generator=g, device="cuda").to(dtype) for t, n in ((Tq, Hq), (Tk, Hkv), (Tk, Hkv), (Tq, Hq)))
+    for left, right in ((2 ** 31 - 1, None), (None, 2 ** 31 - 1), (2 ** 30, 2 ** 30), (2 ** 31 - 1, 0), (2 ** 29, None), (2 ** 29 - 100, 2 ** 29 + 90), (None, 2 ** 29 + 3)):
+        how = dict(left=left, right=right, sinks=2, q_pos=pos)
+        want = definition(q, k, v, visible(N, Tq, Tk, left, right, 2, None, None, clamped.long()), 0.125, dout)
+        out, lse = dic.window_attention(q, k, v, **how)
+        for name, t in zip(("out", "lse", "dq", "dk", "dv"), (out, lse, *dic.window_attention_grad(dout, q, k, v, out, lse, **how))):
+            holds(name, t, want[name])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("Tq", [2, 60])
 def test_masks_of_more_tiles_than_are_read_at_once(dtype, Tq):
     """A mask over 35000 keys (547 tiles of 64, 1094 of 32), most of them hidden; the queries stand at the end."""
