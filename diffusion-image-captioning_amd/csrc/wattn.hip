@@ -245,7 +245,10 @@ __device__ __forceinline__ Seq sequence(const WinArgs& a, int n) {
     return s;
 }
 // Query at position t sees the keys [lo, hi) and [0, sk).
-struct Span { int lo, hi, sk; };
+struct Span {
+    int lo, hi, sk;
+    __device__ __forceinline__ int keys() const { return max(0, hi - lo) + min(sk, lo); }        // (sinks inside the window are counted once)
+};
 __device__ __forceinline__ Span span_of(const WinArgs& a, int t, int kvl) {
     Span s;
     s.lo = a.left < 0 ? 0 : max(0, t - a.left);
@@ -642,7 +645,7 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 3>)) void win_
     const int hk = item % a.Hkv, n = item / a.Hkv, h = hk * a.G + g;
     const Seq sq = sequence(a, n);
     const Span s0 = span_of(a, sq.pos + qt * bm, sq.kvl), s1 = span_of(a, sq.pos + min(qt * bm + bm, a.Tq) - 1, sq.kvl);
-    if (BF16<T> && min(s0.hi - s0.lo + s0.sk, s1.hi - s1.lo + s1.sk) <= FEW_KEYS) dq_rows<T, DH, BN, NW, KS, BF16<T>>(a, n, hk, h, qt, sq, smem, table);
+    if (BF16<T> && min(s0.keys(), s1.keys()) <= FEW_KEYS) dq_rows<T, DH, BN, NW, KS, BF16<T>>(a, n, hk, h, qt, sq, smem, table);
     else dq_rows<T, DH, BN, NW, KS, false>(a, n, hk, h, qt, sq, smem, table);
 }
 

@@ -329,6 +329,24 @@ def test_few_keys_share_a_row_and_its_gradients_are_as_good_as_two_roundings(sha
         assert float((t.double() - value).norm() / value.norm()) < 2.0 ** -8 * math.sqrt(2 / 3), name
 
 
+def gradients_of_peaked_rows(left, sinks, mask, scale):
+    """bf16 dq, dk, dv and their exact values for 2 x 900 rows, 4 query and 2 key heads, causal: logits spread widely enough that a few keys hold a row's weight."""
+    N, T, Hq, Hkv, dh = 2, 900, 4, 2, 64
+    g = torch.Generator(device="cuda").manual_seed(T)
+    q, k, v, dout = (torch.randn(N, T, h, dh, generator=g, device="cuda").to(BF16) for h in (Hq, Hkv, Hkv, Hq))
+    how = dict(left=left, right=0, sinks=sinks, key_mask=mask, scale=scale)
+    want = definition(q, k, v, visible(N, T, T, left, 0, sinks, mask, None, None), scale, dout)
+    out, lse = dic.window_attention(q, k, v, **how)
+    return dict(zip(("dq", "dk", "dv"), dic.window_attention_grad(dout, q, k, v, out, lse, **how))), {k: want[k][0] for k in ("dq", "dk", "dv")}
+
+
+def test_sinks_inside_the_window_count_once_where_few_keys_share_a_row():
+    """Rows 128 to 255 of a causal text see at most 256 keys, all inside the window, the sinks among them: as good as two roundings (above)."""
+    got, want = gradients_of_peaked_rows(500, 400, None, 0.6)
+    part = slice(128, 256)
+    assert float((got["dq"].double() - want["dq"])[:, part].norm() / want["dq"][:, part].norm()) < 2.0 ** -8 * math.sqrt(2 / 3)
+
+
 @pytest.mark.parametrize("Tq,Tk", [(0, 5), (5, 0), (0, 0)])
 def test_window_attention_of_nothing(Tq, Tk):
     q, k = torch.randn(2, Tq, 4, 64, device="cuda"), torch.randn(2, Tk, 2, 64, device="cuda")
