@@ -506,6 +506,27 @@ template <int ND> __device__ __forceinline__ float exactly(f32x16 (&acc)[ND], co
         for (int r = 0; r < 16; ++r) acc[d][r] = fmaf(-off, mean[d][r], acc[d][r]);
     return off;
 }
+// Does key_mask leave a row between those of the spans s0 (the first) and s1 (the last) at most FEW_KEYS keys?  Counts the keys that all of these rows see, so
+// that no such row is missed; some rows with up to the workgroup's row count more then get the exact form, too.  Every wave counts for itself (the same bytes,
+// the same answer), 512 keys to a round trip, and stops once there are enough: one or two round trips where most keys are there (masked backward pass, 2 x 4096 rows, 16 heads of
+// 128, a tenth of the keys masked: windows of 1024 325 -> 329 us; of 341, whose rows share 214 keys, in the exact form now: 184 -> 196).
+__device__ __forceinline__ bool mask_leaves_few(const WinArgs& a, int n, const Span& s0, const Span& s1) {
+    const uint8_t* mask = a.key_mask + (size_t)n * a.Tk;
+    const int lane = threadIdx.x & 63;
+    int count = 0;
+    auto add = [&](int lo, int hi) {
+        for (int j0 = lo; j0 < hi && count <= FEW_KEYS; j0 += 512) {
+            int byte[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) { const int j = j0 + 64 * e + lane; byte[e] = j < hi ? mask[j] : 0; }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) count += __popcll(__ballot(byte[e] != 0));
+        }
+    };
+    add(s1.lo, s0.hi);
+    add(0, min(s0.sk, s1.lo));
+    return count <= FEW_KEYS;
+}
 // acc += the part of dq / scale that 32 keys have; bit of `word`: the lane's query sees that key (`full`: all of them).
 // EXACT (bf16): delta is dout . out with the ROUNDED out, off by e_i; where few keys share a row's weight that outweighs what rounding ds costs (windows of 3 keys in
 // bf16: dq and dk 3.7e-3 off, in norm, of which rounding the results themselves is 1.7e-3).  Then `off` sums ds in 32 bits over the lane's keys, which is
@@ -645,7 +666,7 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 3>)) void win_
     const int hk = item % a.Hkv, n = item / a.Hkv, h = hk * a.G + g;
     const Seq sq = sequence(a, n);
     const Span s0 = span_of(a, sq.pos + qt * bm, sq.kvl), s1 = span_of(a, sq.pos + min(qt * bm + bm, a.Tq) - 1, sq.kvl);
-    if (BF16<T> && min(s0.keys(), s1.keys()) <= FEW_KEYS) dq_rows<T, DH, BN, NW, KS, BF16<T>>(a, n, hk, h, qt, sq, smem, table);
+    if (BF16<T> && (min(s0.keys(), s1.keys()) <= FEW_KEYS || (a.key_mask && mask_leaves_few(a, n, s0, s1)))) dq_rows<T, DH, BN, NW, KS, BF16<T>>(a, n, hk, h, qt, sq, smem, table);
     else dq_rows<T, DH, BN, NW, KS, false>(a, n, hk, h, qt, sq, smem, table);
 }
 

@@ -347,6 +347,16 @@ def test_sinks_inside_the_window_count_once_where_few_keys_share_a_row():
     assert float((got["dq"].double() - want["dq"])[:, part].norm() / want["dq"][:, part].norm()) < 2.0 ** -8 * math.sqrt(2 / 3)
 
 
+@pytest.mark.parametrize("left,sinks,every", [(None, 0, 4), (600, 0, 200), (600, 5, 200), (300, 600, 4), (400, 40, 9)])
+def test_few_keys_that_a_mask_leaves_share_a_row(left, sinks, every):
+    """Long spans of which key_mask leaves at most 256 keys: as good as two roundings, as if there were no others."""
+    mask = torch.zeros(2, 900, dtype=torch.bool, device="cuda")
+    mask[:, ::every] = True
+    got, want = gradients_of_peaked_rows(left, sinks, mask, 0.6)
+    for name in got:
+        assert float((got[name].double() - want[name]).norm() / want[name].norm()) < 2.0 ** -8 * math.sqrt(2 / 3), name
+
+
 @pytest.mark.parametrize("Tq,Tk", [(0, 5), (5, 0), (0, 0)])
 def test_window_attention_of_nothing(Tq, Tk):
     q, k = torch.randn(2, Tq, 4, 64, device="cuda"), torch.randn(2, Tk, 2, 64, device="cuda")
