@@ -1187,7 +1187,8 @@ int check(int dtype, const DicWinAttnParams* p, bool bwd, bool pointers = true) 
     DIC_REQUIRE(p->N >= 0 && p->Tq >= 0 && p->Tk >= 0 && p->Tq <= (1 << 28) && p->Tk <= (1 << 28), "dic_win_attn: sizes out of range");
     DIC_REQUIRE(p->H > 0 && p->Hkv > 0 && p->H % p->Hkv == 0, "dic_win_attn: the number of heads must be a multiple of the number of key heads");
     DIC_REQUIRE(p->sinks >= 0 && std::isfinite(p->scale) && p->scale > 0.f, "dic_win_attn: sinks >= 0 and a positive finite scale are needed");
-    DIC_REQUIRE((long long)p->N * p->H * (p->Tq / 32 + 1) < (1ll << 31) && (long long)p->N * p->Hkv * (p->Tk / 32 + 1) < (1ll << 31), "dic_win_attn: too many tiles for one launch");
+    const long long heads = (long long)p->N * p->H, most = 1ll << 31;          // (heads >= N Hkv; bounded by itself first, as three factors may pass 64 bits)
+    DIC_REQUIRE(heads < most && heads * (p->Tq / 32 + 1) < most && (long long)p->N * p->Hkv * (p->Tk / 32 + 1) < most, "dic_win_attn: too many tiles for one launch");
     if (!pointers) return 0;
     const bool nq = p->N && p->Tq, nk = p->N && p->Tk;
     DIC_REQUIRE(!nq || (p->q && (bwd ? p->out && p->lse && p->dout && p->dq : p->out != nullptr)), "dic_win_attn: null query-side pointer");
@@ -1280,7 +1281,13 @@ WinArgs args_of(const DicWinAttnParams* p) {
     return a;
 }
 constexpr int MOST_LDS = 150 << 10;                              // of a workgroup, beside what kernels hold under a name
-template <auto KERNEL, typename... More> int launch(long long blocks, int threads, size_t lds, hipStream_t st, More... more) {
+// A call goes through its launches twice: once to see that each can be made (a grid holds less than 2^32 threads), so that none runs in front of one that cannot.
+struct Where { hipStream_t st; bool look; };
+template <auto KERNEL, typename... More> int launch(long long blocks, int threads, size_t lds, Where w, More... more) {
+    if (w.look) {
+        DIC_REQUIRE(blocks < (1ll << 31) && blocks * threads < (1ll << 32), "dic_win_attn: too many workgroups for one launch");
+        return 0;
+    }
     if (lds > (64 << 10)) {                     // once for each device: the attribute belongs to its copy of the kernel
         static std::atomic<unsigned long long> allowed{0};
         int dev = 0;
@@ -1291,7 +1298,7 @@ template <auto KERNEL, typename... More> int launch(long long blocks, int thread
         }
         if (e != hipSuccess) { dic_set_error(hipGetErrorString(e)); return (int)e; }
     }
-    hipLaunchKernelGGL(KERNEL, dim3((unsigned)blocks), dim3(threads), lds, st, more...);
+    hipLaunchKernelGGL(KERNEL, dim3((unsigned)blocks), dim3(threads), lds, w.st, more...);
     DIC_CHECK_LAUNCH();
     return 0;
 }
@@ -1317,27 +1324,27 @@ template <typename T, int DH, int BN, typename F> int over_keys(const WinArgs& a
     if (blocks <= SPLIT) return go(four, two, 4, heads * ((rows + 1) / 2), 2 * turns > sums ? 2 * turns : sums);
     return go(four, one, 4, blocks, turns);
 }
-template <typename T, int DH> int fwd(const WinArgs& a, hipStream_t st) {
+template <typename T, int DH> int fwd(const WinArgs& a, Where w) {
     constexpr int BN = sizeof(T) == 2 ? 64 : 32;
     if (few_rows(a)) {
         const int splits = splits_of(a);
-        if (int rc = launch<win_few_kernel<T, DH>>((long long)a.N * a.Hkv * splits, 64 * Few<T, DH>::NW, Few<T, DH>::LDS, st, a, splits)) return rc;
-        return splits > 1 ? launch<win_merge_kernel<T, DH>>(((long long)a.N * a.H * a.Tq + 3) / 4, 256, 0, st, a, splits) : 0;
+        if (int rc = launch<win_few_kernel<T, DH>>((long long)a.N * a.Hkv * splits, 64 * Few<T, DH>::NW, Few<T, DH>::LDS, w, a, splits)) return rc;
+        return splits > 1 ? launch<win_merge_kernel<T, DH>>(((long long)a.N * a.H * a.Tq + 3) / 4, 256, 0, w, a, splits) : 0;
     }
     // 128 wide rows that see many keys: tiles of 32, which take the registers and LDS of three workgroups a CU instead of two (one text of 8192 rows, 4096 keys
     // each, 16 heads: 249 us against 277; rows of 1024 keys, 2 x 4096 rows: 104 us against 96)
     if constexpr (sizeof(T) == 2 && DH == 128)
         if (span_keys(a) >= 2048 && (long long)a.N * a.H * ((a.Tq + 4 * BQ - 1) / (4 * BQ)) > SPLIT)
             return launch<win_fwd_kernel<T, DH, 32, 4, 1>>((long long)a.N * a.H * ((a.Tq + 4 * BQ - 1) / (4 * BQ)), 256, 
-                          (size_t)4 * Lay<T, DH>::bytes(32), st, a);
-    return over_keys<T, DH, BN>(a, [&](auto nw, auto ks, int waves, long long blocks, size_t lds) { return launch<win_fwd_kernel<T, DH, BN, decltype(nw)::value, decltype(ks)::value>>(blocks, 64 * waves, lds, st, a); });
+                          (size_t)4 * Lay<T, DH>::bytes(32), w, a);
+    return over_keys<T, DH, BN>(a, [&](auto nw, auto ks, int waves, long long blocks, size_t lds) { return launch<win_fwd_kernel<T, DH, BN, decltype(nw)::value, decltype(ks)::value>>(blocks, 64 * waves, lds, w, a); });
 }
 template <typename T, int DH> size_t dkv_lds(int kg, int qh, int u, int buffers) {
     const size_t stages = (size_t)buffers * qh * u * (2 * Lay<T, DH>::bytes(BQ) + 256) + kg * PARKED<T, DH> * 1024, sums = (size_t)(qh - 1) * kg * BQ * DH * sizeof(float);
     const size_t out = WHOLE_ROWS<T, DH> ? (size_t)kg * 32 * OUT_ROW<T, DH> : 0, most = stages > sums ? stages : sums;
     return most > out ? most : out;
 }
-template <typename T, int DH> int bwd(const WinArgs& a, hipStream_t st) {
+template <typename T, int DH> int bwd(const WinArgs& a, Where w) {
     constexpr int BN = sizeof(T) == 2 ? 64 : 32;
     const int waves = ((a.Tq > a.Tk ? a.Tq : a.Tk) + BQ - 1) / BQ;
     const size_t whole = (size_t)waves * (2 * Lay<T, DH>::bytes(BQ) + 256 + PARKED<T, DH> * 1024);
@@ -1345,22 +1352,30 @@ template <typename T, int DH> int bwd(const WinArgs& a, hipStream_t st) {
     // 28; fp32, 768 heads of 128 x 64: 116 against 142, 24 heads: 39 against 34), and always for rows of 128 bytes, of which a wave holds and multiplies the
     // least (256 x 12 heads of 130: 168 against 202 us; 12 heads of 146: 16 against 19, of 256: 23.5 against 23).
     if (a.G == 1 && a.Tq > 0 && a.Tk > 0 && waves <= MOST_WAVES<T> && whole <= MOST_LDS && ((long long)a.N * a.H >= 256 || Lay<T, DH>::ROWB == 128))
-        return launch<win_bwd_short_kernel<T, DH>>((long long)a.N * a.H, 64 * waves, whole, st, a);
+        return launch<win_bwd_short_kernel<T, DH>>((long long)a.N * a.H, 64 * waves, whole, w, a);
     if (a.Tq > 0)
-        if (int rc = over_keys<T, DH, BN>(a, [&](auto nw, auto ks, int waves, long long blocks, size_t lds) { return launch<win_bwd_dq_kernel<T, DH, BN, decltype(nw)::value, decltype(ks)::value>>(blocks, 64 * waves, lds, st, a); }))
+        if (int rc = over_keys<T, DH, BN>(a, [&](auto nw, auto ks, int waves, long long blocks, size_t lds) { return launch<win_bwd_dq_kernel<T, DH, BN, decltype(nw)::value, decltype(ks)::value>>(blocks, 64 * waves, lds, w, a); }))
             return rc;
     if (a.Tk == 0) return 0;
     if (a.sink_keys > 0)
         if (int rc = launch<win_bwd_dkv_kernel<T, DH, true>>((long long)a.N * a.Hkv * (a.sink_rows / BQ) * a.chunks, 64 * ROW_GROUPS<T, DH>,
-                            dkv_lds<T, DH>(1, ROW_GROUPS<T, DH>, 1, 2), st, a, 1, ROW_GROUPS<T, DH>, 1, 2)) return rc;
+                            dkv_lds<T, DH>(1, ROW_GROUPS<T, DH>, 1, 2), w, a, 1, ROW_GROUPS<T, DH>, 1, 2)) return rc;
     constexpr int WAVES = 4;
     const Shape s = shape_of(a, WAVES, MOST_WAVES<T>, ROW_GROUPS<T, DH>);
     // all queries in one stage where they take no more LDS than lets two workgroups share a CU; else as many to a stage (barriers) as two buffers hold
     const int all = s.qh == 1 && a.G == 1 ? (a.Tq + BQ - 1) / BQ : 0;
     int u = WAVES / 2 / s.qh > 1 ? WAVES / 2 / s.qh : 1, buffers = 2;
     if (all > 0 && dkv_lds<T, DH>(s.kg, 1, all, 1) <= SHARED_CU_LDS) { u = all; buffers = 1; }
-    return launch<win_bwd_dkv_kernel<T, DH, false>>((long long)a.N * a.Hkv * ((a.Tk + s.kg * BQ - 1) / (s.kg * BQ)), 64 * s.kg * s.qh, dkv_lds<T, DH>(s.kg, s.qh, u, buffers), st, a,
+    return launch<win_bwd_dkv_kernel<T, DH, false>>((long long)a.N * a.Hkv * ((a.Tk + s.kg * BQ - 1) / (s.kg * BQ)), 64 * s.kg * s.qh, dkv_lds<T, DH>(s.kg, s.qh, u, buffers), w, a,
                   s.kg, s.qh, u, buffers);
+}
+int fwd(int dtype, int dh, const WinArgs& a, Where w) {
+    if (dtype == DIC_BF16) return dh == 64 ? fwd<bf16_t, 64>(a, w) : fwd<bf16_t, 128>(a, w);
+    return dh == 64 ? fwd<float, 64>(a, w) : fwd<float, 128>(a, w);
+}
+int bwd(int dtype, int dh, const WinArgs& a, Where w) {
+    if (dtype == DIC_BF16) return dh == 64 ? bwd<bf16_t, 64>(a, w) : bwd<bf16_t, 128>(a, w);
+    return dh == 64 ? bwd<float, 64>(a, w) : bwd<float, 128>(a, w);
 }
 }  // namespace
 
@@ -1373,23 +1388,21 @@ extern "C" int dic_win_attn_fwd(int dtype, const DicWinAttnParams* p, void* stre
     if (int rc = check(dtype, p, false)) return rc;
     if (p->N == 0 || p->Tq == 0) return 0;
     WinArgs a = args_of(p);
+    if (int rc = fwd(dtype, p->dh, a, Where{nullptr, true})) return rc;
     const size_t need = ws_bytes(a, p->dh, false);
     DIC_REQUIRE(need == 0 || (p->ws && aligned(p->ws) && p->ws_bytes >= need), "dic_win_attn_fwd: workspace missing or too small (dic_win_attn_ws_bytes)");
     a.parts = (float*)p->ws;
-    hipStream_t st = (hipStream_t)stream;
-    if (dtype == DIC_BF16) return p->dh == 64 ? fwd<bf16_t, 64>(a, st) : fwd<bf16_t, 128>(a, st);
-    return p->dh == 64 ? fwd<float, 64>(a, st) : fwd<float, 128>(a, st);
+    return fwd(dtype, p->dh, a, Where{(hipStream_t)stream, false});
 }
 
 extern "C" int dic_win_attn_bwd(int dtype, const DicWinAttnParams* p, void* stream) {
     if (int rc = check(dtype, p, true)) return rc;
     if (p->N == 0) return 0;
     WinArgs a = args_of(p);
+    if (int rc = bwd(dtype, p->dh, a, Where{nullptr, true})) return rc;
     const size_t need = ws_bytes(a, p->dh, true);
     DIC_REQUIRE(need == 0 || (p->ws && aligned(p->ws) && p->ws_bytes >= need), "dic_win_attn_bwd: workspace missing or too small (dic_win_attn_ws_bytes)");
     a.stats = (float*)p->ws;
     a.sinks_ws = a.stats + stats_floats(p->N, p->H, p->Tq);
-    hipStream_t st = (hipStream_t)stream;
-    if (dtype == DIC_BF16) return p->dh == 64 ? bwd<bf16_t, 64>(a, st) : bwd<bf16_t, 128>(a, st);
-    return p->dh == 64 ? bwd<float, 64>(a, st) : bwd<float, 128>(a, st);
+    return bwd(dtype, p->dh, a, Where{(hipStream_t)stream, false});
 }

@@ -99,6 +99,27 @@ def test_attention_refuses_other_types_and_missing_workspaces():
     assert L.dic_win_attn_ws_bytes(1, 1, C.byref(attn(dh=65))) == 0
 
 
+MORE_THAN_ONE_LAUNCH = [
+    dict(N=1 << 26, H=1, Hkv=1, Tq=1, Tk=1),                                  # a workgroup of 64 threads for each row: 2^32 threads
+    dict(N=1 << 25, H=2, Hkv=2, Tq=32, Tk=40), dict(N=1 << 24, H=4, Hkv=1, Tq=32, Tk=40), dict(N=3 << 22, H=2, Hkv=2, Tq=128, Tk=128),
+    dict(N=1 << 30, H=1 << 30, Hkv=1, Tq=15 * 32, Tk=1),                      # 2^64 tiles: the product passes 64 bits
+    dict(N=1 << 30, H=1 << 30, Hkv=1 << 30, Tq=1, Tk=15 * 32),
+]
+
+
+@pytest.mark.parametrize("kw", MORE_THAN_ONE_LAUNCH, ids=str)
+@pytest.mark.parametrize("dtype", [0, 1])
+def test_attention_refuses_what_no_launch_holds_in_front_of_any(dtype, kw):
+    L, p = dic.lib(), attn(**kw)
+    assert L.dic_win_attn_fwd(dtype, C.byref(p), None) == 1001 and L.dic_last_error().endswith(b"for one launch")
+    assert L.dic_win_attn_bwd(dtype, C.byref(p), None) == 1001 and L.dic_last_error().endswith(b"for one launch")
+
+
+def test_attention_refuses_too_many_workgroups_of_the_few_rows_form():
+    L, p = dic.lib(), attn(N=1 << 24, H=8, Hkv=1, Tq=2, Tk=65)                # four waves each (two in fp32 at dh 128)
+    assert L.dic_win_attn_fwd(1, C.byref(p), None) == 1001 and L.dic_last_error().endswith(b"for one launch")
+
+
 def norms(**kw):
     p = dic._lib.GatedNormParams()
     base = dict(rows=8, rows_per_gate=4, D=96, residual_scale=1.0, post_kind=1, pre_kind=2, post_eps=1e-6, pre_eps=1e-6, ws=4096, ws_bytes=1 << 20)
