@@ -1174,10 +1174,81 @@ bool fits(const DicStrides& d, int N, int T, int H, int size) {
     // 16-byte rows, and 64 rows of a tile inside a descriptor's 31-bit range
     const Strides s = st(d, N, T, H);
     const int per = 16 / size;
-    return s.n % per == 0 && s.t % per == 0 && s.h % per == 0 && s.n >= 0 && s.t >= 0 && s.h >= 0 && s.t <= (1ll << 24) / size;
+    constexpr long long MOST = 1ll << 52;                        // elements that a dimension spans (what the sums of offsets are sure to hold)
+    return s.n % per == 0 && s.t % per == 0 && s.h % per == 0 && s.n >= 0 && s.t >= 0 && s.h >= 0 && s.t <= (1ll << 24) / size
+           && s.n <= MOST / (N > 0 ? N : 1) && s.h <= MOST / (H > 0 ? H : 1);
 }
 bool apart(const DicStrides& s, int N, int T, int H, int dh) { return (N <= 1 || s.n >= dh) && (T <= 1 || s.t >= dh) && (H <= 1 || s.h >= dh); }
 bool aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+// The bytes of an argument: rows of w at p + v_0 s_0 + v_1 s_1 + v_2 s_2 with 0 <= v_i < n_i (as far as n_i > 1).
+struct Area { const char* p; long long s[3], n[3], w; };
+struct Term { long long s, lo, hi; };                            // v s with lo <= v <= hi, s > 0
+enum { NO = 0, YES = 1, UNTOLD = 2 };
+// Can a sum of the terms, sorted by falling s, lie in [from, to]?  Depth first, over the values that the smaller terms can still make up for: where a stride
+// spans what lies inside of it, one to three for each term.  Interleaved layouts of other orders take more, and are given up on after `steps` sums.
+int reaches(const Term* t, int count, long long from, long long to, int& steps) {
+    if (count == 0) return from <= 0 && to >= 0 ? YES : NO;
+    long long lo = 0, hi = 0;                                    // of the terms behind this one
+    for (int i = 1; i < count; ++i) { lo += t[i].lo * t[i].s; hi += t[i].hi * t[i].s; }
+    auto down = [](long long a, long long b) { return a >= 0 ? a / b : -((-a + b - 1) / b); };
+    const long long v0 = -down(hi - from, t->s), v1 = down(to - lo, t->s);
+    for (long long v = v0 > t->lo ? v0 : t->lo; v <= (v1 < t->hi ? v1 : t->hi); ++v) {
+        if (--steps < 0) return UNTOLD;
+        if (int r = reaches(t + 1, count - 1, from - v * t->s, to - v * t->s, steps)) return r;
+    }
+    return NO;
+}
+long long extent(const Area& a) { return (a.n[0] - 1) * a.s[0] + (a.n[1] - 1) * a.s[1] + (a.n[2] - 1) * a.s[2] + a.w; }
+int overlap(const Area& a, const Area& b) {
+    if (!a.p || !b.p || a.n[0] * a.n[1] * a.n[2] * a.w == 0 || b.n[0] * b.n[1] * b.n[2] * b.w == 0) return NO;
+    if (a.p + extent(a) <= b.p || b.p + extent(b) <= a.p) return NO;
+    Term t[6];
+    int count = 0;
+    auto add = [&](long long s, long long lo, long long hi) {
+        if (s == 0 || lo == hi) return;
+        int i = 0;
+        while (i < count && t[i].s > s) ++i;
+        if (i < count && t[i].s == s) { t[i].lo += lo; t[i].hi += hi; return; }
+        for (int k = count++; k > i; --k) t[k] = t[k - 1];
+        t[i] = Term{s, lo, hi};
+    };
+    for (int i = 0; i < 3; ++i) { add(a.s[i], 0, a.n[i] - 1); add(b.s[i], 1 - b.n[i], 0); }
+    // a row of a begins less than b.w behind and less than a.w in front of one of b
+    const long long d = b.p - a.p;
+    int steps = 1 << 16;
+    return reaches(t, count, d - a.w + 1, d + b.w - 1, steps);
+}
+int check_areas(const DicWinAttnParams* p, int size, bool bwd, size_t ws) {
+    auto rows = [&](const void* at, const DicStrides& d, int T, int H) {
+        const Strides s = st(d, p->N, T, H);
+        return Area{(const char*)at, {s.n * size, s.t * size, s.h * size}, {p->N, T, H}, (long long)p->dh * size};
+    };
+    auto flat = [](const void* at, long long bytes) { return Area{(const char*)at, {0, 0, 0}, {1, 1, 1}, bytes}; };
+    const Area q = rows(p->q, p->q_stride, p->Tq, p->H), k = rows(p->k, p->k_stride, p->Tk, p->Hkv), v = rows(p->v, p->v_stride, p->Tk, p->Hkv);
+    const Area out = rows(p->out, p->out_stride, p->Tq, p->H), lse = flat(p->lse, 4ll * p->N * p->H * p->Tq), work = flat(p->ws, (long long)ws);
+    const Area mask = flat(p->key_mask, (long long)p->N * p->Tk), len = flat(p->kv_len, 4ll * p->N), pos = flat(p->q_pos, 4ll * p->N);
+    Area in[8] = {q, k, v, mask, len, pos}, written[4] = {out, lse, work};
+    int ni = 6, nw = 3;
+    if (bwd) {
+        in[ni++] = out; in[ni++] = lse;
+        written[0] = work;
+        written[1] = rows(p->dq, p->dq_stride, p->Tq, p->H); written[2] = rows(p->dk, p->dk_stride, p->Tk, p->Hkv); written[3] = rows(p->dv, p->dv_stride, p->Tk, p->Hkv);
+        nw = 4;
+    }
+    const Area dout = rows(bwd ? p->dout : nullptr, p->dout_stride, p->Tq, p->H);
+    auto apart = [](int r) {
+        DIC_REQUIRE(r != YES, "dic_win_attn: an output overlaps an input or another output");
+        DIC_REQUIRE(r == NO, "dic_win_attn: an output and an input or another output share memory with strides that leave open whether they overlap");
+        return 0;
+    };
+    for (int i = 0; i < nw; ++i) {
+        for (int j = 0; j < ni; ++j) if (int rc = apart(overlap(written[i], in[j]))) return rc;
+        if (int rc = apart(overlap(written[i], dout))) return rc;
+        for (int j = 0; j < i; ++j) if (int rc = apart(overlap(written[i], written[j]))) return rc;
+    }
+    return 0;
+}
 
 int check(int dtype, const DicWinAttnParams* p, bool bwd, bool pointers = true) {
     DIC_REQUIRE(p != nullptr, "dic_win_attn: no parameters");
@@ -1390,6 +1461,7 @@ extern "C" int dic_win_attn_fwd(int dtype, const DicWinAttnParams* p, void* stre
     WinArgs a = args_of(p);
     if (int rc = fwd(dtype, p->dh, a, Where{nullptr, true})) return rc;
     const size_t need = ws_bytes(a, p->dh, false);
+    if (int rc = check_areas(p, dtype == DIC_BF16 ? 2 : 4, false, need)) return rc;
     DIC_REQUIRE(need == 0 || (p->ws && aligned(p->ws) && p->ws_bytes >= need), "dic_win_attn_fwd: workspace missing or too small (dic_win_attn_ws_bytes)");
     a.parts = (float*)p->ws;
     return fwd(dtype, p->dh, a, Where{(hipStream_t)stream, false});
@@ -1401,6 +1473,7 @@ extern "C" int dic_win_attn_bwd(int dtype, const DicWinAttnParams* p, void* stre
     WinArgs a = args_of(p);
     if (int rc = bwd(dtype, p->dh, a, Where{nullptr, true})) return rc;
     const size_t need = ws_bytes(a, p->dh, true);
+    if (int rc = check_areas(p, dtype == DIC_BF16 ? 2 : 4, true, need)) return rc;
     DIC_REQUIRE(need == 0 || (p->ws && aligned(p->ws) && p->ws_bytes >= need), "dic_win_attn_bwd: workspace missing or too small (dic_win_attn_ws_bytes)");
     a.stats = (float*)p->ws;
     a.sinks_ws = a.stats + stats_floats(p->N, p->H, p->Tq);

@@ -300,7 +300,7 @@ int dic_attn_bwd(int dtype, const void* qkv, const uint8_t* key_mask, const void
  *     result, whatever its rows of k and v hold.  (A row of q, k, v or dout that takes part and is not finite may reach results of other rows near it.)
  *     Sums, maxima and lse are fp32; with DIC_BF16 the probabilities are rounded to bf16 in front of the product with v.
  * bwd: dq, dk, dv from dout and the forward's out and lse; every row is written (zeros where nothing is seen).  Deterministic, no atomics.
- * No output may lie in place of an input or of another output.  kv_len is read as clamped to [0, Tk], q_pos to +-2^29 (bounds act as given beside it).  ws: dic_win_attn_ws_bytes(dtype, backward, p) bytes, 16-byte aligned, private to the call
+ * No output (lse and ws are ones) may overlap an input or another output; rows of one packed tensor may lie between each other's.  kv_len is read as clamped to [0, Tk], q_pos to +-2^29 (bounds act as given beside it).  ws: dic_win_attn_ws_bytes(dtype, backward, p) bytes, 16-byte aligned, private to the call
  * until it has run; N, Tq or Tk may be 0.  A call is refused in front of any launch if one of its grids would need 2^32 threads (64 a wave for 32 rows of a head).   */
 typedef struct DicStrides { int64_t n, t, h; } DicStrides;            /* elements between sequences, tokens, heads */
 typedef struct DicWinAttnParams {

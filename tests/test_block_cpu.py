@@ -120,6 +120,83 @@ def test_attention_refuses_too_many_workgroups_of_the_few_rows_form():
     assert L.dic_win_attn_fwd(1, C.byref(p), None) == 1001 and L.dic_last_error().endswith(b"for one launch")
 
 
+def apart(**kw):
+    """Far from each other unless `kw` moves one; without a workspace, so that no call gets as far as a launch."""
+    return attn(**{**{n: 1 << 20 << i for i, n in enumerate(("q", "k", "v", "out", "lse", "dout", "dq", "dk", "dv"))}, "ws": None, **kw})
+
+
+def told(p):
+    assert dic.lib().dic_win_attn_bwd(1, C.byref(p), None) == 1001
+    return dic.lib().dic_last_error()
+
+
+def test_attention_refuses_outputs_that_overlap_in_part():
+    at = {n: getattr(apart(), n) for n in ("q", "k", "v", "out", "lse", "dout", "dq", "dk", "dv")}
+    assert b"workspace" in told(apart())
+    row, flat = 256 * 2, 4 * 2 * 4 * 8                                        # bytes of a token row of q, of lse
+    for y in ("dq", "dk", "dv"):
+        size = 2 * 8 * (row if y == "dq" else row // 2)
+        for x in ("q", "k", "v", "out", "dout"):
+            other = 2 * 8 * (row if x in ("q", "out", "dout") else row // 2)
+            assert b"overlaps" in told(apart(**{y: at[x] + other - 16})) and b"overlaps" in told(apart(**{y: at[x] - size + 16})), (y, x)
+            assert b"workspace" in told(apart(**{y: at[x] + other})) and b"workspace" in told(apart(**{y: at[x] - size})), (y, x)
+        assert b"overlaps" in told(apart(**{y: at["lse"] + flat - 16})) and b"workspace" in told(apart(**{y: at["lse"] + flat}))
+        for n, bytes_ in (("key_mask", 16), ("kv_len", 8), ("q_pos", 8)):
+            assert b"overlaps" in told(apart(**{n: at[y] + 16})) and b"workspace" in told(apart(**{n: at[y] - bytes_}))
+        for z in ("dq", "dk", "dv"):
+            if z != y:
+                assert b"overlaps" in told(apart(**{y: at[z] + 16}))
+    p = apart(ws=at["dq"] + 2 * 8 * row - 16, ws_bytes=1 << 20)
+    assert b"overlaps" in told(p)
+    L = dic.lib()
+    for kw in (dict(out=at["q"] + 16), dict(out=at["v"] - 16), dict(lse=at["out"] + 64), dict(lse=at["k"]), dict(key_mask=at["out"] + 8)):
+        assert L.dic_win_attn_fwd(1, C.byref(apart(**kw)), None) == 1001 and b"overlaps" in L.dic_last_error(), kw
+
+
+def test_attention_takes_outputs_that_lie_between_each_other():
+    """Views of one packed tensor [N, T, heads, dh], of its transposed form, and of caches of which a call reads every other sequence."""
+    for n, t, h in ((8 * 512, 512, 64), (8 * 512, 64, 8 * 64)):
+        kw = {f"{x}_stride_{d}": v for x in ("dq", "dk", "dv") for d, v in (("n", n), ("t", t), ("h", h))}
+        at = 1 << 30
+        assert b"workspace" in told(apart(dq=at, dk=at + 2 * (4 * h), dv=at + 2 * (6 * h), **kw))
+        assert b"overlaps" in told(apart(dq=at, dk=at + 2 * (4 * h) - 16, dv=at + 2 * (6 * h), **kw))
+        assert b"overlaps" in told(apart(dq=at, dk=at + 2 * (3 * h), dv=at + 2 * (6 * h), **kw))
+    k = {f"k_stride_{d}": v for d, v in (("n", 2 * 8 * 128), ("t", 128), ("h", 64))}
+    dk = {f"dk_stride_{d}": v for d, v in (("n", 2 * 8 * 128), ("t", 128), ("h", 64))}
+    assert b"workspace" in told(apart(k=1 << 30, dk=(1 << 30) + 2 * 8 * 128, **k, **dk))
+    assert b"overlaps" in told(apart(k=1 << 30, dk=(1 << 30) + 2 * 7 * 128, **k, **dk))
+
+
+def test_overlaps_of_small_layouts_are_told_exactly():
+    """Random strides, compared with the rows counted out."""
+    import itertools
+    import random
+    rng, seen = random.Random(5), {True: 0, False: 0}
+    for _ in range(1500):
+        N, T, H = rng.randint(1, 4), rng.randint(1, 5), rng.randint(1, 4)
+        a, b = ([8 * rng.randint(0 if which else 8, rng.choice((9, 20, 60, 200))) for _ in range(3)] for which in (0, 1))
+        if a[0] == a[1] or a[1] == a[2] or a[0] == a[2]:                       # (an output's own rows are another matter)
+            continue
+        at = 1 << 30, (1 << 30) + 16 * rng.randint(-300, 300)
+        starts = [{p + 2 * (n * s[0] + t * s[1] + h * s[2]) for n, t, h in itertools.product(range(N), range(T), range(H))} for p, s in zip(at, (a, b))]
+        want = any(abs(x - y) < 128 for x in starts[0] for y in starts[1])
+        kw = {f"{n}_stride_{d}": s[i] for n, s in (("dq", a), ("q", b), *((n, (64 * T * H, 64 * H, 64)) for n in ("k", "v", "dk", "dv")))
+              for i, d in enumerate("nth")}
+        got = told(apart(N=N, Tq=T, Tk=T, H=H, Hkv=H, q=at[1], dq=at[0], out=1 << 40, dout=1 << 41, lse=1 << 42, dk=1 << 43, dv=1 << 44, k=1 << 45, v=1 << 46, **kw))
+        if at[0] == at[1]:
+            continue
+        if b"rows of an output overlap" in got:
+            continue
+        assert (b"overlaps an input" in got) == want and (b"workspace" in got) == (not want), (N, T, H, a, b, at)
+        seen[want] += 1
+    assert min(seen.values()) > 100
+
+
+def test_strides_beyond_the_address_space_are_refused():
+    for kw in (dict(q_stride_n=1 << 60), dict(k_stride_h=1 << 55), dict(dv_stride_n=1 << 62)):
+        assert b"strides" in told(apart(**kw)), kw
+
+
 def norms(**kw):
     p = dic._lib.GatedNormParams()
     base = dict(rows=8, rows_per_gate=4, D=96, residual_scale=1.0, post_kind=1, pre_kind=2, post_eps=1e-6, pre_eps=1e-6, ws=4096, ws_bytes=1 << 20)
