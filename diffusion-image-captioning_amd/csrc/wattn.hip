@@ -1178,7 +1178,6 @@ bool fits(const DicStrides& d, int N, int T, int H, int size) {
     return s.n % per == 0 && s.t % per == 0 && s.h % per == 0 && s.n >= 0 && s.t >= 0 && s.h >= 0 && s.t <= (1ll << 24) / size
            && s.n <= MOST / (N > 0 ? N : 1) && s.h <= MOST / (H > 0 ? H : 1);
 }
-bool apart(const DicStrides& s, int N, int T, int H, int dh) { return (N <= 1 || s.n >= dh) && (T <= 1 || s.t >= dh) && (H <= 1 || s.h >= dh); }
 bool aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 // The bytes of an argument: rows of w at p + v_0 s_0 + v_1 s_1 + v_2 s_2 with 0 <= v_i < n_i (as far as n_i > 1).
@@ -1218,6 +1217,29 @@ int overlap(const Area& a, const Area& b) {
     const long long d = b.p - a.p;
     int steps = 1 << 16;
     return reaches(t, count, d - a.w + 1, d + b.w - 1, steps);
+}
+// Are an output's rows of dh elements apart from each other?
+bool apart(const DicStrides& d, int N, int T, int H, int dh) {
+    if (N == 0 || T == 0 || H == 0) return true;
+    const long long s[3] = {d.n, d.t, d.h}, n[3] = {N, T, H};
+    Term t[3];
+    int count = 0;
+    for (int i = 0; i < 3; ++i) {
+        if (n[i] <= 1) continue;
+        int k = count++;
+        for (; k > 0 && t[k - 1].s < s[i]; --k) t[k] = t[k - 1];
+        t[k] = Term{s[i], 1 - n[i], n[i] - 1};
+        if (s[i] < dh || (k > 0 && t[k - 1].s == s[i])) return false;
+    }
+    for (int i = 0; i < count; ++i) {                            // two rows that differ in t[i] first: either way round, so forwards
+        long long inside = dh;
+        for (int k = i + 1; k < count; ++k) inside += t[k].hi * t[k].s;
+        int steps = 1 << 16;
+        t[i].lo = 1;
+        if (t[i].s < inside && reaches(t + i, count - i, 1 - dh, dh - 1, steps) != NO) return false;
+        t[i].lo = -t[i].hi;
+    }
+    return true;
 }
 int check_areas(const DicWinAttnParams* p, int size, bool bwd, size_t ws) {
     auto rows = [&](const void* at, const DicStrides& d, int T, int H) {

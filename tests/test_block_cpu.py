@@ -107,16 +107,23 @@ MORE_THAN_ONE_LAUNCH = [
 ]
 
 
+def packed(N, Tq, Tk, H, Hkv):
+    """Sizes with the strides of contiguous tensors."""
+    strides = {f"{x}_stride_{d}": v for names, t, h in ((("q", "out", "dout", "dq"), Tq, H), (("k", "v", "dk", "dv"), Tk, Hkv)) for x in names
+               for d, v in (("n", 64 * t * h), ("t", 64 * h), ("h", 64))}
+    return attn(N=N, Tq=Tq, Tk=Tk, H=H, Hkv=Hkv, **strides)
+
+
 @pytest.mark.parametrize("kw", MORE_THAN_ONE_LAUNCH, ids=str)
 @pytest.mark.parametrize("dtype", [0, 1])
 def test_attention_refuses_what_no_launch_holds_in_front_of_any(dtype, kw):
-    L, p = dic.lib(), attn(**kw)
+    L, p = dic.lib(), packed(**kw)
     assert L.dic_win_attn_fwd(dtype, C.byref(p), None) == 1001 and L.dic_last_error().endswith(b"for one launch")
     assert L.dic_win_attn_bwd(dtype, C.byref(p), None) == 1001 and L.dic_last_error().endswith(b"for one launch")
 
 
 def test_attention_refuses_too_many_workgroups_of_the_few_rows_form():
-    L, p = dic.lib(), attn(N=1 << 24, H=8, Hkv=1, Tq=2, Tk=65)                # four waves each (two in fp32 at dh 128)
+    L, p = dic.lib(), packed(N=1 << 24, H=8, Hkv=1, Tq=2, Tk=65)                # four waves each (two in fp32 at dh 128)
     assert L.dic_win_attn_fwd(1, C.byref(p), None) == 1001 and L.dic_last_error().endswith(b"for one launch")
 
 
@@ -190,6 +197,26 @@ def test_overlaps_of_small_layouts_are_told_exactly():
         assert (b"overlaps an input" in got) == want and (b"workspace" in got) == (not want), (N, T, H, a, b, at)
         seen[want] += 1
     assert min(seen.values()) > 100
+
+
+def test_an_output_whose_rows_overlap_is_refused():
+    """Every stride at least a row long, and yet: two strides the same, or one that another's steps reach.  Random ones, compared with the rows counted out."""
+    import itertools
+    import random
+    for s in ((4096, 64, 64), (64, 256, 64), (4096, 192, 128), (1984, 1000, 64)):
+        p = apart(N=2, Tq=8, H=4, **{f"dq_stride_{d}": v for d, v in zip("nth", s)})
+        assert b"rows of an output overlap" in told(p), s
+    rng, seen = random.Random(6), {True: 0, False: 0}
+    for _ in range(3000):
+        N, T, H = rng.randint(1, 4), rng.randint(1, 5), rng.randint(1, 4)
+        s = [8 * rng.randint(8, rng.choice((9, 20, 60, 200))) for _ in range(3)]
+        starts = [n * s[0] + t * s[1] + h * s[2] for n, t, h in itertools.product(range(N), range(T), range(H))]
+        want = any(abs(x - y) < 64 for x, y in itertools.combinations(starts, 2))
+        kw = {f"{n}_stride_{d}": st[i] for n, st in (("dq", s), *((n, (64 * T * H, 64 * H, 64)) for n in ("q", "k", "v", "out", "dout", "dk", "dv"))) for i, d in enumerate("nth")}
+        got = told(apart(N=N, Tq=T, Tk=T, H=H, Hkv=H, **kw))
+        assert (b"rows of an output overlap" in got) == want and (b"workspace" in got) == (not want), (N, T, H, s)
+        seen[want] += 1
+    assert min(seen.values()) > 300
 
 
 def test_strides_beyond_the_address_space_are_refused():
