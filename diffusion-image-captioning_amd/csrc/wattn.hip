@@ -1279,7 +1279,7 @@ int check(int dtype, const DicWinAttnParams* p, bool bwd, bool pointers = true) 
     DIC_REQUIRE(p->dh == 64 || p->dh == 128, "dic_win_attn: head dim must be 64 or 128");
     DIC_REQUIRE(p->N >= 0 && p->Tq >= 0 && p->Tk >= 0 && p->Tq <= (1 << 28) && p->Tk <= (1 << 28), "dic_win_attn: sizes out of range");
     DIC_REQUIRE(p->H > 0 && p->Hkv > 0 && p->H % p->Hkv == 0, "dic_win_attn: the number of heads must be a multiple of the number of key heads");
-    DIC_REQUIRE(p->sinks >= 0 && std::isfinite(p->scale) && p->scale > 0.f, "dic_win_attn: sinks >= 0 and a positive finite scale are needed");
+    DIC_REQUIRE(p->sinks >= 0 && std::isfinite(p->scale * LOG2E) && p->scale > 0.f, "dic_win_attn: sinks >= 0 and a positive scale, finite times log2(e), are needed");
     const long long heads = (long long)p->N * p->H, most = 1ll << 31;          // (heads >= N Hkv; bounded by itself first, as three factors may pass 64 bits)
     DIC_REQUIRE(heads < most && heads * (p->Tq / 32 + 1) < most && (long long)p->N * p->Hkv * (p->Tk / 32 + 1) < most, "dic_win_attn: too many tiles for one launch");
     if (!pointers) return 0;

@@ -315,7 +315,7 @@ typedef struct DicWinAttnParams {
     const int32_t* q_pos;       /* [N] or NULL */
     int N, Tq, Tk, H, Hkv, dh;
     int left, right, sinks;
-    float scale;                /* > 0 */
+    float scale;                /* > 0; scale log2(e) and, for every pair, scale log2(e) q . k finite in fp32 */
     void* ws; size_t ws_bytes;
 } DicWinAttnParams;
 size_t dic_win_attn_ws_bytes(int dtype, int backward, const DicWinAttnParams* p);

@@ -224,6 +224,12 @@ def test_strides_beyond_the_address_space_are_refused():
         assert b"strides" in told(apart(**kw)), kw
 
 
+def test_attention_refuses_a_scale_that_is_infinite_times_log2_e():
+    """The kernels' exponentials are powers of two: 2.5e38 log2(e) is infinite, and 0 times that no logit."""
+    for entry in (dic.lib().dic_win_attn_fwd, dic.lib().dic_win_attn_bwd):
+        assert entry(1, C.byref(attn(scale=2.5e38)), None) == 1001 and b"scale" in dic.lib().dic_last_error()
+
+
 def norms(**kw):
     p = dic._lib.GatedNormParams()
     base = dict(rows=8, rows_per_gate=4, D=96, residual_scale=1.0, post_kind=1, pre_kind=2, post_eps=1e-6, pre_eps=1e-6, ws=4096, ws_bytes=1 << 20)
