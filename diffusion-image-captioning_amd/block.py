@@ -18,6 +18,7 @@ _DTYPES = {torch.float32: _lib.DIC_F32, torch.bfloat16: _lib.DIC_BF16}
 _RES_F32 = 0x200
 _KINDS = {"layer": 1, "rms": 2}
 _FAR = 2 ** 31 - 1
+_FLT_MAX = 3.4028234663852886e38
 # The parameter structs as bytes: packing one takes a fifth of the time of filling its ctypes mirror, and a call on one caption is all host time.
 _WIN = struct.Struct("9P24q3P9if2P")
 _NORM = struct.Struct("17Pif2Pif2qif2P")
@@ -65,8 +66,16 @@ def _on(t, like, name, dtypes, shape=None):
     raise ValueError(f"{name} asks for a gradient: this package has no autograd, call the operator's _grad function on detached tensors")
 
 
+def _unfit(e):
+    """For what came up while the arguments were packed: sizes beyond 32 bits, and tensors that are sparse or inside a function transform."""
+    return ValueError(f"a size that does not fit: {e}") if isinstance(e, struct.error) else TypeError(f"a tensor without memory of its own: {e}")
+
+
 def _ptr(t):
-    return 0 if t is None else t.data_ptr()
+    try:
+        return 0 if t is None else t.data_ptr()
+    except RuntimeError as e:
+        raise _unfit(e) from None
 
 
 def _first(t, name):
@@ -80,13 +89,34 @@ def _first(t, name):
         raise TypeError(f"{name}: {t.dtype} where torch.float32 or torch.bfloat16 is needed")
 
 
+def _number(x, name):
+    """x as a float that fp32 holds.  A tensor on the GPU would be waited for, and is refused."""
+    if type(x) is not float:
+        if isinstance(x, torch.Tensor) and (x.device.type != "cpu" or x.requires_grad or x.numel() != 1) or isinstance(x, (str, bytes)):
+            raise TypeError(f"{name} must be a number")
+        try:
+            x = float(x)
+        except OverflowError:
+            raise ValueError(f"{name} must fit fp32") from None
+        except (TypeError, ValueError, RuntimeError):
+            raise TypeError(f"{name} must be a number") from None
+    if not -_FLT_MAX <= x <= _FLT_MAX:
+        raise ValueError(f"{name} must be finite and fit fp32")
+    return x
+
+
 # ------------------------------------------------------------------------------------------------ attention
 def _bound(x, name):
     if x is None:
         return -1
+    if type(x) is not int:
+        value = _number(x, name)
+        if value != int(value):
+            raise ValueError(f"{name} must be a whole number")
+        x = int(value)
     if x < 0:
         raise ValueError(f"{name} must be None (no bound) or at least 0")
-    return min(int(x), _FAR)
+    return min(x, _FAR)
 
 
 def _check_rows(t, like, name, shape):
@@ -131,10 +161,10 @@ def _attention(q, k, v, left, right, sinks, key_mask, kv_len, q_pos, scale):
             _on(x, q, name, (torch.int32,), (N,))
             if not x.is_contiguous():
                 raise ValueError(f"{name} must be contiguous")
-    scale = dh ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < 3e38:
-        raise ValueError("scale must be positive and finite")
-    return (*sq[:3], *sk[:3], *sv[:3]), (_ptr(key_mask), _ptr(kv_len), _ptr(q_pos), N, Tq, Tk, H, Hkv, dh, _bound(left, "left"), _bound(right, "right"), _bound(sinks or 0, "sinks"), scale), code
+    scale = (dh or 1) ** -0.5 if scale is None else _number(scale, "scale")
+    if not scale > 0.0:
+        raise ValueError("scale must be positive")
+    return (*sq[:3], *sk[:3], *sv[:3]), (_ptr(key_mask), _ptr(kv_len), _ptr(q_pos), N, Tq, Tk, H, Hkv, dh, _bound(left, "left"), _bound(right, "right"), _bound(0 if sinks is None else sinks, "sinks"), scale), code
 
 
 _NO_STRIDES = (0,) * 12
@@ -155,8 +185,12 @@ def window_attention(q, k, v, *, left=None, right=None, sinks=0, key_mask=None, 
     else:
         _check_rows(out, q, "out", q.shape)
     lse = q.new_empty((tail[3], tail[6], tail[4]), dtype=torch.float32)
-    fields = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), 0, 0, 0, 0, *strides, *out.stride()[:3], *_NO_STRIDES, *tail)
-    size = _fn("dic_win_attn_ws_bytes")(code, 0, _WIN.pack(*fields, 0, 0))
+    ws_bytes = _fn("dic_win_attn_ws_bytes")
+    try:
+        fields = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), 0, 0, 0, 0, *strides, *out.stride()[:3], *_NO_STRIDES, *tail)
+        size = ws_bytes(code, 0, _WIN.pack(*fields, 0, 0))
+    except (RuntimeError, struct.error) as e:
+        raise _unfit(e) from None
     ws = q.new_empty(size, dtype=torch.uint8) if size else None
     _launch("dic_win_attn_fwd", code, _WIN.pack(*fields, _ptr(ws), size), q.device)
     return out, lse
@@ -172,7 +206,9 @@ def window_attention_grad(dout, q, k, v, out, lse, *, left=None, right=None, sin
     if not lse.is_contiguous():
         raise ValueError("lse must be contiguous")
     per = 16 // q.element_size()
-    if not dout.is_contiguous() and (dout.stride(3) != 1 or any(s % per for s in dout.stride()[:3])) or dout.data_ptr() % 16:
+    if not dout.is_contiguous() and (dout.stride(3) != 1 or any(s % per for s in dout.stride()[:3])) or _ptr(dout) % 16:
+        if dout.layout is not torch.strided:
+            raise TypeError("dout must be a dense tensor")
         dout = dout.clone(memory_format=torch.contiguous_format)                 # an expanded or transposed gradient
     if grads is None:
         dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
@@ -180,9 +216,13 @@ def window_attention_grad(dout, q, k, v, out, lse, *, left=None, right=None, sin
         dq, dk, dv = grads
         for t, like, name in ((dq, q, "dq"), (dk, k, "dk"), (dv, k, "dv")):
             _check_rows(t, q, name, like.shape)
-    fields = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-              *strides, *out.stride()[:3], *dout.stride()[:3], *dq.stride()[:3], *dk.stride()[:3], *dv.stride()[:3], *tail)
-    size = _fn("dic_win_attn_ws_bytes")(code, 1, _WIN.pack(*fields, 0, 0))
+    ws_bytes = _fn("dic_win_attn_ws_bytes")
+    try:
+        fields = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                  *strides, *out.stride()[:3], *dout.stride()[:3], *dq.stride()[:3], *dk.stride()[:3], *dv.stride()[:3], *tail)
+        size = ws_bytes(code, 1, _WIN.pack(*fields, 0, 0))
+    except (RuntimeError, struct.error) as e:
+        raise _unfit(e) from None
     ws = q.new_empty(size, dtype=torch.uint8) if size else None
     _launch("dic_win_attn_bwd", code, _WIN.pack(*fields, _ptr(ws), size), q.device)
     return dq, dk, dv
@@ -197,19 +237,23 @@ class NormParams(NamedTuple):
     eps: float = 1e-12
 
 
-_WEIGHT, _BIAS = {"post": "post weight", "pre": "pre weight"}, {"post": "post bias", "pre": "pre bias"}
+_WEIGHT, _BIAS, _EPS = ({side: f"{side} {what}" for side in ("post", "pre")} for what in ("weight", "bias", "eps"))
 
 
 def _norm(norm, like, D, side):
     """The packed fields of one norm."""
     if norm is None:
         return 0, 0, 0, 0.0
-    if norm.kind not in _KINDS:
+    try:
+        kind, weight, bias, eps = norm.kind, norm.weight, norm.bias, norm.eps
+    except AttributeError:
+        raise TypeError(f"{side} must be NormParams or None") from None
+    if kind not in _KINDS:
         raise ValueError(f'{side}: a norm is "layer" or "rms"')
-    for t, name in ((norm.weight, _WEIGHT[side]), (norm.bias, _BIAS[side])):
+    for t, name in ((weight, _WEIGHT[side]), (bias, _BIAS[side])):
         if t is not None:
             _packed(t, like, name, torch.float32, (D,))
-    return _ptr(norm.weight), _ptr(norm.bias), _KINDS[norm.kind], norm.eps
+    return _ptr(weight), _ptr(bias), _KINDS[kind], _number(eps, _EPS[side])
 
 
 def _shapes(x, gate):
@@ -233,7 +277,7 @@ def _packed(t, like, name, dtype, shape):
     try:                                                             # (the whole check in one expression: a call on one caption's rows is all host time)
         if t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.get_device() == like.get_device() and not (t.requires_grad and torch.is_grad_enabled()):
             return
-    except AttributeError:
+    except (AttributeError, RuntimeError):
         pass
     _on(t, like, name, (dtype,), shape)
     raise ValueError(f"{name} must be contiguous")
@@ -263,13 +307,18 @@ def gated_norm(x, y=None, *, post=None, gate=None, residual_scale=1.0, pre=None,
     else:
         if not (post is None and gate is None and pre is not None):
             raise ValueError("without y there is a pre norm and nothing else")
+    residual_scale = _number(residual_scale, "residual_scale")
     rows, D, per_gate = _shapes(x, gate)
     sides = *_norm(post, x, D, "post"), *_norm(pre, x, D, "pre")
     x_new = x if y is None and residual_scale == 1.0 else torch.empty_like(x)
     a = None if pre is None else torch.empty_like(x if y is None else y, dtype=inner)
     saved = x.new_empty((4, rows), dtype=torch.float32)
-    _launch("dic_gated_norm_fwd", code, _NORM.pack(x.data_ptr(), _ptr(y), 0 if x_new is x else x_new.data_ptr(), _ptr(a), _ptr(gate), saved.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, 0,
-                                                   *sides, rows, per_gate, D, residual_scale, 0, 0), x.device)
+    try:
+        params = _NORM.pack(x.data_ptr(), _ptr(y), 0 if x_new is x else x_new.data_ptr(), _ptr(a), _ptr(gate), saved.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, 0,
+                            *sides, rows, per_gate, D, residual_scale, 0, 0)
+    except (RuntimeError, struct.error) as e:
+        raise _unfit(e) from None
+    _launch("dic_gated_norm_fwd", code, params, x.device)
     return x_new, a, saved
 
 
@@ -295,6 +344,7 @@ def gated_norm_grad(dx_new, da, x_new, y, saved, *, post=None, gate=None, residu
     else:
         if not (post is None and gate is None and pre is not None):
             raise ValueError("without y there is a pre norm and nothing else")
+    residual_scale = _number(residual_scale, "residual_scale")
     rows, D, per_gate = _shapes(x_new, gate)
     sides = *_norm(post, x_new, D, "post"), *_norm(pre, x_new, D, "pre")
     _packed(saved, x_new, "saved", torch.float32, (4, rows))
@@ -307,7 +357,7 @@ def gated_norm_grad(dx_new, da, x_new, y, saved, *, post=None, gate=None, residu
              for name, t in ((side + "_weight", norm.weight), (side + "_bias", norm.bias)) if t is not None]
     if names:
         got.update(zip(names, x_new.new_empty((len(names), D), dtype=torch.float32).unbind(0)))      # (one allocation)
-    fields = (0, _ptr(y), x_new.data_ptr(), 0, _ptr(gate), saved.data_ptr(), _ptr(dx_new), _ptr(da), got["dx"].data_ptr(), _ptr(got.get("dy")), _ptr(got.get("gate")),
+    fields = (0, _ptr(y), _ptr(x_new), 0, _ptr(gate), _ptr(saved), _ptr(dx_new), _ptr(da), got["dx"].data_ptr(), _ptr(got.get("dy")), _ptr(got.get("gate")),
               _ptr(got.get("post_weight")), _ptr(got.get("post_bias")), _ptr(got.get("pre_weight")), _ptr(got.get("pre_bias")), *sides, rows, per_gate, D, residual_scale)
     size = _fn("dic_gated_norm_ws_bytes")(code, _NORM.pack(*fields, 0, 0))
     ws = x_new.new_empty(size, dtype=torch.uint8) if size else None

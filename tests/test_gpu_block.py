@@ -741,3 +741,68 @@ def test_refused_arguments():
     for kw in (dict(da=None), dict(pre=None), dict(saved=saved[:3]), dict(y=x.to(BF16)), dict(dx_new=x[:2]), dict(dx_new=None, da=None, pre=None)):
         with pytest.raises((ValueError, TypeError)):
             dic.gated_norm_grad(**{**dict(dx_new=x, da=x, x_new=x_new, y=x, saved=saved, pre=n), **kw})
+
+
+class Number:
+    def __float__(self):
+        return 0.5
+
+
+def test_numbers_that_do_not_fit_are_refused_by_name():
+    """ValueError or TypeError, never another exception and never a copy to the host; whole numbers and reals of any kind are taken."""
+    q = torch.randn(1, 40, 2, 64, device="cuda")
+    x = torch.randn(4, 6, 96, device="cuda")
+    n = dic.NormParams("layer", torch.ones(96, device="cuda"))
+    on_gpu, leaf = torch.tensor(1.0, device="cuda"), torch.tensor(1.0, requires_grad=True)
+    import numpy as np
+    out, lse = dic.window_attention(q, q, q, scale=0.5, left=4, right=2, sinks=3)
+    x_new, a, saved = dic.gated_norm(x, x, pre=n, residual_scale=0.5)
+    wrong = ("0.5", b"1", None, [1.0], 1j, on_gpu, leaf, torch.ones(2), object(), 1e39, 10 ** 400, math.nan, math.inf, -math.inf)
+    with torch.cuda.device(q.device):
+        torch.cuda.set_sync_debug_mode("error")
+        try:
+            for bad in wrong:
+                calls = [lambda: dic.gated_norm(x, x, pre=n, residual_scale=bad), lambda: dic.gated_norm_grad(x, a, x_new, x, saved, pre=n, residual_scale=bad),
+                         lambda: dic.gated_norm(x, x, pre=n._replace(eps=bad)), lambda: dic.gated_norm_grad(x, a, x_new, x, saved, pre=n._replace(eps=bad))]
+                if bad is not None:
+                    for kw in (dict(scale=bad), dict(left=bad), dict(right=bad), dict(sinks=bad)):
+                        if type(bad) is not int or "scale" in kw:            # (a whole number, if a large one: no bound)
+                            calls += [lambda kw=kw: dic.window_attention(q, q, q, **kw), lambda kw=kw: dic.window_attention_grad(q, q, q, q, out, lse, **kw)]
+                for call in calls:
+                    with pytest.raises((ValueError, TypeError)):
+                        call()
+            for kw in (dict(left=2.5), dict(right=0.1), dict(sinks=7.5), dict(left=-0.5), dict(scale=-1), dict(scale=1e-60)):
+                with pytest.raises(ValueError):
+                    dic.window_attention(q, q, q, **kw)
+            with pytest.raises(ValueError):
+                dic.gated_norm(x, x, pre=n._replace(eps=-1e-6))
+            for post in (torch.ones(96, device="cuda"), "layer", ("layer", None, None, 1e-6), n._replace(kind=[1])):
+                with pytest.raises((ValueError, TypeError)):
+                    dic.gated_norm(x, x, post=post)
+            for half, four in ((np.float32(0.5), np.int64(4)), (torch.tensor(0.5), torch.tensor(4)), (np.float64(0.5), 4.0), (Number(), np.float32(4))):
+                again = dic.window_attention(q, q, q, scale=half, left=four, right=np.int32(2), sinks=3.0)
+                assert all(type(u) is torch.Tensor for u in again)
+                dic.gated_norm(x, x, pre=n, residual_scale=half)
+        finally:
+            torch.cuda.set_sync_debug_mode("default")
+    for u, v in zip(again, (out, lse)):
+        assert torch.equal(u, v)
+    everything, far = (dic.window_attention(q, q, q, left=b, right=b)[0] for b in (None, 10 ** 400))
+    assert torch.equal(everything, far)
+
+
+def test_tensors_without_memory_of_their_own_are_refused():
+    q, x, n = torch.randn(3, 1, 40, 2, 64, device="cuda"), torch.randn(3, 4, 96, device="cuda"), dic.NormParams("rms")
+    with pytest.raises((ValueError, TypeError)):
+        torch.func.vmap(lambda t: dic.window_attention(t, t, t)[0])(q)
+    with pytest.raises((ValueError, TypeError)):
+        torch.func.vmap(lambda t: dic.gated_norm(t, t, pre=n)[0])(x)
+    with pytest.raises((ValueError, TypeError)):
+        dic.gated_norm(x[0].to_sparse(), None, pre=n)
+    with pytest.raises((ValueError, TypeError)):
+        dic.window_attention(q[0].to_sparse(), q[0], q[0])
+    out, lse = dic.window_attention(q[0], q[0], q[0])
+    with pytest.raises((ValueError, TypeError)):
+        dic.window_attention_grad(out.to_sparse(), q[0], q[0], q[0], out, lse)
+    with pytest.raises((ValueError, TypeError)):
+        dic.window_attention(q[0, ..., :0], q[0, ..., :0], q[0, ..., :0])
