@@ -1,7 +1,8 @@
 """Operators of an encoder block over longer token rows than the reference's: attention in a sliding window whose first keys stay visible, and the norms
 before and after a block with its gate and the residual scale (csrc/wattn.hip, csrc/gnorm.hip; include/dic_hip.h states the formulas).
 
-As everywhere in this package there is no autograd: each forward call has a call that computes its gradients, and a tensor that asks for a gradient is refused.
+As everywhere in this package there is no autograd: each forward call has a call that computes its gradients, and a tensor that asks for a gradient or
+carries a forward-mode tangent is refused.
 Calls run on the current stream of the tensors' device, allocate what they return and their workspaces from torch's allocator, never synchronise, and can
 be captured into a graph.  Arguments that do not fit raise ValueError or TypeError before anything is launched."""
 from __future__ import annotations
@@ -11,6 +12,7 @@ import struct
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -69,6 +71,13 @@ def _on(t, like, name, dtypes, shape=None):
 def _unfit(e):
     """For what came up while the arguments were packed: sizes beyond 32 bits, and tensors that are sparse or inside a function transform."""
     return ValueError(f"a size that does not fit: {e}") if isinstance(e, struct.error) else TypeError(f"a tensor without memory of its own: {e}")
+
+
+def _no_tangents(*tensors):
+    """Inside forward-mode differentiation (forward_ad._current_level >= 0): a tangent would be dropped."""
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError("a tensor carries a forward-mode tangent: this package has no autograd, call the operator on its primal")
 
 
 def _ptr(t):
@@ -179,6 +188,8 @@ def window_attention(q, k, v, *, left=None, right=None, sinks=0, key_mask=None, 
     no bound.  A row that sees nothing gives zeros and lse = -inf.  `out`: write there instead of into a new tensor.
 
     One new token behind a cache: Tq = 1, kv_len = the cache's lengths with the new key in place, q_pos = kv_len - 1, right = 0."""
+    if forward_ad._current_level >= 0:
+        _no_tangents(q, k, v, out)
     strides, tail, code = _attention(q, k, v, left, right, sinks, key_mask, kv_len, q_pos, scale)
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
@@ -199,6 +210,8 @@ def window_attention(q, k, v, *, left=None, right=None, sinks=0, key_mask=None, 
 def window_attention_grad(dout, q, k, v, out, lse, *, left=None, right=None, sinks=0, key_mask=None, kv_len=None, q_pos=None, scale=None, grads=None):
     """(dq, dk, dv) of window_attention for the gradient `dout` of its output; the other arguments as they went into and came out of that call.
     `grads`: three tensors to write them into (views of a packed gradient, say).  dk and dv are summed over the query heads of each key head."""
+    if forward_ad._current_level >= 0:
+        _no_tangents(dout, q, k, v, out, lse)
     strides, tail, code = _attention(q, k, v, left, right, sinks, key_mask, kv_len, q_pos, scale)
     _on(dout, q, "dout", (q.dtype,), q.shape)
     _check_rows(out, q, "out", q.shape)
@@ -214,6 +227,8 @@ def window_attention_grad(dout, q, k, v, out, lse, *, left=None, right=None, sin
         dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
     else:
         dq, dk, dv = grads
+        if forward_ad._current_level >= 0:
+            _no_tangents(dq, dk, dv)
         for t, like, name in ((dq, q, "dq"), (dk, k, "dk"), (dv, k, "dv")):
             _check_rows(t, q, name, like.shape)
     ws_bytes = _fn("dic_win_attn_ws_bytes")
@@ -238,6 +253,10 @@ class NormParams(NamedTuple):
 
 
 _WEIGHT, _BIAS, _EPS = ({side: f"{side} {what}" for side in ("post", "pre")} for what in ("weight", "bias", "eps"))
+
+
+def _inside(norm):
+    return getattr(norm, "weight", None), getattr(norm, "bias", None), getattr(norm, "eps", None)
 
 
 def _norm(norm, like, D, side):
@@ -296,6 +315,8 @@ def gated_norm(x, y=None, *, post=None, gate=None, residual_scale=1.0, pre=None,
     norm; without pre, a is None).  gate: float32 [D], [N, D] (one row for each of N equal runs of rows: the sequences of [N, T, D]), or None.  `saved`
     [4, rows] holds the rows' statistics for gated_norm_grad.  Without y it is a stack's first norm: a = pre(residual_scale x), of type `dtype` (x's); at
     scale 1 x_new is then x itself."""
+    if forward_ad._current_level >= 0:
+        _no_tangents(x, y, gate, residual_scale, *_inside(post), *_inside(pre))
     _first(x, "x")
     inner = y.dtype if isinstance(y, torch.Tensor) else (dtype or x.dtype)
     code = _norm_code(x.dtype, inner)
@@ -325,6 +346,8 @@ def gated_norm(x, y=None, *, post=None, gate=None, residual_scale=1.0, pre=None,
 def gated_norm_grad(dx_new, da, x_new, y, saved, *, post=None, gate=None, residual_scale=1.0, pre=None):
     """Gradients of gated_norm as a dict: "dx", "dy", "gate", "post_weight", "post_bias", "pre_weight", "pre_bias", as far as there are such inputs.
     dx_new (None: zero) and da (None without pre) are the gradients of its outputs; x_new, y and saved as they went into and came out of that call."""
+    if forward_ad._current_level >= 0:
+        _no_tangents(dx_new, da, x_new, y, saved, gate, residual_scale, *_inside(post), *_inside(pre))
     _first(x_new, "x_new")
     given = y if y is not None else da
     inner = given.dtype if isinstance(given, torch.Tensor) else x_new.dtype

@@ -806,3 +806,27 @@ def test_tensors_without_memory_of_their_own_are_refused():
         dic.window_attention_grad(out.to_sparse(), q[0], q[0], q[0], out, lse)
     with pytest.raises((ValueError, TypeError)):
         dic.window_attention(q[0, ..., :0], q[0, ..., :0], q[0, ..., :0])
+
+
+def test_forward_mode_tangents_are_refused():
+    import torch.autograd.forward_ad as fw
+    q, x, w = torch.randn(1, 40, 2, 64, device="cuda"), torch.randn(4, 96, device="cuda"), torch.ones(96, device="cuda")
+    out, lse = dic.window_attention(q, q, q)
+    n = dic.NormParams("layer", w, w, 1e-5)
+    how = dict(post=n, gate=w, pre=n)
+    x_new, a, saved = dic.gated_norm(x, x, **how)
+    fwd, bwd = dict(q=q, k=q, v=q), dict(dout=out, q=q, k=q, v=q, out=out, lse=lse)
+    norm, back = dict(x=x, y=x, **how), dict(dx_new=x, da=a, x_new=x_new, y=x, saved=saved, **how)
+    with fw.dual_level():
+        dual = lambda t: fw.make_dual(t, torch.ones_like(t))                 # noqa: E731
+        for call, args in ((dic.window_attention, fwd), (dic.window_attention_grad, bwd), (dic.gated_norm, norm), (dic.gated_norm_grad, back)):
+            call(**args)                                                     # a level without tangents is no obstacle
+            for name, t in args.items():
+                given = [n._replace(weight=dual(w)), n._replace(bias=dual(w))] if t is n else [dual(t)]
+                for g in given:
+                    with pytest.raises(ValueError, match="tangent"):
+                        call(**{**args, name: g})
+        with pytest.raises(ValueError, match="tangent"):
+            dic.window_attention_grad(**bwd, grads=(dual(q), torch.empty_like(q), torch.empty_like(q)))
+    with pytest.raises((ValueError, TypeError)):
+        torch.func.jvp(lambda t: dic.gated_norm(t, x, **how)[0], (x,), (x,))
