@@ -34,6 +34,8 @@ EXPORTS = [
     "dic_lin_prep", "dic_lin_prep_ws_bytes", "dic_ln_fwd_cen", "dic_ln_bwd_cen", "dic_set_option", "dic_rank1_add",
     "dic_win_attn_fwd", "dic_win_attn_bwd", "dic_win_attn_ws_bytes", "dic_gated_norm_fwd", "dic_gated_norm_bwd", "dic_gated_norm_ws_bytes",
 ]
+# Entries that came without a change to what was there before, at the same version: a library loaded through DIC_HIP_LIB may be older, and what it has is used.
+LATER_EXPORTS = ("dic_win_attn_fwd", "dic_win_attn_bwd", "dic_win_attn_ws_bytes", "dic_gated_norm_fwd", "dic_gated_norm_bwd", "dic_gated_norm_ws_bytes")
 
 
 class GemmParams(C.Structure):
@@ -131,8 +133,8 @@ def lib():
                                "run __graft_entry__.build()")
         L = C.CDLL(_AB_LIB if _AB_LIB else LIB_PATH)
         for name in EXPORTS:
-            if not hasattr(L, name):
-                raise RuntimeError(f"{LIB_PATH} does not export {name}")
+            if not hasattr(L, name) and not (_AB_LIB and name in LATER_EXPORTS):
+                raise RuntimeError(f"{_AB_LIB or LIB_PATH} does not export {name}")
         L.dic_last_error.restype = C.c_char_p
         if L.dic_version() != ABI_VERSION:
             raise RuntimeError(f"{_AB_LIB or LIB_PATH} reports ABI version {L.dic_version()}, this binding was written for {ABI_VERSION} "
@@ -198,14 +200,11 @@ def lib():
         L.dic_adamw_hl.argtypes = [P, P, P, P, P, P, I64, F, F, F, F, F, F, F, F, P]
         L.dic_cast_bf16_hl.argtypes = [P, P, P, I64, P]
         L.dic_probe_tr16.argtypes = [P, P, P]
-        for fn in ("dic_win_attn_fwd", "dic_win_attn_bwd"):
-            getattr(L, fn).argtypes = [I, C.POINTER(WinAttnParams), P]
-        for fn in ("dic_gated_norm_fwd", "dic_gated_norm_bwd"):
-            getattr(L, fn).argtypes = [I, C.POINTER(GatedNormParams), P]
-        L.dic_win_attn_ws_bytes.argtypes = [I, I, C.POINTER(WinAttnParams)]
-        L.dic_win_attn_ws_bytes.restype = C.c_size_t
-        L.dic_gated_norm_ws_bytes.argtypes = [I, C.POINTER(GatedNormParams)]
-        L.dic_gated_norm_ws_bytes.restype = C.c_size_t
+        for fn in LATER_EXPORTS:
+            if hasattr(L, fn):
+                params = C.POINTER(WinAttnParams if "win_attn" in fn else GatedNormParams)
+                getattr(L, fn).argtypes = [I, params, P] if not fn.endswith("ws_bytes") else [I, I, params] if "win_attn" in fn else [I, params]
+                getattr(L, fn).restype = C.c_size_t if fn.endswith("ws_bytes") else I
         L.dic_gemm_set_variant.argtypes = [I]
         L.dic_set_option.argtypes = [C.c_char_p, I]
         L.dic_gemm_set_w4a.argtypes = [I]
@@ -218,6 +217,14 @@ def lib():
         options.push_to_library(L)          # the library reads no environment: its process-global switches come from the one record
         _lib = L
     return _lib
+
+
+def entry(name):
+    """A C entry as an object of its own (argument types set on it are seen by nobody else)."""
+    try:
+        return lib()[name]
+    except AttributeError:
+        raise RuntimeError(f"{_AB_LIB or LIB_PATH} does not export {name}: an older build, which has other operators only") from None
 
 
 def loaded() -> bool:

@@ -31,7 +31,7 @@ def _fn(name):
     """A C entry that takes its params as bytes."""
     f = _fns.get(name)
     if f is None:
-        f = _lib.lib()[name]
+        f = _lib.entry(name)
         f.argtypes = [C.c_int, C.c_int, C.c_char_p] if name == "dic_win_attn_ws_bytes" else [C.c_int, C.c_char_p] if name.endswith("ws_bytes") else [C.c_int, C.c_char_p, C.c_void_p]
         f.restype = C.c_size_t if name.endswith("ws_bytes") else C.c_int
         _fns[name] = f

@@ -258,3 +258,26 @@ def test_norms_refuse_missing_pointers():
     for dtype in (-1, 2, 0x200):
         assert L.dic_gated_norm_fwd(dtype, C.byref(norms()), None) == 1001
     assert L.dic_gated_norm_fwd(0, None, None) == 1001
+
+
+def test_an_older_library_can_be_loaded_for_a_comparison(tmp_path):
+    """DIC_HIP_LIB with a library of the same version that has no such entries (a stand-in built here): it loads, and a call of one names the file."""
+    import subprocess
+    import sys
+    older = [n for n in dic._lib.EXPORTS if n not in dic._lib.LATER_EXPORTS]
+    assert set(dic._lib.LATER_EXPORTS) < set(dic._lib.EXPORTS)
+
+    def build(path, names):
+        src = tmp_path / "stub.c"
+        src.write_text("".join("const char* %s(void) { return \"\"; }\n" % n if n == "dic_last_error" else
+                               "int %s(void) { return %d; }\n" % (n, dic._lib.ABI_VERSION if n == "dic_version" else 0) for n in names))
+        subprocess.run(["gcc", "-shared", "-fPIC", "-o", str(path), str(src)], check=True)
+        code = ("import importlib\ndic = importlib.import_module('diffusion-image-captioning_amd')\nL = dic.lib()\nassert L.dic_version() == %d\n"
+                "from importlib import import_module\nblock = import_module('diffusion-image-captioning_amd.block')\nblock._fn('dic_win_attn_fwd')" % dic._lib.ABI_VERSION)
+        run = subprocess.run([sys.executable, "-c", code], cwd=ROOT, env={**os.environ, "DIC_HIP_LIB": str(path)}, capture_output=True, text=True)
+        return run.stderr
+
+    said = build(tmp_path / "older.so", older)
+    assert "older.so does not export dic_win_attn_fwd: an older build" in said, said
+    said = build(tmp_path / "broken.so", [n for n in older if n != "dic_gemm"])
+    assert "broken.so does not export dic_gemm" in said and "an older build" not in said, said
