@@ -86,10 +86,10 @@ LAST_BUILD = None        # "compiled" | "reused": what the last build() call did
 
 def build(verbose: bool = False, force: bool = False) -> str:
     """Compile every HIP source for gfx950 into one shared library, in-tree (it travels with the snapshot).
-    force: compile even when the library is newer than every source (the driver's "does it build" check must compile, not trust mtimes)."""
+    force: compile even when the library is newer than every source and this file, which holds the flags (the driver's "does it build" check must compile, not trust mtimes)."""
     global LAST_BUILD
     srcs = [os.path.join(CSRC, s) for s in SOURCES]
-    deps = srcs + [os.path.join(CSRC, h) for h in ("common.h", "gemm_w4a.h", "gemm_w4a_asm.inc", "gemm_w4n.h", "gemm_w4n_asm.inc")] + [os.path.join(os.path.dirname(HERE), "include", "dic_hip.h")]
+    deps = srcs + [os.path.abspath(__file__)] + [os.path.join(CSRC, h) for h in ("common.h", "gemm_w4a.h", "gemm_w4a_asm.inc", "gemm_w4n.h", "gemm_w4n_asm.inc")] + [os.path.join(os.path.dirname(HERE), "include", "dic_hip.h")]
     if not force and os.path.exists(LIB_PATH) and all(os.path.getmtime(LIB_PATH) >= os.path.getmtime(d) for d in deps):
         LAST_BUILD = "reused"
         return LIB_PATH

@@ -281,3 +281,25 @@ def test_an_older_library_can_be_loaded_for_a_comparison(tmp_path):
     assert "older.so does not export dic_win_attn_fwd: an older build" in said, said
     said = build(tmp_path / "broken.so", [n for n in older if n != "dic_gemm"])
     assert "broken.so does not export dic_gemm" in said and "an older build" not in said, said
+
+
+def test_a_library_older_than_the_flags_is_not_reused(monkeypatch):
+    """The flags decide which instructions the kernels hold, and stand in _lib.py."""
+    class Compiles(Exception):
+        pass
+
+    def popen(*_, **__):
+        raise Compiles
+
+    lib = dic._lib
+    monkeypatch.setattr(lib.subprocess, "Popen", popen)
+    monkeypatch.setattr(lib, "LAST_BUILD", None)
+    monkeypatch.setattr(lib.os.path, "exists", lambda p: True)
+    times = {lib.LIB_PATH: 2.0}
+    monkeypatch.setattr(lib.os.path, "getmtime", lambda p: times.get(p, 1.0))
+    assert lib.build() == lib.LIB_PATH and lib.LAST_BUILD == "reused"
+    for newer in (os.path.abspath(lib.__file__), os.path.join(lib.CSRC, "wattn.hip"), os.path.join(ROOT, "include", "dic_hip.h")):
+        times[newer] = 3.0
+        with pytest.raises(Compiles):
+            lib.build()
+        del times[newer]
