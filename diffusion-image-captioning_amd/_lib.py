@@ -84,6 +84,18 @@ class GatedNormParams(C.Structure):
 LAST_BUILD = None        # "compiled" | "reused": what the last build() call did (printed by __graft_entry__.build)
 
 
+def compile_command(source: str, obj: str, extra=()) -> list:
+    """The command that compiles one of SOURCES into `obj`."""
+    cmd = [os.environ.get("HIPCC", "/opt/rocm/bin/hipcc"), "--offload-arch=gfx950", "-O3", "-std=c++20", "-fPIC", "-Wno-unused-value", *extra, "-c", os.path.join(CSRC, source), "-o", obj]
+    if source == "misc.hip":
+        # q_sample must round a*x, eps*b and their sum separately to be bit-exact with the reference (ref :360-362);
+        # everything in misc.hip is HBM-bound, so no FMA contraction in this file costs nothing
+        cmd.insert(3, "-ffp-contract=off")
+    if source in NO_PACKED_F32_SOURCES:
+        cmd[3:3] = NO_PACKED_F32
+    return cmd
+
+
 def build(verbose: bool = False, force: bool = False) -> str:
     """Compile every HIP source for gfx950 into one shared library, in-tree (it travels with the snapshot).
     force: compile even when the library is newer than every source and this file, which holds the flags (the driver's "does it build" check must compile, not trust mtimes)."""
@@ -100,13 +112,7 @@ def build(verbose: bool = False, force: bool = False) -> str:
     for s in srcs:
         o = s[:-4] + ".o"
         objs.append(o)
-        cmd = [hipcc, "--offload-arch=gfx950", "-O3", "-std=c++20", "-fPIC", "-Wno-unused-value", "-c", s, "-o", o]
-        if s.endswith("misc.hip"):
-            # q_sample must round a*x, eps*b and their sum separately to be bit-exact with the reference (ref :360-362);
-            # everything in misc.hip is HBM-bound, so no FMA contraction in this file costs nothing
-            cmd.insert(3, "-ffp-contract=off")
-        if os.path.basename(s) in NO_PACKED_F32_SOURCES:
-            cmd[3:3] = NO_PACKED_F32
+        cmd = compile_command(os.path.basename(s), o)
         procs.append((cmd, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)))
     for cmd, p in procs:
         out, _ = p.communicate()

@@ -5,14 +5,22 @@ set -e
 R=$(cd "$(dirname "$0")/.." && pwd)
 NAME=$1; FLAGS=$2
 mkdir -p $R/abl/obj_$NAME
-C=$R/diffusion-image-captioning_amd/csrc
+cd $R
+# one line per source: its compile command with the flags of the shipped build (_lib.py)
+python - $R/abl/obj_$NAME $FLAGS > $R/abl/obj_$NAME/commands <<'END'
+import importlib, os, shlex, sys
+lib = importlib.import_module("diffusion-image-captioning_amd._lib")
+for s in lib.SOURCES:
+    print(shlex.join(lib.compile_command(s, os.path.join(sys.argv[1], s[:-4] + ".o"), sys.argv[2:])))
+END
 pids=""
-for f in gemm attn norm misc; do
-  extra=""; [ $f = misc ] && extra="-ffp-contract=off"
-  /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 $extra -std=c++20 -fPIC -Wno-unused-value $FLAGS -c $C/$f.hip -o $R/abl/obj_$NAME/$f.o 2> $R/abl/obj_$NAME/$f.log &
+n=0
+while read -r cmd; do
+  n=$((n + 1))
+  eval "$cmd" 2> $R/abl/obj_$NAME/$n.log < /dev/null &
   pids="$pids $!"
-done
+done < $R/abl/obj_$NAME/commands
 for p in $pids; do wait $p || { echo "build_variant.sh $NAME: a compile FAILED:"; grep -h -A3 "error" $R/abl/obj_$NAME/*.log | head -20; exit 1; }; done      # (a bare `wait` hides a failed compile: round 6 found a 0.5 MB "library" without its GEMMs)
-/opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -o $R/abl/libdic_$NAME.so $R/abl/obj_$NAME/*.o
+${HIPCC:-/opt/rocm/bin/hipcc} --offload-arch=gfx950 -shared -fPIC -o $R/abl/libdic_$NAME.so $R/abl/obj_$NAME/*.o
 rm -rf $R/abl/obj_$NAME
 ls -la $R/abl/libdic_$NAME.so

@@ -303,3 +303,24 @@ def test_a_library_older_than_the_flags_is_not_reused(monkeypatch):
         with pytest.raises(Compiles):
             lib.build()
         del times[newer]
+
+
+def test_the_script_for_variants_builds_every_source_with_its_flags(tmp_path):
+    """scripts/build_variant.sh in a copy of the tree's layout, with a compiler that writes down how it is called."""
+    import shutil
+    import subprocess
+    root, log = tmp_path / "tree", tmp_path / "calls"
+    (root / "scripts").mkdir(parents=True)
+    shutil.copy(os.path.join(ROOT, "scripts", "build_variant.sh"), root / "scripts")
+    os.symlink(os.path.dirname(dic._lib.__file__), root / "diffusion-image-captioning_amd")
+    hipcc = tmp_path / "hipcc"
+    hipcc.write_text('#!/bin/bash\necho "$@" >> %s\nwhile [ $# -gt 0 ]; do if [ "$1" = -o ]; then touch "$2"; fi; shift; done\n' % log)
+    hipcc.chmod(0o755)
+    run = subprocess.run(["bash", str(root / "scripts" / "build_variant.sh"), "x", "-DONE -DTWO=2"], env={**os.environ, "HIPCC": str(hipcc)}, capture_output=True, text=True)
+    assert run.returncode == 0 and (root / "abl" / "libdic_x.so").exists(), run.stderr
+    calls = log.read_text().splitlines()
+    for s in dic._lib.SOURCES:
+        call, = (c for c in calls if f"/{s} " in c)
+        assert "-DONE -DTWO=2" in call and ("-packed-fp32-ops" in call) == (s in dic._lib.NO_PACKED_F32_SOURCES) and ("-ffp-contract=off" in call) == (s == "misc.hip"), call
+    link, = (c for c in calls if "-shared" in c)
+    assert all(f"/{s[:-4]}.o" in link for s in dic._lib.SOURCES)
