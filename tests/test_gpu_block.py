@@ -193,6 +193,37 @@ def test_keys_that_nobody_may_see_are_not_read_into_results(dtype, Tq):
             run_both(dtype, (N, Tq, Tk, 4, 2, 64, left, right, 2), key_mask=key_mask, kv_len=kv_len, spoil=True)
 
 
+WIDE = {
+    # N, Tq, Tk, H, Hkv, dh, left, right, sinks: spans of more than 2000 keys, in many workgroups (of 128 wide rows: tiles of 32 keys) and in few
+    "many workgroups, window": (5, 140, 2600, 26, 13, 128, 2100, 30, 5), "many workgroups, causal": (5, 140, 2600, 26, 2, 128, None, 0, 0),
+    "many workgroups, sinks over a tile": (5, 129, 2500, 26, 26, 128, 2060, 0, 70), "many workgroups, 64 wide": (5, 140, 2600, 26, 13, 64, 2100, 30, 5),
+    "few workgroups": (5, 140, 2600, 2, 1, 128, 2100, 30, 5), "few rows": (5, 4, 2600, 8, 1, 128, 2100, 30, 5), "whole text": (1, 2300, 2300, 2, 1, 128, 2060, 0, 3),
+}
+
+
+@pytest.mark.parametrize("hidden", ["nothing", "a mask", "lengths and positions", "all of them"])
+@pytest.mark.parametrize("case", WIDE)
+def test_wide_windows_in_bf16(case, hidden):
+    """Besides the bounds, which are wide here, the norms: P or ds, the result, and with dq and dk `out` behind delta are rounded, each by at most h = 2^-8 and, evenly
+    spread, h / sqrt 3 in the mean square: h together.  A key too many or too few at the edge of n changes a row by about 1 / sqrt n of its norm, 0.02 here."""
+    N, Tq, Tk, Hq, Hkv, dh, left, right, sinks = WIDE[case]
+    g = torch.Generator(device="cuda").manual_seed(Tq + dh)
+    q, k, v, dout = (torch.randn(N, t, n, dh, generator=g, device="cuda").to(BF16) for t, n in ((Tq, Hq), (Tk, Hkv), (Tk, Hkv), (Tq, Hq)))
+    mask = torch.rand(N, Tk, generator=g, device="cuda") < 0.9 if hidden in ("a mask", "all of them") else None
+    lens, pos = None, torch.full((N,), Tk - Tq, dtype=torch.int32, device="cuda")
+    if hidden in ("lengths and positions", "all of them"):
+        lens = torch.tensor([Tk, Tk - 1, Tk - 33, Tk - 64, Tk // 2][:N], dtype=torch.int32, device="cuda")
+        pos = torch.tensor([Tk - Tq, Tk - Tq - 1, Tk - Tq - 40, 0, Tk // 2 - Tq][:N], dtype=torch.int32, device="cuda")
+    how = dict(left=left, right=right, sinks=sinks, key_mask=mask, kv_len=lens, q_pos=pos)
+    want = definition(q, k, v, visible(N, Tq, Tk, left, right, sinks, mask, lens, pos), dh ** -0.5, dout)
+    out, lse = dic.window_attention(q, k, v, **how)
+    for name, t in zip(("out", "lse", "dq", "dk", "dv"), (out, lse, *dic.window_attention_grad(dout, q, k, v, out, lse, **how))):
+        holds(name, t, want[name])
+        if name != "lse":
+            value = want[name][0]
+            assert float((t.double() - value).norm() / value.norm()) < 2.0 ** -8, name
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("N,H,dh", [(24, 8, 64), (24, 6, 128), (3, 2, 64), (3, 2, 128)])
 def test_many_and_few_workgroups_with_masks_lengths_and_positions(dtype, N, H, dh):
