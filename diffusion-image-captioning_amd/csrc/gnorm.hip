@@ -239,7 +239,9 @@ __global__ __launch_bounds__((Team<TPR, NV>::THREADS)) void gated_norm_fwd_kerne
 
 // A workgroup walks consecutive pieces (ONE: it has one); its teams take the rows of a piece in turn.  Column sums: d and d u over a piece give that
 // piece's share of the gate's gradient (w sum(d u) + b sum(d), folded over the teams through LDS), and, times the gate, of the post norm's weight and bias.
-// 17408 rows of 768, fp32 stream, bf16 blocks: 247 MB in 60 us, 4.1 TB/s, and 5 us for the fold; 8200 rows of 2048 in fp32: 403 MB in 90 us, 4.5 TB/s.
+// 17408 rows of 768, fp32 stream, bf16 blocks: 247 MB in 60 us, 4.1 TB/s, and 5 us for the fold; 8200 rows of 2048 in fp32: 403 MB in 93 us, 4.3 TB/s.
+// Above 4096 columns a row's operands, column sums and vectors are more than the 128 registers that 16 waves leave each: 17 to 29 are spilled in fp32, 70 to 99
+// with bf16 blocks (2052 rows of 8192: 119 us in fp32, 147 in bf16, 150 beside an fp32 stream; a copy's rate would be 84, 42 and 63).
 template <typename T, typename TX, int TPR, int NV, bool ONE>
 __global__ __launch_bounds__((Team<TPR, NV>::THREADS)) void gated_norm_bwd_kernel(const NormArgs p) {
     using TM = Team<TPR, NV>;

@@ -208,8 +208,10 @@ template <typename T, int DH> __device__ __forceinline__ void store_row(const f3
         for (int r = 0; r < 16; r += 4) Mma<T>::st4(to + 32 * d + tok(r, hi), acc[d][r] * mul, acc[d][r + 1] * mul, acc[d][r + 2] * mul, acc[d][r + 3] * mul);
 }
 // The same through LDS (32 rows of ROWB + 16 bytes, the wave's own) into 32 rows, `rows` of them real: a store instruction then writes whole rows instead of
-// 16 bytes of each of 32.  It takes registers and a barrier, and pays in the dk / dv kernel for 128 wide bf16 rows alone (205 -> 187 us at 2 x 4096 keys, 16
-// heads; 117 -> 126 us for 64 wide rows; forward and dq, any type: no difference).
+// 16 bytes of each of 32.  It takes registers and a barrier.  In the dk / dv kernel of 128 wide bf16 rows it pays where a workgroup has all keys of a head (whole
+// backward passes: 600 key heads of 256 keys 256 us, without it 267; of 200 keys 244 and 254) and costs 1 to 3 per cent where it has four waves (4 x 2048
+// rows, 16 query and 4 key heads: 417 and 405; the kernel alone at 2 x 4096 keys in windows of 1024: 169 and 165).  64 wide rows lose by it (117 -> 126 us);
+// forward and dq, any type: no difference.
 template <typename T, int DH> constexpr int OUT_ROW = Lay<T, DH>::ROWB + 16;
 template <typename T, int DH> constexpr bool WHOLE_ROWS = sizeof(T) == 2 && DH == 128;
 template <typename T, int DH>
@@ -354,11 +356,13 @@ template <typename T, int DH, int BN, int NW, int KS> struct KeyTiles {
 };
 
 // ------------------------------------------------------------------------------------------------ forward
-// One pass over the keys with the running maximum and sum per query.  P is rounded to bf16 in front of its product, relative to its size, and the sums are fp32.
+// One pass over the keys with the running maximum and sum per query.  P is rounded to bf16 in front of its product, relative to its size, and the sums are fp32
+// (l of the unrounded P: a product of bf16 operands is what the matrix unit has, and each P is off by half a step at most, evenly to both sides).
 // Long spans are bound by the issue of matrix and vector instructions together (a 32 x 32 block is 16 of the former at 32 cycles a SIMD, and some 450 cycles of
-// exponentials, masks, maxima and conversions; two or three waves a SIMD overlap them in part): 8192 rows that see 4096 keys, 16 heads of 128: 240 us, 860
-// TFLOP/s of visible pairs, where a library matrix product reaches 1350; in windows of 1024, 2 x 4096 rows: 95 us, 630.  Short ones are bound by moving their
-// rows with little to compute meanwhile: 256 x 12 heads of 130 x 64: 197 MB in 67 us, 2.9 TB/s.  8 x 2050 rows in windows of 513, 12 heads of 64: 51 us.
+// exponentials, masks, maxima and conversions; two or three waves a SIMD overlap them in part): 8192 rows that see 4096 keys, 16 heads of 128: 250 us, 825
+// TFLOP/s of visible pairs, where a library matrix product reaches 1350; in windows of 1024, 2 x 4096 rows: 90 us, 670.  The matrix unit is busy 41 and 34 per
+// cent of the CUs' time there, LDS reads 22 and 18, without a bank conflict: neither is the limit by itself.  Short ones are bound by moving their rows with
+// little to compute meanwhile: 256 x 12 heads of 130 x 64: 197 MB in 66 us, 3.0 TB/s.  8 x 2050 rows in windows of 513, 12 heads of 64: 51 us.
 template <typename T, int DH, int BN, int NW, int KS>
 __global__ __launch_bounds__(64 * MOST_WAVES<T>, (DH == 128 && BN == 32 && sizeof(T) == 2 ? 3 : RESIDENT<T, DH, 4>)) void win_fwd_kernel(const WinArgs a) {
     using L = Lay<T, DH>;
@@ -493,9 +497,11 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (DH == 128 && BN == 32 && sizeo
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dq (and delta)
-// Rows that see at most FEW_KEYS keys get the exact delta (dq_block): those of narrow windows and the first ones of a causal text, whose gradients are the
-// largest.  Beyond that it changes less than a tenth of the rounding errors, and costs a third more products.  Carrying both forms costs the plain one its best
-// schedule: 139 us for 130 (2 x 4096 rows, 16 heads of 128, windows of 1024), where a branch inside of one loop took 153.
+// Rows that see at most FEW_KEYS keys get the exact delta (dq_block): those of narrow windows and masks and the first ones of a causal text, whose gradients
+// are the largest.  Beyond that, with logits of deviation 1, it changes less than a tenth of the rounding errors; where the weight of such a row rests on a few of
+// its keys all the same, the rounded `out` shows (logits of deviation 5 over up to 900 keys: dq 3.7e-3 and dk 3.4e-3 of the norm off), as it is when `out` is all
+// that the forward pass keeps.  The exact form costs a third more products, and carrying both the plain one its best schedule: 126 us for 121 (2 x 4096 rows,
+// 16 heads of 128, windows of 1024), where a branch inside of one loop cost more.
 template <typename T> constexpr bool BF16 = sizeof(T) == 2;
 constexpr int FEW_KEYS = 256;
 template <int ND> __device__ __forceinline__ float exactly(f32x16 (&acc)[ND], const f32x16 (&mean)[ND], float off) {        // acc with the exact delta; returns off of the row
@@ -560,8 +566,8 @@ __device__ __forceinline__ void dq_block(const char* kt, const char* vt, const t
         if constexpr (EXACT) mean[d] = M::mac_t(t, M::right(st), mean[d]);
     }
 }
-// Bound as the forward pass is, with three products a block for its two.  2 x 4096 rows in windows of 1024, 16 heads of 128: 139 us, 650 TFLOP/s of visible
-// pairs; fp32, 4 x 513 rows in windows of 257, 12 heads of 64: 47 us.  ds is rounded to bf16 in front of its product.
+// Bound as the forward pass is, with three products a block for its two.  2 x 4096 rows in windows of 1024, 16 heads of 128: 126 us, 720 TFLOP/s of visible
+// pairs, 4 registers spilled; fp32, 4 x 513 rows in windows of 257, 12 heads of 64: 44 us.  ds is rounded to bf16 in front of its product.
 // The rows of one workgroup: query tile qt of query head h, key head hk, sequence n
 template <typename T, int DH, int BN, int NW, int KS, bool EXACT>
 __device__ __forceinline__ void dq_rows(const WinArgs& a, int n, int hk, int h, int qt, const Seq& sq, char* smem, unsigned long long* table) {
@@ -674,8 +680,9 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 3>)) void win_
 // Fragments of a key group's values (in the short kernel below: also of dout's rows) that stay in LDS instead of registers: at 128 wide bf16 rows the accumulators and both operands take all 256 registers
 // that two waves a SIMD leave each, and one that was reloaded from scratch memory in every turn made the turn wait for the next stage's DMA, too.
 template <typename T, int DH> constexpr int PARKED = sizeof(T) == 2 && DH == 128 ? 4 : 0;
-// Four products a block; P and ds are rounded to bf16 in front of theirs.  2 x 4096 rows in windows of 1024, 16 query and 4 key heads of 128: 187 us and 24 us
-// for the sinks, 570 TFLOP/s of visible pairs: the accumulators and both operands leave two waves to a SIMD, and loading and barriers alone take 120 us of it.
+// Four products a block; P and ds are rounded to bf16 in front of theirs.  2 x 4096 rows in windows of 1024, 16 query and 4 key heads of 128: 169 us and 23 us
+// for the sinks, 715 TFLOP/s of visible pairs: the accumulators and both operands leave two waves to a SIMD, and a wave of a 2 x 2 workgroup has one block
+// between two barriers.  The matrix unit is busy 33 per cent of the CUs' time, LDS reads 23.  (64 wide bf16 rows: 5 registers spilled.)
 // A workgroup owns kg groups of 32 keys and walks the queries that see them, 32 qh at a time: wave w takes key group w % kg and query rows 32 (w / kg).
 // The qh partial sums of a key group are added through LDS at the end.  A stage holds u of those row groups for each; all queries in one stage, and one
 // buffer, where they are few.
@@ -851,7 +858,7 @@ __global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 3>)) void win_
 
 // ------------------------------------------------------------------------------------------------ backward of short sequences
 // dk / scale and dv += the parts of 32 queries with the statistics st2; bit of `bits`: that query sees the lane's key.  (The dk / dv kernel above has the
-// same steps in its loop: as a call of this function its 128 wide form spilled 19 registers there and took 237 us for 187.)
+// same steps in its loop: as a call of this function its 128 wide form spilled 19 registers there and took a quarter longer.)
 template <typename T, int DH>
 __device__ __forceinline__ void dkv_block(const char* qt, const char* dt, const float* st2, const typename Mma<T>::Frag (&kf)[Lay<T, DH>::NF],
                                           const typename Mma<T>::Frag (&vf)[Lay<T, DH>::NF - PARKED<T, DH>], const char* parked, float c, unsigned bits, f32x16 (&dk)[DH / 32],
@@ -890,8 +897,8 @@ __device__ __forceinline__ void dkv_block(const char* qt, const char* dt, const 
     }
 }
 // One workgroup has a head's queries and keys whole, wave w queries 32 w.. and keys 32 w.., and reads them once: keys and values lie in LDS and the wave's
-// query rows in registers for dq; then they change places, and dk and dv follow without another read.  256 x 12 heads of 130 x 64 in bf16: 168 us (160
-// without the exact delta) for the two kernels' 202; 8 tensors of 51 MB at 2.4 TB/s, where moving them alone would take 90 us: of 130 rows the fifth wave's 30
+// query rows in registers for dq; then they change places, and dk and dv follow without another read.  256 x 12 heads of 130 x 64 in bf16: 160 us (8 less
+// without the exact delta), the two kernels 202; 8 tensors of 51 MB at 2.6 TB/s, where moving them alone would take 90 us: of 130 rows the fifth wave's 30
 // are padding, and two workgroups of five waves share a CU (bounded to 128 registers, for three, it spilled 23 and was 17 us slower).
 template <typename T, int DH>
 __global__ __launch_bounds__(64 * MOST_WAVES<T>, (RESIDENT<T, DH, 3>)) void win_bwd_short_kernel(const WinArgs a) {

@@ -297,8 +297,10 @@ int dic_attn_bwd(int dtype, const void* qkv, const uint8_t* key_mask, const void
  *     (j >= t - left (left >= 0)  or  j < sinks);                      left / right < 0: no bound on that side.
  * fwd: out = softmax(scale q k^T over the visible keys) v, lse [N][H][Tq] (optional) = the logarithm of the softmax's denominator.  A row that sees
  *     nothing gets out = 0 and lse = -inf.  A key that no row of its sequence sees (behind kv_len, masked by key_mask, outside of every window) reaches no
- *     result, whatever its rows of k and v hold.  (A row of q, k, v or dout that takes part and is not finite may reach results of other rows near it.)
- *     Sums, maxima and lse are fp32; with DIC_BF16 the probabilities are rounded to bf16 in front of the product with v.
+ *     result, whatever its rows of k and v hold.  (A key that some row sees and that is not finite may reach
+ *     results of other rows near it, and so may, in dk and dv, any row of q or dout that is not finite, one that sees nothing included.)
+ *     Sums, maxima and lse are fp32; with DIC_BF16 the probabilities are rounded to bf16 in front of the product with v (in bwd also with dout,
+ *     and ds in front of those with k and q).
  * bwd: dq, dk, dv from dout and the forward's out and lse; every row is written (zeros where nothing is seen).  Deterministic, no atomics.
  * No output (lse and ws are ones) may overlap an input or another output; rows of one packed tensor may lie between each other's.  kv_len is read as clamped to [0, Tk], q_pos to +-2^29 (bounds act as given beside it).  ws: dic_win_attn_ws_bytes(dtype, backward, p) bytes, 16-byte aligned, private to the call
  * until it has run; N, Tq or Tk may be 0.  A call is refused in front of any launch if one of its grids would need 2^32 threads (64 a wave for 32 rows of a head).   */
