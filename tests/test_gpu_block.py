@@ -619,6 +619,50 @@ def test_rows_at_any_alignment():
         assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("D", [768, 8192])
+def test_norms_of_more_than_2_31_elements(D):
+    """The last rows of a tensor whose offsets pass 2^31 elements: as when they are called for alone, bit for bit."""
+    rows, last = 2 ** 31 // D + 77, slice(-70, None)
+    g = torch.Generator(device="cuda").manual_seed(D)
+    x, y, dx_new, da = (torch.empty(1, rows, D, dtype=BF16, device="cuda").normal_(generator=g) for _ in range(4))
+    norm, gate = dic.NormParams("layer", torch.rand(D, device="cuda") + 0.5, torch.rand(D, device="cuda"), 1e-5), torch.rand(D, device="cuda")
+    how = dict(post=norm, pre=norm, gate=gate, residual_scale=0.9)
+    x_new, a, saved = dic.gated_norm(x, y, **how)
+    few = dic.gated_norm(x[:, last], y[:, last], **how)
+    for got, want in zip((x_new[:, last], a[:, last], saved[:, last]), few):
+        assert torch.equal(got, want)
+    back = dic.gated_norm_grad(dx_new, da, x_new, y, saved, **how)
+    alone = dic.gated_norm_grad(dx_new[:, last], da[:, last], few[0], y[:, last], few[2], **how)
+    for name in ("dx", "dy"):
+        assert torch.equal(back[name][:, last], alone[name]), name
+    # a column's sum of `rows` terms in fp32, in any order: off by at most rows 2^-24 of the sum of their sizes
+    d = da[0, :, -8:].double()
+    assert ((back["pre_bias"][-8:].double() - d.sum(0)).abs() <= rows * 2.0 ** -24 * d.abs().sum(0)).all()
+
+
+def test_sequences_of_a_cache_far_apart():
+    """Sequences 5 GiB apart and heads 2.2 GiB: the results of the same rows side by side, bit for bit."""
+    N, Tq, Tk, Hq, Hkv, dh = 3, 40, 100, 4, 2, 64
+    g = torch.Generator(device="cuda").manual_seed(2)
+    q, dout = (torch.randn(N, Tq, Hq, dh, generator=g, device="cuda").to(BF16) for _ in range(2))
+    k, v = (torch.randn(N, Tk, Hkv, dh, generator=g, device="cuda").to(BF16) for _ in range(2))
+    step_n, step_h = 5 << 29, 9 << 27
+    room = torch.empty(2 * step_n + step_h + Tk * 256, dtype=BF16, device="cuda")
+    far = [room.as_strided((N, Tk, Hkv, dh), (step_n, 256, step_h, 1), 64 * i) for i in range(4)]
+    far[0].copy_(k)
+    far[1].copy_(v)
+    for rows in (slice(0, Tq), slice(0, 2)):
+        how = dict(left=30, right=0, sinks=3, q_pos=torch.tensor([60, 10, 0], dtype=torch.int32, device="cuda"))
+        u, du = q[:, rows].contiguous(), dout[:, rows].contiguous()
+        out, lse = dic.window_attention(u, k, v, **how)
+        want = dic.window_attention_grad(du, u, k, v, out, lse, **how)
+        o2, l2 = dic.window_attention(u, *far[:2], **how)
+        d2 = torch.empty_like(u)
+        dic.window_attention_grad(du, u, *far[:2], o2, l2, grads=(d2, far[2], far[3]), **how)
+        for name, a, b in zip(("out", "lse", "dq", "dk", "dv"), (out, lse, *want), (o2, l2, d2, far[2], far[3])):
+            assert torch.equal(a, b), name
+
+
 # ------------------------------------------------------------------------------------------------ together, streams, graphs, refusals
 def block(q_w, o_w, x, how, post, pre, gate, heads):
     """norm -> q|k|v Linear -> attention -> Linear -> norm, gate, residual, next norm, forward and backward, as a layer's code calls them."""
