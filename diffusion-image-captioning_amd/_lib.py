@@ -1,7 +1,7 @@
 """Builds and loads `libdic_hip.so` (the C-ABI of include/dic_hip.h) and exposes thin ctypes callers.
 
 No CPU fallback exists: every op goes through the HIP library, and a missing library or missing GPU is a
-loud `RuntimeError` (the judge checks that GPU tests cannot pass on a silent eager path).
+loud `RuntimeError` (GPU tests cannot pass on a silent eager path).
 """
 from __future__ import annotations
 
@@ -98,7 +98,7 @@ def compile_command(source: str, obj: str, extra=()) -> list:
 
 def build(verbose: bool = False, force: bool = False) -> str:
     """Compile every HIP source for gfx950 into one shared library, in-tree (it travels with the snapshot).
-    force: compile even when the library is newer than every source and this file, which holds the flags (the driver's "does it build" check must compile, not trust mtimes)."""
+    force: compile even when the library is newer than every source and this file, which holds the flags (a check that everything builds must compile, not trust mtimes)."""
     global LAST_BUILD
     srcs = [os.path.join(CSRC, s) for s in SOURCES]
     deps = srcs + [os.path.abspath(__file__)] + [os.path.join(CSRC, h) for h in ("common.h", "gemm_w4a.h", "gemm_w4a_asm.inc", "gemm_w4n.h", "gemm_w4n_asm.inc")] + [os.path.join(os.path.dirname(HERE), "include", "dic_hip.h")]
